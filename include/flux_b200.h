@@ -207,6 +207,91 @@ int32_t fb_qk_norm_rope(const uint16_t* qkv, int64_t ld_qkv, int32_t batch, int3
                         const float* rope_sin, uint16_t* q, uint16_t* k, uint16_t* v, int32_t seq_total,
                         int32_t seq_offset, void* stream);
 
+/* ---- token-wise operators for blocks other than the fixed FLUX ones: rotary positions from position ids, layer
+ * norm with its backward pass, and a Linear with activation and residual. Types are fb_dtype; sums and statistics
+ * are held in 32 bits, and each output is rounded once. */
+
+enum fb_ids_type { FB_IDS_F32 = 0, FB_IDS_F64 = 1, FB_IDS_I32 = 2, FB_IDS_I64 = 3 };
+enum fb_rope_pairs {
+  FB_ROPE_INTERLEAVED = 0,   /* slot s turns the elements (2s, 2s + 1) of a head (selas/models/flux.py:117-121) */
+  FB_ROPE_HALVES = 1         /* slot s turns the elements (s, s + head_dim / 2) */
+};
+
+/* One tensor [batch, heads, seq, head_dim] (unit stride along head_dim) and where its rotation goes. out may be x with
+ * x's strides (in place); any other overlap is not allowed. */
+typedef struct fb_rope_tensor {
+  const void* x;
+  void* out;
+  int64_t x_stride_b, x_stride_h, x_stride_l;
+  int64_t out_stride_b, out_stride_h, out_stride_l;
+  int32_t heads;
+} fb_rope_tensor;
+
+/* Rotary positions with several axes, for 1 or 2 tensors (q and k, which may differ in heads) in one launch. Axis a owns
+ * axes_dim[a] / 2 slots with the frequencies theta[a]^(-2j / axes_dim[a]) (the order of rope_tables,
+ * selas/models/flux.py:106-114; the axes_dim add up to head_dim <= 512), turned by ids[b, l, a] times the frequency:
+ * no cos/sin table is made, and the angle is reduced in 64 bits. inverse != 0 turns the other way: the gradient. ids
+ * has strides ids_stride_b (0: one set for all images), _l and _a, in elements. */
+int32_t fb_rope_axes(const fb_rope_tensor* tensors, int32_t count, int32_t dtype, int32_t batch, int32_t seq,
+                     int32_t head_dim, const void* ids, int32_t ids_type, int64_t ids_stride_b, int64_t ids_stride_l,
+                     int64_t ids_stride_a, int32_t axes, const int32_t* axes_dim, const double* theta, int32_t pairs,
+                     int32_t inverse, void* stream);
+
+/* Layer norm of the rows of x [outer, inner, dim] (unit stride along dim; outer and inner strides in elements):
+ *   y  = xhat * w + bias,  xhat = (x - mean) / sqrt(var + eps),
+ * with w = weight, or 1 + weight (weight_plus_one, adaLN's scale), or 1 (weight NULL), and weight and bias shared by
+ * all rows (w_outer_stride 0) or one row per outer index.
+ * Backward (dy like x; x is normalised again, nothing is saved by the forward):
+ *   g = dy * w,  dx = (g - mean(g) - xhat * mean(g * xhat)) / sqrt(var + eps) [+ add],
+ *   dweight = sum of dy * xhat,  dbias = sum of dy   (fp32 [dim], or [outer, dim] with sum_per_outer; both or neither),
+ * summed in a fixed order through `work` (fb_layer_norm_work_floats floats). dx has x's type. */
+typedef struct fb_layer_norm_args {
+  const void* x; int64_t x_outer_stride, x_inner_stride;
+  const void* dy; int64_t dy_outer_stride, dy_inner_stride;        /* backward */
+  const void* add; int64_t add_outer_stride, add_inner_stride;     /* backward, x's type, or NULL */
+  void* out; int64_t out_outer_stride, out_inner_stride;           /* y (y_dtype), or dx (x_dtype) */
+  const void* weight; const void* bias; int64_t w_outer_stride;    /* w_dtype, or NULL */
+  float* dweight; float* dbias;                                    /* backward */
+  float* work; int64_t work_floats;                                /* backward with dweight */
+  int64_t outer, inner;
+  int32_t dim;
+  int32_t x_dtype, y_dtype, w_dtype;                               /* y_dtype: y, or dy */
+  int32_t weight_plus_one, sum_per_outer;
+  float eps;
+} fb_layer_norm_args;
+
+int32_t fb_layer_norm(const fb_layer_norm_args* args, void* stream);
+int32_t fb_layer_norm_backward(const fb_layer_norm_args* args, void* stream);
+int64_t fb_layer_norm_work_floats(int64_t outer, int64_t inner, int32_t dim, int32_t sum_per_outer);
+
+enum fb_act {
+  FB_ACT_NONE = 0,
+  FB_ACT_RELU = 1,
+  FB_ACT_GELU = 2,           /* z/2 (1 + erf(z / sqrt 2)) */
+  FB_ACT_GELU_TANH = 3,
+  FB_ACT_QUICK_GELU = 4,     /* z sigmoid(1.702 z) */
+  FB_ACT_SILU = 5            /* z sigmoid(z) */
+};
+
+/* out = act(x w^T + bias) + residual, on the fp32 accumulator with one rounding: x [m, k] and w [n, k] both bf16 or both
+ * fp16, bias [n] of their type or NULL, residual [m, n] of their type or fp32 or NULL, out of their type or fp32; unit
+ * stride along the last dim, row strides in elements, any m, n and k >= 0. residual may be out. x or w whose rows do
+ * not start on 16 bytes is copied to `work` first (fb_linear_act_work_bytes bytes, 16-byte aligned; 0 when both do). */
+typedef struct fb_linear_act_args {
+  const void* x; int64_t ldx;
+  const void* w; int64_t ldw;
+  const void* bias;
+  const void* residual; int64_t ld_residual;
+  void* out; int64_t ld_out;
+  void* work; int64_t work_bytes;
+  int32_t m, n, k;
+  int32_t dtype, residual_dtype, out_dtype;
+  int32_t act;
+} fb_linear_act_args;
+
+int32_t fb_linear_act(const fb_linear_act_args* args, void* stream);
+int64_t fb_linear_act_work_bytes(const fb_linear_act_args* args);
+
 /* ---- sequence parallelism over NVLink (Ulysses, one image; no counterpart in the reference, which has
  * no multi-GPU path). Buffers are shared between the ranks' processes with CUDA IPC; the two
  * all-to-alls of Ulysses attention are done by the kernels' own stores into the peers' buffers, with

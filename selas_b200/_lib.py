@@ -16,6 +16,9 @@ LIB_PATH = Path(__file__).resolve().parent / "lib" / "libflux_b200.so"
 FB_F32, FB_F16, FB_BF16 = 0, 1, 2
 FB_PROBE_WORK_DOUBLES = 4096
 FB_VAE_ROUND_OUT, FB_VAE_OUT_NCHW_CLAMP = 1, 2
+FB_IDS_F32, FB_IDS_F64, FB_IDS_I32, FB_IDS_I64 = range(4)
+FB_ROPE_INTERLEAVED, FB_ROPE_HALVES = range(2)
+FB_ACT_NONE, FB_ACT_RELU, FB_ACT_GELU, FB_ACT_GELU_TANH, FB_ACT_QUICK_GELU, FB_ACT_SILU = range(6)
 FB_EPI_STORE_BF16, FB_EPI_STORE_F32, FB_EPI_GELU, FB_EPI_GATED_RESIDUAL, FB_EPI_QKV = range(5)
 DEVICE_CODES = {0: "ok", 1: "timeout waiting for TMA", 2: "timeout waiting for tensor-core work",
                 3: "timeout waiting for epilogue/softmax warps", 4: "bad shape seen on the device",
@@ -59,6 +62,12 @@ SIGNATURES = {
     "fb_attention_split": ([_P, _P, _P, _P, _I64, _P, _I64, _I32, _I32, _I32, _I32, _I32, _F, _P], _I32),
     "fb_gated_add": ([_P, _P, _P, _P, _I64, _I32, _I32, _I64, _I32, _P], _I32),
     "fb_gelu_tanh": ([_P, _P, _I64, _P], _I32),
+    "fb_rope_axes": ([_P, _I32, _I32, _I32, _I32, _I32, _P, _I32, _I64, _I64, _I64, _I32, _P, _P, _I32, _I32, _P], _I32),
+    "fb_layer_norm": ([_P, _P], _I32),
+    "fb_layer_norm_backward": ([_P, _P], _I32),
+    "fb_layer_norm_work_floats": ([_I64, _I64, _I32, _I32], _I64),
+    "fb_linear_act": ([_P, _P], _I32),
+    "fb_linear_act_work_bytes": ([_P], _I64),
     "fb_qk_norm_rope": ([_P, _I64, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _P], _I32),
 }
 
@@ -72,6 +81,41 @@ class FbLnModProblem(ctypes.Structure):
 
     _fields_ = [("x", _P), ("rows", _I64), ("dim", _I32), ("rows_per_batch", _I32), ("shift", _P), ("scale", _P),
                 ("mod_batch_stride", _I64), ("out", _P)]
+
+
+class FbRopeTensor(ctypes.Structure):
+    """``fb_rope_tensor`` of include/flux_b200.h, field for field."""
+
+    _fields_ = [("x", _P), ("out", _P), ("x_stride_b", _I64), ("x_stride_h", _I64), ("x_stride_l", _I64),
+                ("out_stride_b", _I64), ("out_stride_h", _I64), ("out_stride_l", _I64), ("heads", _I32)]
+
+
+class FbLayerNormArgs(ctypes.Structure):
+    """``fb_layer_norm_args`` of include/flux_b200.h, field for field."""
+
+    _fields_ = [
+        ("x", _P), ("x_outer_stride", _I64), ("x_inner_stride", _I64),
+        ("dy", _P), ("dy_outer_stride", _I64), ("dy_inner_stride", _I64),
+        ("add", _P), ("add_outer_stride", _I64), ("add_inner_stride", _I64),
+        ("out", _P), ("out_outer_stride", _I64), ("out_inner_stride", _I64),
+        ("weight", _P), ("bias", _P), ("w_outer_stride", _I64),
+        ("dweight", _P), ("dbias", _P),
+        ("work", _P), ("work_floats", _I64),
+        ("outer", _I64), ("inner", _I64), ("dim", _I32),
+        ("x_dtype", _I32), ("y_dtype", _I32), ("w_dtype", _I32),
+        ("weight_plus_one", _I32), ("sum_per_outer", _I32), ("eps", _F),
+    ]
+
+
+class FbLinearActArgs(ctypes.Structure):
+    """``fb_linear_act_args`` of include/flux_b200.h, field for field."""
+
+    _fields_ = [
+        ("x", _P), ("ldx", _I64), ("w", _P), ("ldw", _I64), ("bias", _P), ("residual", _P), ("ld_residual", _I64),
+        ("out", _P), ("ld_out", _I64), ("work", _P), ("work_bytes", _I64),
+        ("m", _I32), ("n", _I32), ("k", _I32), ("dtype", _I32), ("residual_dtype", _I32), ("out_dtype", _I32),
+        ("act", _I32),
+    ]
 
 
 class FbLinear(ctypes.Structure):

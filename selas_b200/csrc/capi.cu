@@ -75,6 +75,7 @@ DeviceState* current_device(std::string& err) {
   }
   std::string msg = gemm_setup();
   if (msg.empty()) msg = attention_setup();
+  if (msg.empty()) msg = linear_act_setup();
   if (!msg.empty()) {
     err = msg;
     return nullptr;
@@ -104,6 +105,18 @@ DeviceState* current_device(std::string& err) {
 }  // namespace fb
 
 using namespace fb;
+
+// Runs `f(err)`, an FB_ERR_* code; a C++ exception (out of host memory) becomes an error code too.
+template <typename F>
+static int32_t guarded(const char* who, F f) {
+  try {
+    std::string err;
+    const int rc = f(err);
+    return rc ? fail(rc, err) : FB_OK;
+  } catch (...) {
+    return fail(FB_ERR_INIT, std::string(who) + ": host error");
+  }
+}
 
 extern "C" {
 
@@ -314,5 +327,46 @@ int32_t fb_qk_norm_rope(const uint16_t* qkv, int64_t ld_qkv, int32_t batch, int3
                                      q, k, v, seq_total, seq_offset, static_cast<cudaStream_t>(stream)),
                  "fb_qk_norm_rope");
 }
+
+int32_t fb_rope_axes(const fb_rope_tensor* tensors, int32_t count, int32_t dtype, int32_t batch, int32_t seq,
+                     int32_t head_dim, const void* ids, int32_t ids_type, int64_t ids_stride_b, int64_t ids_stride_l,
+                     int64_t ids_stride_a, int32_t axes, const int32_t* axes_dim, const double* theta, int32_t pairs,
+                     int32_t inverse, void* stream) {
+  if (int rc = ready_or_fail()) return rc;
+  return guarded("fb_rope_axes", [&](std::string& err) {
+    return launch_rope_axes(tensors, count, dtype, batch, seq, head_dim, ids, ids_type, ids_stride_b, ids_stride_l,
+                            ids_stride_a, axes, axes_dim, theta, pairs, inverse, static_cast<cudaStream_t>(stream), err);
+  });
+}
+
+int32_t fb_layer_norm(const fb_layer_norm_args* args, void* stream) {
+  if (int rc = ready_or_fail()) return rc;
+  if (!args) return fail(FB_ERR_ARG, "fb_layer_norm: null arguments");
+  return guarded("fb_layer_norm", [&](std::string& err) {
+    return launch_layer_norm(*args, false, static_cast<cudaStream_t>(stream), err);
+  });
+}
+
+int32_t fb_layer_norm_backward(const fb_layer_norm_args* args, void* stream) {
+  if (int rc = ready_or_fail()) return rc;
+  if (!args) return fail(FB_ERR_ARG, "fb_layer_norm_backward: null arguments");
+  return guarded("fb_layer_norm_backward", [&](std::string& err) {
+    return launch_layer_norm(*args, true, static_cast<cudaStream_t>(stream), err);
+  });
+}
+
+int64_t fb_layer_norm_work_floats(int64_t outer, int64_t inner, int32_t dim, int32_t sum_per_outer) {
+  return layer_norm_work_floats(outer, inner, dim, sum_per_outer);
+}
+
+int32_t fb_linear_act(const fb_linear_act_args* args, void* stream) {
+  if (int rc = ready_or_fail()) return rc;
+  if (!args) return fail(FB_ERR_ARG, "fb_linear_act: null arguments");
+  return guarded("fb_linear_act", [&](std::string& err) {
+    return launch_linear_act(*args, static_cast<cudaStream_t>(stream), err);
+  });
+}
+
+int64_t fb_linear_act_work_bytes(const fb_linear_act_args* args) { return args ? linear_act_work_bytes(*args) : 0; }
 
 }  // extern "C"

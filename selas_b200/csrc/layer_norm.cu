@@ -1,0 +1,591 @@
+// layer_norm.cu — layer norm with an affine map, and its backward pass with the gradients of the map, for plain norms
+// (one weight for every row) and for adaLN (weight 1 + scale[b], bias shift[b] per image).
+//
+//   forward   y  = xhat * w + b,  xhat = (x - mean) * rstd,  rstd = 1 / sqrt(var + eps)
+//   backward  g  = dy * w;  dx = rstd * (g - mean(g) - xhat * mean(g * xhat)) [+ add]
+//             dw = sum over rows of dy * xhat,  db = sum over rows of dy
+//
+// Bound: HBM. Every kernel reads each input once: a row stays in the registers of a group of threads between the
+// passes over it (mean first, then the squares of the centred values, so a large mean costs no precision), and the
+// backward pass works mean and rstd out again from x, which it has to read anyway, instead of reading saved ones. The
+// column sums dw and db stay in registers too (a thread owns the same columns of every row it takes), are joined
+// across the block's groups in shared memory, and go out as one fp32 partial row per block; a second kernel adds the
+// partials in a fixed order, so results do not depend on the order in which blocks run.
+#include "fb_internal.h"
+
+namespace fb {
+namespace norm {
+
+constexpr int kMaxDimRegs = 16384;  // the widest row that a group of 1024 threads holds in registers
+
+struct Args {
+  const void *x, *dy, *add;
+  void* out;  // y, or dx
+  const void *w, *b;
+  float *part, *dw, *db;  // partials [sum group][block][2][dim]; with one block per group dw and db are written directly
+  int64_t xo, xi, yo, yi, ao, ai, oo, oi;  // strides of x, dy, add, out: outer index, inner index (elements)
+  int64_t w_stride;                        // of w and b per outer index (0: shared)
+  int64_t rows;                            // rows of a sum group (forward: all rows)
+  int64_t inner;                           // row = outer * inner + index
+  int dim;
+  int x_type, y_type, w_type;              // fb_dtype; y_type: y (forward) or dy
+  float w_plus;                            // w is read as w_plus + w (1 for adaLN's scale)
+  float eps;
+};
+
+// CH consecutive elements (4: one vector access, 1: any alignment) widened to fp32.
+template <int CH>
+__device__ __forceinline__ void load_chunk(const void* p, int type, int64_t at, float* f) {
+  if (type == FB_F32) {
+    const float* s = static_cast<const float*>(p) + at;
+    if constexpr (CH == 4) {
+      const float4 v = __ldg(reinterpret_cast<const float4*>(s));
+      f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
+    } else {
+      f[0] = __ldg(s);
+    }
+  } else if (type == FB_BF16) {
+    const uint16_t* s = static_cast<const uint16_t*>(p) + at;
+    if constexpr (CH == 4) {
+      const uint2 u = __ldg(reinterpret_cast<const uint2*>(s));
+      f[0] = __uint_as_float(u.x << 16), f[1] = __uint_as_float(u.x & 0xFFFF0000u);
+      f[2] = __uint_as_float(u.y << 16), f[3] = __uint_as_float(u.y & 0xFFFF0000u);
+    } else {
+      f[0] = bf16_bits_to_f32(__ldg(s));
+    }
+  } else {
+    const __half* s = static_cast<const __half*>(p) + at;
+    if constexpr (CH == 4) {
+      const uint2 u = __ldg(reinterpret_cast<const uint2*>(s));
+      const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
+      const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+      f[0] = lo.x, f[1] = lo.y, f[2] = hi.x, f[3] = hi.y;
+    } else {
+      f[0] = __half2float(__ldg(s));
+    }
+  }
+}
+
+template <int CH>
+__device__ __forceinline__ void store_chunk(void* p, int type, int64_t at, const float* f) {
+  if (type == FB_F32) {
+    float* d = static_cast<float*>(p) + at;
+    if constexpr (CH == 4) {
+      *reinterpret_cast<float4*>(d) = make_float4(f[0], f[1], f[2], f[3]);
+    } else {
+      d[0] = f[0];
+    }
+  } else if (type == FB_BF16) {
+    uint16_t* d = static_cast<uint16_t*>(p) + at;
+    if constexpr (CH == 4) {
+      *reinterpret_cast<uint2*>(d) = make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
+    } else {
+      *reinterpret_cast<__nv_bfloat16*>(d) = __float2bfloat16_rn(f[0]);
+    }
+  } else {
+    __half* d = static_cast<__half*>(p) + at;
+    if constexpr (CH == 4) {
+      const __half2 lo = __floats2half2_rn(f[0], f[1]), hi = __floats2half2_rn(f[2], f[3]);
+      *reinterpret_cast<uint2*>(d) =
+          make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    } else {
+      d[0] = __float2half_rn(f[0]);
+    }
+  }
+}
+
+// The elements of a row that one thread of its group holds: NCH chunks of CH, chunk c at column CH * (t + GT * c);
+// zeros past the end. The type branch is outside the loop, so the loads of a row go out together.
+template <int GT, int NCH, int CH>
+__device__ __forceinline__ void load_row(const void* p, int type, int64_t base, int t, int dim, float (&f)[NCH * CH]) {
+  auto each = [&](int ty) {
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      const int col = CH * (t + GT * c);
+      if (col < dim) {
+        load_chunk<CH>(p, ty, base + col, f + CH * c);
+      } else {
+#pragma unroll
+        for (int j = 0; j < CH; ++j) f[CH * c + j] = 0.f;
+      }
+    }
+  };
+  if (type == FB_F32) {
+    each(FB_F32);
+  } else if (type == FB_BF16) {
+    each(FB_BF16);
+  } else {
+    each(FB_F16);
+  }
+}
+
+template <int GT, int NCH, int CH>
+__device__ __forceinline__ void store_row(void* p, int type, int64_t base, int t, int dim, const float (&f)[NCH * CH]) {
+  auto each = [&](int ty) {
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      const int col = CH * (t + GT * c);
+      if (col < dim) store_chunk<CH>(p, ty, base + col, f + CH * c);
+    }
+  };
+  if (type == FB_F32) {
+    each(FB_F32);
+  } else if (type == FB_BF16) {
+    each(FB_BF16);
+  } else {
+    each(FB_F16);
+  }
+}
+
+// Sums of two values over a group of GT threads (all of them get both). One warp: shuffles. More: one entry per warp
+// in shared memory and a barrier of the group's own; `buf` alternates between calls, so one barrier per sum is enough.
+template <int GT>
+__device__ __forceinline__ float2 group_sum2(float a, float b, int group, float2* slots, int& buf) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    a += __shfl_xor_sync(0xffffffffu, a, o);
+    b += __shfl_xor_sync(0xffffffffu, b, o);
+  }
+  if constexpr (GT == 32) return make_float2(a, b);
+  constexpr int W = GT / 32;
+  float2* s = slots + (buf * (blockDim.x / GT) + group) * W;
+  buf ^= 1;
+  const int warp = (threadIdx.x % GT) >> 5;
+  if ((threadIdx.x & 31) == 0) s[warp] = make_float2(a, b);
+  asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(GT) : "memory");
+  float2 r = s[0];
+#pragma unroll
+  for (int w = 1; w < W; ++w) r.x += s[w].x, r.y += s[w].y;
+  return r;
+}
+
+template <int GT>
+constexpr int block_threads() {
+  return GT < 256 ? 256 : GT;
+}
+
+// Forward: one group per row at a time.
+template <int GT, int NCH, int CH>
+__global__ void __launch_bounds__(block_threads<GT>()) fwd_kernel(const __grid_constant__ Args a) {
+  constexpr int E = NCH * CH, NG = block_threads<GT>() / GT;
+  __shared__ float2 slots[2 * NG * (GT / 32)];
+  const int group = threadIdx.x / GT, t = threadIdx.x % GT;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * NG + group;
+  if (row >= a.rows) return;  // whole groups
+  int buf = 0;
+  const int64_t o = row / a.inner, i = row - o * a.inner;
+  float x[E];
+  load_row<GT, NCH, CH>(a.x, a.x_type, o * a.xo + i * a.xi, t, a.dim, x);
+  const float inv = 1.0f / static_cast<float>(a.dim);
+  float s = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) s += x[e];
+  const float mean = group_sum2<GT>(s, 0.f, group, slots, buf).x * inv;
+  float q = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int col = CH * (t + GT * (e / CH));
+    x[e] = col < a.dim ? x[e] - mean : 0.f;
+    q += x[e] * x[e];
+  }
+  const float rstd = 1.0f / sqrtf(group_sum2<GT>(q, 0.f, group, slots, buf).x * inv + a.eps);
+  if (a.w != nullptr) {
+    float w[E];
+    load_row<GT, NCH, CH>(a.w, a.w_type, o * a.w_stride, t, a.dim, w);
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = x[e] * rstd * (a.w_plus + w[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] *= rstd;
+  }
+  if (a.b != nullptr) {
+    float b[E];
+    load_row<GT, NCH, CH>(a.b, a.w_type, o * a.w_stride, t, a.dim, b);
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] += b[e];
+  }
+  store_row<GT, NCH, CH>(a.out, a.y_type, o * a.oo + i * a.oi, t, a.dim, x);
+}
+
+// Backward: block p of sum group blockIdx.y takes every (gridDim.x * groups)-th row of it.
+template <int GT, int NCH, int CH>
+__global__ void __launch_bounds__(block_threads<GT>()) bwd_kernel(const __grid_constant__ Args a) {
+  constexpr int E = NCH * CH, T = block_threads<GT>(), NG = T / GT;
+  __shared__ float2 slots[2 * NG * (GT / 32)];
+  __shared__ float join[NG > 1 ? T * E : 1];
+  const int group = threadIdx.x / GT, t = threadIdx.x % GT;
+  const float inv = 1.0f / static_cast<float>(a.dim);
+  int buf = 0;
+  float dw[E], db[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.f;
+  const int64_t first = static_cast<int64_t>(blockIdx.y) * a.rows;
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * NG + group; r < a.rows; r += static_cast<int64_t>(gridDim.x) * NG) {
+    const int64_t row = first + r, o = row / a.inner, i = row - o * a.inner;
+    float x[E], g[E];
+    load_row<GT, NCH, CH>(a.x, a.x_type, o * a.xo + i * a.xi, t, a.dim, x);
+    load_row<GT, NCH, CH>(a.dy, a.y_type, o * a.yo + i * a.yi, t, a.dim, g);
+    float w[E];
+    if (a.w != nullptr) {
+      load_row<GT, NCH, CH>(a.w, a.w_type, o * a.w_stride, t, a.dim, w);
+#pragma unroll
+      for (int e = 0; e < E; ++e) w[e] += a.w_plus;
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) w[e] = 1.f;
+    }
+    float sx = 0.f, sg = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) sx += x[e], sg += g[e] * w[e];
+    const float2 m = group_sum2<GT>(sx, sg, group, slots, buf);
+    const float mean = m.x * inv, gmean = m.y * inv;
+    float qx = 0.f, qg = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int col = CH * (t + GT * (e / CH));
+      x[e] = col < a.dim ? x[e] - mean : 0.f;
+      qx += x[e] * x[e];
+      qg += g[e] * w[e] * x[e];
+    }
+    const float2 v = group_sum2<GT>(qx, qg, group, slots, buf);
+    const float rstd = 1.0f / sqrtf(v.x * inv + a.eps);
+    const float gx = v.y * inv * rstd;  // mean(g * xhat)
+    float dx[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float h = x[e] * rstd;
+      dw[e] += g[e] * h;
+      db[e] += g[e];
+      dx[e] = rstd * (g[e] * w[e] - gmean - h * gx);
+    }
+    if (a.add != nullptr) {
+      float ad[E];
+      load_row<GT, NCH, CH>(a.add, a.x_type, o * a.ao + i * a.ai, t, a.dim, ad);
+#pragma unroll
+      for (int e = 0; e < E; ++e) dx[e] += ad[e];
+    }
+    store_row<GT, NCH, CH>(a.out, a.x_type, o * a.oo + i * a.oi, t, a.dim, dx);
+  }
+  if (a.part == nullptr && a.dw == nullptr) return;
+  // join the groups' sums, in the order of the groups
+  if constexpr (NG > 1) {
+    for (int k = 0; k < 2; ++k) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < E; ++e) join[e * T + threadIdx.x] = k ? db[e] : dw[e];
+      __syncthreads();
+      if (group == 0) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          float s = 0.f;
+          for (int n = 0; n < NG; ++n) s += join[e * T + n * GT + t];
+          (k ? db[e] : dw[e]) = s;
+        }
+      }
+    }
+    if (group != 0) return;
+  }
+  float *pw, *pb;
+  if (gridDim.x == 1) {
+    pw = a.dw + static_cast<int64_t>(blockIdx.y) * a.dim;
+    pb = a.db + static_cast<int64_t>(blockIdx.y) * a.dim;
+  } else {
+    pw = a.part + (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * 2 * a.dim;
+    pb = pw + a.dim;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int col = CH * (t + GT * (e / CH)) + e % CH;
+    if (col < a.dim) pw[col] = dw[e], pb[col] = db[e];
+  }
+}
+
+// dw, db [sum group][dim] = the partials' sums. 32 columns x 8 runs of the partials per block, joined in order.
+__global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ part, int blocks, int dim,
+                                                   float* __restrict__ dw, float* __restrict__ db) {
+  __shared__ float s[8][32];
+  const int lane = threadIdx.x & 31, run = threadIdx.x >> 5;
+  const int64_t n2 = 2ll * dim;
+  const int64_t col = static_cast<int64_t>(blockIdx.x) * 32 + lane;  // over dw, then db
+  const float* p = part + static_cast<int64_t>(blockIdx.y) * blocks * n2 + col;
+  float v = 0.f;
+  if (col < n2) {
+    const int lo = static_cast<int>(static_cast<int64_t>(blocks) * run / 8);
+    const int hi = static_cast<int>(static_cast<int64_t>(blocks) * (run + 1) / 8);
+#pragma unroll 8
+    for (int k = lo; k < hi; ++k) v += p[k * n2];
+  }
+  s[run][lane] = v;
+  __syncthreads();
+  if (run == 0 && col < n2) {
+#pragma unroll
+    for (int r = 1; r < 8; ++r) v += s[r][lane];
+    float* d = col < dim ? dw : db - dim;
+    d[static_cast<int64_t>(blockIdx.y) * dim + col] = v;
+  }
+}
+
+// ---- rows wider than kMaxDimRegs: one block per row, the row read again for each pass (from L2)
+
+template <typename F>
+__device__ __forceinline__ float2 wide_sum2(int dim, float2* slots, F f) {
+  float a = 0.f, b = 0.f;
+  for (int col = threadIdx.x; col < dim; col += 1024) f(col, a, b);
+  int buf = 0;
+  const float2 r = group_sum2<1024>(a, b, 0, slots, buf);
+  __syncthreads();  // the slots are free again
+  return r;
+}
+
+__global__ void __launch_bounds__(1024) fwd_wide_kernel(const __grid_constant__ Args a) {
+  __shared__ float2 slots[2 * 32];
+  const int64_t row = blockIdx.x, o = row / a.inner, i = row - o * a.inner;
+  const int64_t xb = o * a.xo + i * a.xi, ob = o * a.oo + i * a.oi, wb = o * a.w_stride;
+  const float inv = 1.0f / static_cast<float>(a.dim);
+  auto at = [](const void* p, int type, int64_t k) {
+    float f;
+    load_chunk<1>(p, type, k, &f);
+    return f;
+  };
+  const float mean = wide_sum2(a.dim, slots, [&](int c, float& s, float&) { s += at(a.x, a.x_type, xb + c); }).x * inv;
+  const float var = wide_sum2(a.dim, slots, [&](int c, float& s, float&) {
+    const float d = at(a.x, a.x_type, xb + c) - mean;
+    s += d * d;
+  }).x * inv;
+  const float rstd = 1.0f / sqrtf(var + a.eps);
+  for (int c = threadIdx.x; c < a.dim; c += 1024) {
+    float y = (at(a.x, a.x_type, xb + c) - mean) * rstd;
+    if (a.w) y *= a.w_plus + at(a.w, a.w_type, wb + c);
+    if (a.b) y += at(a.b, a.w_type, wb + c);
+    store_chunk<1>(a.out, a.y_type, ob + c, &y);
+  }
+}
+
+// dx of a row, and its mean and rstd into part[row][2] for the column sums.
+__global__ void __launch_bounds__(1024) bwd_wide_kernel(const __grid_constant__ Args a) {
+  __shared__ float2 slots[2 * 32];
+  const int64_t row = blockIdx.x, o = row / a.inner, i = row - o * a.inner;
+  const int64_t xb = o * a.xo + i * a.xi, yb = o * a.yo + i * a.yi, ab = o * a.ao + i * a.ai, ob = o * a.oo + i * a.oi;
+  const int64_t wb = o * a.w_stride;
+  const float inv = 1.0f / static_cast<float>(a.dim);
+  auto at = [](const void* p, int type, int64_t k) {
+    float f;
+    load_chunk<1>(p, type, k, &f);
+    return f;
+  };
+  auto weight = [&](int c) { return a.w ? a.w_plus + at(a.w, a.w_type, wb + c) : 1.0f; };
+  const float2 m = wide_sum2(a.dim, slots, [&](int c, float& s, float& g) {
+    s += at(a.x, a.x_type, xb + c);
+    g += at(a.dy, a.y_type, yb + c) * weight(c);
+  });
+  const float mean = m.x * inv, gmean = m.y * inv;
+  const float2 v = wide_sum2(a.dim, slots, [&](int c, float& s, float& g) {
+    const float d = at(a.x, a.x_type, xb + c) - mean;
+    s += d * d;
+    g += at(a.dy, a.y_type, yb + c) * weight(c) * d;
+  });
+  const float rstd = 1.0f / sqrtf(v.x * inv + a.eps), gx = v.y * inv * rstd;
+  if (threadIdx.x == 0 && a.part) a.part[2 * row] = mean, a.part[2 * row + 1] = rstd;
+  for (int c = threadIdx.x; c < a.dim; c += 1024) {
+    const float h = (at(a.x, a.x_type, xb + c) - mean) * rstd;
+    float dx = rstd * (at(a.dy, a.y_type, yb + c) * weight(c) - gmean - h * gx);
+    if (a.add) dx += at(a.add, a.x_type, ab + c);
+    store_chunk<1>(a.out, a.x_type, ob + c, &dx);
+  }
+}
+
+// dw, db of 32 columns of one sum group: 8 warps take every 8th row.
+__global__ void __launch_bounds__(256) sums_wide_kernel(const __grid_constant__ Args a) {
+  __shared__ float sw[8][32], sb[8][32];
+  const int lane = threadIdx.x & 31, run = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + lane;
+  float w = 0.f, b = 0.f;
+  if (c < a.dim) {
+    for (int64_t r = run; r < a.rows; r += 8) {
+      const int64_t row = static_cast<int64_t>(blockIdx.y) * a.rows + r, o = row / a.inner, i = row - o * a.inner;
+      float x, g;
+      load_chunk<1>(a.x, a.x_type, o * a.xo + i * a.xi + c, &x);
+      load_chunk<1>(a.dy, a.y_type, o * a.yo + i * a.yi + c, &g);
+      w += g * ((x - a.part[2 * row]) * a.part[2 * row + 1]);
+      b += g;
+    }
+  }
+  sw[run][lane] = w, sb[run][lane] = b;
+  __syncthreads();
+  if (run == 0 && c < a.dim) {
+#pragma unroll
+    for (int r = 1; r < 8; ++r) w += sw[r][lane], b += sb[r][lane];
+    a.dw[static_cast<int64_t>(blockIdx.y) * a.dim + c] = w;
+    a.db[static_cast<int64_t>(blockIdx.y) * a.dim + c] = b;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- host
+
+// The group of threads for a row of `dim` elements: at most 16 elements a thread.
+static int group_threads(int dim) {
+  int gt = 32;
+  while (gt * 16 < dim) gt *= 2;
+  return gt;
+}
+
+// Blocks per sum group of the backward pass: enough groups of threads for every row, at most `kBwdBlocks` in all.
+constexpr int kBwdBlocks = 2 * kNumSms;
+static int64_t bwd_blocks(int64_t rows, int dim, int64_t sum_groups) {
+  const int gt = group_threads(dim), ng = std::max(1, 256 / gt);
+  const int64_t need = std::max<int64_t>(1, (rows + ng - 1) / ng);
+  return std::max<int64_t>(1, std::min(need, kBwdBlocks / std::max<int64_t>(1, sum_groups)));
+}
+
+template <int GT, int NCH, int CH>
+static cudaError_t go(const Args& a, bool bwd, int64_t sum_groups, cudaStream_t st) {
+  constexpr int T = block_threads<GT>(), NG = T / GT;
+  if (!bwd) {
+    fwd_kernel<GT, NCH, CH><<<static_cast<unsigned>((a.rows + NG - 1) / NG), T, 0, st>>>(a);
+    return cudaGetLastError();
+  }
+  const int64_t blocks = bwd_blocks(a.rows, a.dim, sum_groups);
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(sum_groups));
+  bwd_kernel<GT, NCH, CH><<<grid, T, 0, st>>>(a);
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess && a.part != nullptr && blocks > 1) {
+    const dim3 jg(static_cast<unsigned>((2ll * a.dim + 31) / 32), static_cast<unsigned>(sum_groups));
+    join_kernel<<<jg, 256, 0, st>>>(a.part, static_cast<int>(blocks), a.dim, a.dw, a.db);
+    e = cudaGetLastError();
+  }
+  return e;
+}
+
+template <int GT>
+static cudaError_t go_gt(const Args& a, bool bwd, int64_t sum_groups, bool vec, cudaStream_t st) {
+  if (!vec) return go<GT, 16, 1>(a, bwd, sum_groups, st);
+  switch ((a.dim + 4 * GT - 1) / (4 * GT)) {
+    case 1: return go<GT, 1, 4>(a, bwd, sum_groups, st);
+    case 2: return go<GT, 2, 4>(a, bwd, sum_groups, st);
+    case 3: return go<GT, 3, 4>(a, bwd, sum_groups, st);
+    default: return go<GT, 4, 4>(a, bwd, sum_groups, st);
+  }
+}
+
+static cudaError_t dispatch(const Args& a, bool bwd, int64_t sum_groups, bool vec, cudaStream_t st) {
+  if (a.dim > kMaxDimRegs) {
+    if (!bwd) {
+      fwd_wide_kernel<<<static_cast<unsigned>(a.rows), 1024, 0, st>>>(a);
+      return cudaGetLastError();
+    }
+    bwd_wide_kernel<<<static_cast<unsigned>(a.rows * sum_groups), 1024, 0, st>>>(a);
+    cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess && a.part != nullptr) {
+      sums_wide_kernel<<<dim3((a.dim + 31) / 32, static_cast<unsigned>(sum_groups)), 256, 0, st>>>(a);
+      e = cudaGetLastError();
+    }
+    return e;
+  }
+  switch (group_threads(a.dim)) {
+    case 32: return go_gt<32>(a, bwd, sum_groups, vec, st);
+    case 64: return go_gt<64>(a, bwd, sum_groups, vec, st);
+    case 128: return go_gt<128>(a, bwd, sum_groups, vec, st);
+    case 256: return go_gt<256>(a, bwd, sum_groups, vec, st);
+    case 512: return go_gt<512>(a, bwd, sum_groups, vec, st);
+    default: return go_gt<1024>(a, bwd, sum_groups, vec, st);
+  }
+}
+
+static bool is_dtype(int t) { return t == FB_F32 || t == FB_F16 || t == FB_BF16; }
+static int size_of(int t) { return t == FB_F32 ? 4 : 2; }
+// Whether chunks of four elements of this tensor are aligned vectors.
+static bool vec4(const void* p, int type, std::initializer_list<int64_t> strides) {
+  if (reinterpret_cast<uintptr_t>(p) % (4 * size_of(type)) != 0) return false;
+  for (int64_t s : strides)
+    if (s % 4 != 0) return false;
+  return true;
+}
+static bool misaligned(const void* p, int type) { return reinterpret_cast<uintptr_t>(p) % size_of(type) != 0; }
+
+}  // namespace norm
+
+int64_t layer_norm_work_floats(int64_t outer, int64_t inner, int32_t dim, int32_t per_outer) {
+  const int64_t rows = per_outer ? inner : outer * inner, groups = per_outer ? outer : 1;
+  if (rows <= 0 || groups <= 0 || dim <= 0) return 0;
+  if (dim > norm::kMaxDimRegs) return 2 * rows * groups;
+  const int64_t blocks = norm::bwd_blocks(rows, dim, groups);
+  return blocks > 1 ? groups * blocks * 2 * dim : 0;
+}
+
+int launch_layer_norm(const fb_layer_norm_args& p, bool bwd, cudaStream_t st, std::string& err) {
+  const char* who = bwd ? "fb_layer_norm_backward" : "fb_layer_norm";
+  auto bad = [&](int code, const char* what) {
+    err = std::string(who) + ": " + what;
+    return code;
+  };
+  if (p.outer < 0 || p.inner < 0 || p.dim < 1) return bad(FB_ERR_ARG, "need outer, inner >= 0 and dim >= 1");
+  if (!norm::is_dtype(p.x_dtype) || !norm::is_dtype(p.y_dtype) || !norm::is_dtype(p.w_dtype))
+    return bad(FB_ERR_ARG, "dtypes must be FB_F32, FB_F16 or FB_BF16");
+  if (!(p.eps >= 0.0f)) return bad(FB_ERR_ARG, "eps must be >= 0");
+  const bool sums = bwd && (p.dweight || p.dbias);
+  if (sums && (!p.dweight || !p.dbias)) return bad(FB_ERR_ARG, "dweight and dbias come together");
+  const int64_t rows_all = (p.inner > 0 && p.outer > (1ll << 31) / p.inner) ? (1ll << 40) : p.outer * p.inner;
+  if (rows_all > 0x7FFFFFFFll) return bad(FB_ERR_UNSUPPORTED, "at most 2^31 - 1 rows per call");
+  const bool per_outer = sums && p.sum_per_outer;
+  const int64_t groups = per_outer ? p.outer : 1;
+  if (groups > 65535) return bad(FB_ERR_UNSUPPORTED, "at most 65535 gradients of their own per call");
+  if (rows_all == 0) {
+    if (sums && groups > 0) {  // sums over no rows
+      const size_t n = static_cast<size_t>(groups) * p.dim * sizeof(float);
+      cudaError_t e = cudaMemsetAsync(p.dweight, 0, n, st);
+      if (e == cudaSuccess) e = cudaMemsetAsync(p.dbias, 0, n, st);
+      if (e != cudaSuccess) {
+        err = std::string(who) + ": " + cudaGetErrorString(e);
+        return FB_ERR_CUDA;
+      }
+    }
+    return FB_OK;
+  }
+  if (!p.x || !p.out || (bwd && !p.dy)) return bad(FB_ERR_ARG, "null pointer");
+  if (norm::misaligned(p.x, p.x_dtype) || norm::misaligned(p.out, bwd ? p.x_dtype : p.y_dtype) ||
+      (bwd && (norm::misaligned(p.dy, p.y_dtype) || (p.add && norm::misaligned(p.add, p.x_dtype)))) ||
+      (p.weight && norm::misaligned(p.weight, p.w_dtype)) || (p.bias && norm::misaligned(p.bias, p.w_dtype)) ||
+      norm::misaligned(p.dweight, FB_F32) || norm::misaligned(p.dbias, FB_F32) || norm::misaligned(p.work, FB_F32))
+    return bad(FB_ERR_ALIGN, "a pointer is not aligned to its elements");
+  norm::Args a;
+  memset(&a, 0, sizeof(a));
+  a.x = p.x;
+  a.dy = p.dy;
+  a.add = bwd ? p.add : nullptr;
+  a.out = p.out;
+  a.w = p.weight;
+  a.b = p.bias;
+  a.xo = p.x_outer_stride, a.xi = p.x_inner_stride;
+  a.yo = p.dy_outer_stride, a.yi = p.dy_inner_stride;
+  a.ao = p.add_outer_stride, a.ai = p.add_inner_stride;
+  a.oo = p.out_outer_stride, a.oi = p.out_inner_stride;
+  a.w_stride = p.w_outer_stride;
+  a.inner = p.inner;
+  a.rows = per_outer ? p.inner : rows_all;
+  a.dim = p.dim;
+  a.x_type = p.x_dtype;
+  a.y_type = p.y_dtype;
+  a.w_type = p.w_dtype;
+  a.w_plus = p.weight_plus_one ? 1.0f : 0.0f;
+  a.eps = p.eps;
+  if (sums) {
+    const int64_t need = layer_norm_work_floats(p.outer, p.inner, p.dim, p.sum_per_outer);
+    if (p.work_floats < need || (need > 0 && !p.work)) return bad(FB_ERR_ARG, "workspace too small");
+    a.part = need > 0 ? p.work : nullptr;
+    a.dw = p.dweight;
+    a.db = p.dbias;
+  }
+  bool vec = p.dim % 4 == 0 && norm::vec4(p.x, p.x_dtype, {a.xo, a.xi}) &&
+             norm::vec4(p.out, bwd ? p.x_dtype : p.y_dtype, {a.oo, a.oi});
+  if (bwd) vec = vec && norm::vec4(p.dy, p.y_dtype, {a.yo, a.yi}) && (!p.add || norm::vec4(p.add, p.x_dtype, {a.ao, a.ai}));
+  if (p.weight) vec = vec && norm::vec4(p.weight, p.w_dtype, {a.w_stride});
+  if (p.bias) vec = vec && norm::vec4(p.bias, p.w_dtype, {a.w_stride});
+  const cudaError_t e = norm::dispatch(a, bwd, groups, vec, st);
+  if (e != cudaSuccess) {
+    err = std::string(who) + ": " + cudaGetErrorString(e);
+    return FB_ERR_CUDA;
+  }
+  return FB_OK;
+}
+
+}  // namespace fb

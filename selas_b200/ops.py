@@ -7,6 +7,7 @@ The wrappers raise ``FluxB200Error`` for anything the kernels do not handle; the
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -383,6 +384,261 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, o
     p.out, p.ld_out = out.data_ptr(), out.stride(0)
     run_linears([p], _lib.FB_EPI_STORE_F32 if out_dtype == F32 else _lib.FB_EPI_STORE_BF16)
     return out.view(*lead, w.shape[0])
+
+
+# ------------------------------------------------------------------------------------------ token-wise operators
+
+# These take tensors on any device of the process: the launch goes to the current stream of the tensors' device.
+_IDS_CODE = {torch.float32: _lib.FB_IDS_F32, torch.float64: _lib.FB_IDS_F64, torch.int32: _lib.FB_IDS_I32,
+             torch.int64: _lib.FB_IDS_I64}
+_PAIRS = {"interleaved": _lib.FB_ROPE_INTERLEAVED, "halves": _lib.FB_ROPE_HALVES}
+ACTIVATIONS = {"none": _lib.FB_ACT_NONE, "relu": _lib.FB_ACT_RELU, "gelu": _lib.FB_ACT_GELU,
+               "gelu_tanh": _lib.FB_ACT_GELU_TANH, "quick_gelu": _lib.FB_ACT_QUICK_GELU, "silu": _lib.FB_ACT_SILU}
+
+
+def _one_device(what: str, *ts: torch.Tensor | None) -> torch.device:
+    """The one CUDA device of all the given tensors."""
+    dev = ts[0].device
+    _cuda(ts[0])
+    for t in ts[1:]:
+        if t is not None and t.device != dev:
+            raise FluxB200Error(f"{what}: every tensor must be on one CUDA device, got {dev} and {t.device}")
+    return dev
+
+
+def _launch(dev: torch.device, what: str, flops: float, nbytes: float, call) -> None:
+    """``call(library, stream)`` of the entry point fb_``what`` with ``dev`` the current device, on its current stream."""
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _launch(dev, what, flops, nbytes, call)
+    lib = _lib.lib()
+    with _prof.region(what, flops, nbytes):
+        _lib.check(call(lib, _stream()), "fb_" + what)
+    _count()
+
+
+@functools.lru_cache(maxsize=64)
+def _rope_plan(axes_dim: tuple, theta) -> tuple:
+    """The C arrays of the axes' dims and bases."""
+    n = len(axes_dim)
+    thetas = tuple(theta) if isinstance(theta, tuple) else (theta,) * n
+    _need(n >= 1 and len(thetas) == n, "rope_axes: theta is one base, or one per axis")
+    return (ctypes.c_int32 * n)(*axes_dim), (ctypes.c_double * n)(*thetas), sum(axes_dim)
+
+
+def _rope(xs: tuple, ids: torch.Tensor, axes_dim, theta, pairs: str, inverse: bool) -> list[torch.Tensor]:
+    x = xs[0]
+    dev = _one_device("rope_axes", *xs, ids)
+    _need(x.dim() == 4 and x.dtype in _DTYPE_CODE, "rope_axes: fp32, bf16 or fp16 [B, H, L, hd] tensors")
+    b, _, l, hd = x.shape
+    axes_dim = tuple(axes_dim)
+    dims, thetas, total = _rope_plan(axes_dim, tuple(theta) if isinstance(theta, (tuple, list)) else float(theta))
+    _need(hd == total, f"rope_axes: the axes' dims {axes_dim} must add up to head_dim {hd}")
+    _need(pairs in _PAIRS, f"rope_axes: pairs is 'interleaved' or 'halves', got {pairs!r}")
+    _need(ids.dtype in _IDS_CODE, "rope_axes: ids must be fp32, fp64, int32 or int64")
+    _need(ids.dim() in (2, 3) and ids.shape[-1] == len(axes_dim) and ids.shape[-2] == l
+          and (ids.dim() == 2 or ids.shape[0] in (1, b)), f"rope_axes: ids must be [L, axes] or [B, L, axes], got {tuple(ids.shape)}")
+    ib = ids.stride(0) if ids.dim() == 3 and ids.shape[0] > 1 else 0
+    arr, outs = (_lib.FbRopeTensor * len(xs))(), []
+    for t, e in zip(xs, arr):
+        _need(t.dim() == 4 and t.dtype == x.dtype and t.shape[0] == b and t.shape[2] == l and t.shape[3] == hd
+              and (t.stride(3) == 1 or hd == 1), "rope_axes: q and k must be [B, H, L, hd] of one type with unit stride along hd")
+        h = t.shape[1]
+        out = torch.empty(b, h, l, hd, dtype=t.dtype, device=dev)
+        outs.append(out)
+        sb, sh, sl, _ = t.stride()
+        e.x, e.x_stride_b, e.x_stride_h, e.x_stride_l, e.heads = t.data_ptr(), sb, sh, sl, h
+        e.out, e.out_stride_b, e.out_stride_h, e.out_stride_l = out.data_ptr(), h * l * hd, l * hd, hd
+    if b * l == 0:
+        return outs
+    nbytes = 2 * sum(t.numel() for t in outs) * x.element_size()
+    _launch(dev, "rope_axes", 0.0, nbytes, lambda lib, st: lib.fb_rope_axes(
+        ctypes.addressof(arr), len(xs), _DTYPE_CODE[x.dtype], b, l, hd, ids.data_ptr(), _IDS_CODE[ids.dtype], ib,
+        ids.stride(-2), ids.stride(-1), len(axes_dim), ctypes.addressof(dims), ctypes.addressof(thetas), _PAIRS[pairs],
+        int(bool(inverse)), st))
+    return outs
+
+
+def rope_axes(x: torch.Tensor, ids: torch.Tensor, axes_dim, theta=10000.0, *, pairs: str = "interleaved",
+              inverse: bool = False) -> torch.Tensor:
+    """Rotary positions with several axes (time, height, width, ...) straight from the position ids: what
+    ``model.rope_tables`` and the rotation after it compute (selas/models/flux.py:106-121), in one kernel.
+
+    x fp32 / bf16 / fp16 [B, H, L, hd], any strides with unit stride along hd (e.g. a transposed slice of a fused
+    projection); ids [L, A] or [B, L, A] int or float; ``axes_dim`` the dims of each axis (even, adding up to hd);
+    ``theta`` one base or one per axis. ``pairs``: "interleaved" turns elements (2s, 2s + 1) by slot s, "halves" elements
+    (s, s + hd / 2). ``inverse`` turns the other way, which is the gradient: dx = rope_axes(dy, ..., inverse=True).
+    Returns a contiguous [B, H, L, hd]."""
+    return _rope((x,), ids, axes_dim, theta, pairs, inverse)[0]
+
+
+def rope_axes_qk(q: torch.Tensor, k: torch.Tensor, ids: torch.Tensor, axes_dim, theta=10000.0, *,
+                 pairs: str = "interleaved", inverse: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """``rope_axes`` of q and k (which may differ in their number of heads) in one launch, each angle computed once."""
+    q, k = _rope((q, k), ids, axes_dim, theta, pairs, inverse)
+    return q, k
+
+
+def _outer_inner(what: str, t: torch.Tensor) -> tuple[int, int]:
+    """(outer, inner) strides of the rows of t [..., D] seen as [outer, inner, D]."""
+    n = t.dim()
+    _need(t.stride(-1) == 1 or t.shape[-1] == 1, f"{what}: the last dim must have unit stride")
+    if n == 3:
+        return t.stride(0), t.stride(1)
+    if n == 2:
+        return 0, t.stride(0)
+    if n == 1:
+        return 0, 0
+    if t.is_contiguous():
+        return t.stride(-3), t.stride(-2)
+    raise FluxB200Error(f"{what}: a tensor of more than three dims must be contiguous")
+
+
+def _norm_args(what: str, x: torch.Tensor, weight, bias, eps: float) -> _lib.FbLayerNormArgs:
+    _need(x.dim() >= 1 and x.dtype in _DTYPE_CODE and x.shape[-1] > 0, f"{what}: x must be fp32, bf16 or fp16 [..., D]")
+    d = x.shape[-1]
+    a = _lib.FbLayerNormArgs()
+    a.x = x.data_ptr()
+    a.x_outer_stride, a.x_inner_stride = _outer_inner(what, x)
+    a.inner = x.shape[-2] if x.dim() > 1 else 1
+    a.outer = math.prod(x.shape[:-2])
+    a.dim, a.x_dtype, a.eps = d, _DTYPE_CODE[x.dtype], eps
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None:
+            _need(t.dtype in _DTYPE_CODE and t.shape == (d,) and t.is_contiguous(), f"{what}: {name} must be fp32, bf16 or fp16 [D]")
+            _need(weight is None or t.dtype == weight.dtype, f"{what}: weight and bias must share a type")
+            a.w_dtype = _DTYPE_CODE[t.dtype]
+            setattr(a, name, t.data_ptr())
+    return a
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5,
+               *, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last dim of x [..., D] (fp32, bf16 or fp16; rows may be
+    strided), statistics in fp32, rounded once to ``out_dtype`` (x's by default). weight and bias: [D] of one type, or
+    None. Returns a contiguous tensor."""
+    dev = _one_device("layer_norm", x, weight, bias)
+    a = _norm_args("layer_norm", x, weight, bias, eps)
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    _need(out_dtype in _DTYPE_CODE, "layer_norm: out_dtype must be fp32, bf16 or fp16")
+    out = torch.empty(x.shape, dtype=out_dtype, device=dev)
+    if out.numel() == 0:
+        return out
+    a.out, a.y_dtype = out.data_ptr(), _DTYPE_CODE[out_dtype]
+    a.out_outer_stride, a.out_inner_stride = a.inner * a.dim, a.dim
+    _launch(dev, "layer_norm", 0.0, x.numel() * (x.element_size() + out.element_size()),
+            lambda lib, st: lib.fb_layer_norm(ctypes.addressof(a), st))
+    return out
+
+
+def _norm_backward(what: str, a: _lib.FbLayerNormArgs, dev, dy, x, add, sums: bool, groups: int):
+    _need(dy.dtype in _DTYPE_CODE and dy.shape == x.shape, f"{what}: dy must be fp32, bf16 or fp16 of x's shape")
+    a.dy, a.y_dtype = dy.data_ptr(), _DTYPE_CODE[dy.dtype]
+    a.dy_outer_stride, a.dy_inner_stride = _outer_inner(what, dy)
+    if add is not None:
+        _need(add.dtype == x.dtype and add.shape == x.shape, f"{what}: add must be of x's shape and type")
+        a.add = add.data_ptr()
+        a.add_outer_stride, a.add_inner_stride = _outer_inner(what, add)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    a.out, a.out_outer_stride, a.out_inner_stride = dx.data_ptr(), a.inner * a.dim, a.dim
+    dw = db = None
+    if sums:
+        lib = _lib.load()
+        need = lib.fb_layer_norm_work_floats(a.outer, a.inner, a.dim, a.sum_per_outer)
+        # the two gradients and the partial sums in one allocation
+        n = groups * a.dim
+        buf = torch.empty(2 * n + need, dtype=F32, device=dev)
+        dw, db, work = buf[:n], buf[n:2 * n], buf[2 * n:]
+        a.dweight, a.dbias, a.work, a.work_floats = dw.data_ptr(), db.data_ptr(), work.data_ptr(), need
+    if x.numel() or (dw is not None and dw.numel()):
+        _launch(dev, "layer_norm_backward", 0.0, x.numel() * ((2 + (add is not None)) * x.element_size() + dy.element_size()),
+                lambda lib, st: lib.fb_layer_norm_backward(ctypes.addressof(a), st))
+    return dx, dw, db
+
+
+def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-5, *,
+                        add: torch.Tensor | None = None, sums: bool = True):
+    """The gradients of ``layer_norm`` for the gradient dy of its output: (dx, dweight, dbias). x is what the forward
+    took (its statistics are computed again, nothing has to be saved); dy fp32, bf16 or fp16 of x's shape. ``add`` (x's
+    type and shape) is added to dx before its one rounding: the gradient that reaches x past the norm, as in a residual
+    stream. dx has x's type; dweight = sum of dy * xhat and dbias = sum of dy are fp32 [D], summed in a fixed order;
+    ``sums=False`` leaves them out (None)."""
+    dev = _one_device("layer_norm_backward", x, dy, weight, add)
+    a = _norm_args("layer_norm_backward", x, weight, None, eps)
+    return _norm_backward("layer_norm_backward", a, dev, dy, x, add, sums, 1)
+
+
+def ln_mod_backward(dy: torch.Tensor, x: torch.Tensor, scale: torch.Tensor, *, add: torch.Tensor | None = None,
+                    sums: bool = True):
+    """The gradients of ``ln_mod`` (bf16(LayerNorm(x) * (1 + scale) + shift), eps 1e-6): (dx, dshift, dscale) for x fp32
+    [B, L, D] (rows may be strided), scale bf16 [B, D] rows as ``ln_mod`` takes them, dy bf16 or fp32 of x's shape. ``add``
+    as in ``layer_norm_backward``. dx fp32; dshift and dscale fp32 [B, D], summed over each image's tokens in a fixed
+    order ([1, D] over all tokens when scale is one row shared by several images)."""
+    dev = _one_device("ln_mod_backward", x, dy, scale, add)
+    _need(x.dtype == F32 and x.dim() == 3, "ln_mod_backward: x must be fp32 [B, L, D]")
+    a = _norm_args("ln_mod_backward", x, None, None, 1e-6)
+    b, _, d = x.shape
+    sc, stride = _mod_rows(scale, b, d)
+    rows = sc.shape[0]
+    a.weight, a.w_dtype, a.weight_plus_one = sc.data_ptr(), _lib.FB_BF16, 1
+    a.w_outer_stride, a.sum_per_outer = stride, int(rows > 1)
+    dx, dscale, dshift = _norm_backward("ln_mod_backward", a, dev, dy, x, add, sums and rows > 0, rows)
+    if sums and rows == 0:
+        dscale = dshift = torch.empty(0, dtype=F32, device=dev)
+    if dscale is None:
+        return dx, None, None
+    return dx, dshift.view(rows, d), dscale.view(rows, d)
+
+
+def _rows(t: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
+    """t [..., cols] as [rows, cols] with unit stride along a row and rows that do not overlap (a copy if it has to be)."""
+    t = t if t.dim() == 2 else t.reshape(rows, cols)
+    ok = (cols <= 1 or t.stride(1) == 1) and (rows <= 1 or t.stride(0) >= cols)
+    return t if ok else t.contiguous()
+
+
+def linear_act(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, act: str = "none",
+               residual: torch.Tensor | None = None, *, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """act(x w^T + bias) + residual on the fp32 accumulator, rounded once to ``out_dtype`` (x's type by default, or fp32).
+
+    x [..., K] and w [N, K] both bf16 or both fp16 (rows may be strided), bias [N] of their type, residual [..., N] of
+    their type or fp32; ``act`` one of ``ACTIVATIONS``. Any number of rows from one up, any K and N; operands whose rows
+    do not start on 16 bytes (K or a row stride not a multiple of 8) are copied to such rows on the way. Unlike
+    ``linear`` with its fused epilogues, nothing is rounded before the activation and the residual."""
+    dev = _one_device("linear_act", x, w, bias, residual)
+    _need(x.dtype in (BF16, torch.float16) and w.dtype == x.dtype, "linear_act: x and w must both be bf16 or both fp16")
+    _need(x.dim() >= 1 and w.dim() == 2 and x.shape[-1] == w.shape[1], f"linear_act: K mismatch {tuple(x.shape)} x {tuple(w.shape)}")
+    _need(act in ACTIVATIONS, f"linear_act: act must be one of {sorted(ACTIVATIONS)}, got {act!r}")
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    _need(out_dtype in (x.dtype, F32), "linear_act: out_dtype must be x's type or fp32")
+    n, k = w.shape
+    _need(n >= 1, "linear_act: w needs at least one row")
+    m = math.prod(x.shape[:-1])
+    x2, w = _rows(x, m, k), _rows(w, n, k)
+    a = _lib.FbLinearActArgs()
+    r2 = None
+    if residual is not None:
+        _need(residual.dtype in (x.dtype, F32) and residual.shape[:-1] == x.shape[:-1] and residual.shape[-1] == n,
+              "linear_act: residual must be [..., N] of x's type or fp32")
+        r2 = _rows(residual, m, n)
+        a.residual, a.ld_residual, a.residual_dtype = r2.data_ptr(), r2.stride(0) if m > 1 else n, _DTYPE_CODE[r2.dtype]
+    if bias is not None:
+        _need(bias.dtype == x.dtype and bias.shape == (n,) and bias.is_contiguous(), "linear_act: bias must be [N] of x's type")
+        a.bias = bias.data_ptr()
+    out = torch.empty(*x.shape[:-1], n, dtype=out_dtype, device=dev)
+    if m == 0:
+        return out
+    a.x, a.ldx, a.w, a.ldw = x2.data_ptr(), x2.stride(0) if m > 1 else k, w.data_ptr(), w.stride(0) if n > 1 else k
+    a.out, a.ld_out, a.m, a.n, a.k = out.data_ptr(), n, m, n, k
+    a.dtype, a.out_dtype, a.act = _DTYPE_CODE[x.dtype], _DTYPE_CODE[out_dtype], ACTIVATIONS[act]
+    need = _lib.load().fb_linear_act_work_bytes(ctypes.addressof(a))
+    work = None
+    if need:
+        work = torch.empty(need, dtype=torch.uint8, device=dev)
+        a.work, a.work_bytes = work.data_ptr(), need
+    _launch(dev, "linear_act", 2.0 * m * n * k, (m * k + n * k) * 2 + m * n * out.element_size(),
+            lambda lib, st: lib.fb_linear_act(ctypes.addressof(a), st))
+    return out
 
 
 # ------------------------------------------------------------------------------------------ step cache

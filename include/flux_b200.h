@@ -227,15 +227,21 @@ typedef struct fb_rope_tensor {
   int32_t heads;
 } fb_rope_tensor;
 
-/* Rotary positions with several axes, for 1 or 2 tensors (q and k, which may differ in heads) in one launch. Axis a owns
+/* Rotary positions with several axes, for `count` = 1 or 2 tensors (q and k, which may differ in heads) in one launch. Axis a owns
  * axes_dim[a] / 2 slots with the frequencies theta[a]^(-2j / axes_dim[a]) (the order of rope_tables,
  * selas/models/flux.py:106-114; the axes_dim add up to head_dim <= 512), turned by ids[b, l, a] times the frequency:
  * no cos/sin table is made, and the angle is reduced in 64 bits. inverse != 0 turns the other way: the gradient. ids
- * has strides ids_stride_b (0: one set for all images), _l and _a, in elements. */
-int32_t fb_rope_axes(const fb_rope_tensor* tensors, int32_t count, int32_t dtype, int32_t batch, int32_t seq,
-                     int32_t head_dim, const void* ids, int32_t ids_type, int64_t ids_stride_b, int64_t ids_stride_l,
-                     int64_t ids_stride_a, int32_t axes, const int32_t* axes_dim, const double* theta, int32_t pairs,
-                     int32_t inverse, void* stream);
+ * has strides ids_stride_b (0: one set for all images), _l and _a, in elements; 1 to 8 axes. */
+typedef struct fb_rope_args {
+  fb_rope_tensor tensor[2];
+  const void* ids; int64_t ids_stride_b, ids_stride_l, ids_stride_a;
+  double theta[8];
+  int32_t axes_dim[8];
+  int32_t count, dtype, batch, seq, head_dim;
+  int32_t ids_type, axes, pairs, inverse;
+} fb_rope_args;
+
+int32_t fb_rope_axes(const fb_rope_args* args, void* stream);
 
 /* Layer norm of the rows of x [outer, inner, dim] (unit stride along dim; outer and inner strides in elements):
  *   y  = xhat * w + bias,  xhat = (x - mean) / sqrt(var + eps),

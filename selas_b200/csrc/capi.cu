@@ -328,15 +328,11 @@ int32_t fb_qk_norm_rope(const uint16_t* qkv, int64_t ld_qkv, int32_t batch, int3
                  "fb_qk_norm_rope");
 }
 
-int32_t fb_rope_axes(const fb_rope_tensor* tensors, int32_t count, int32_t dtype, int32_t batch, int32_t seq,
-                     int32_t head_dim, const void* ids, int32_t ids_type, int64_t ids_stride_b, int64_t ids_stride_l,
-                     int64_t ids_stride_a, int32_t axes, const int32_t* axes_dim, const double* theta, int32_t pairs,
-                     int32_t inverse, void* stream) {
+int32_t fb_rope_axes(const fb_rope_args* args, void* stream) {
   if (int rc = ready_or_fail()) return rc;
-  return guarded("fb_rope_axes", [&](std::string& err) {
-    return launch_rope_axes(tensors, count, dtype, batch, seq, head_dim, ids, ids_type, ids_stride_b, ids_stride_l,
-                            ids_stride_a, axes, axes_dim, theta, pairs, inverse, static_cast<cudaStream_t>(stream), err);
-  });
+  if (!args) return fail(FB_ERR_ARG, "fb_rope_axes: null arguments");
+  return guarded("fb_rope_axes",
+                 [&](std::string& err) { return launch_rope_axes(*args, static_cast<cudaStream_t>(stream), err); });
 }
 
 int32_t fb_layer_norm(const fb_layer_norm_args* args, void* stream) {

@@ -78,10 +78,7 @@ int launch_attention_sp(const uint16_t* q, const uint16_t* k, const uint16_t* v,
                         int64_t ld_out, int col0, int heads, int seq_local, int sp_world, int head_dim, float scale,
                         cudaStream_t st, std::string& err);
 
-int launch_rope_axes(const fb_rope_tensor* tensors, int count, int dtype, int batch, int seq, int head_dim, const void* ids,
-                     int ids_type, int64_t ids_stride_b, int64_t ids_stride_l, int64_t ids_stride_a, int axes,
-                     const int32_t* axes_dim, const double* theta, int pairs, int inverse, cudaStream_t st,
-                     std::string& err);
+int launch_rope_axes(const fb_rope_args& args, cudaStream_t st, std::string& err);
 int launch_layer_norm(const fb_layer_norm_args& args, bool backward, cudaStream_t st, std::string& err);
 int64_t layer_norm_work_floats(int64_t outer, int64_t inner, int32_t dim, int32_t sum_per_outer);
 int launch_linear_act(const fb_linear_act_args& args, cudaStream_t st, std::string& err);

@@ -388,7 +388,9 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, o
 
 # ------------------------------------------------------------------------------------------ token-wise operators
 
-# These take tensors on any device of the process: the launch goes to the current stream of the tensors' device.
+# These take tensors on any device of the process: the launch goes to the current stream of the tensors' device. The
+# smallest calls take a few microseconds on the GPU, less than a wrapper spends on setting a ctypes.Structure's fields or
+# asking for a Stream object, so the arguments are packed in one go (_lib.packer) and the stream is read as its handle.
 _IDS_CODE = {torch.float32: _lib.FB_IDS_F32, torch.float64: _lib.FB_IDS_F64, torch.int32: _lib.FB_IDS_I32,
              torch.int64: _lib.FB_IDS_I64}
 _PAIRS = {"interleaved": _lib.FB_ROPE_INTERLEAVED, "halves": _lib.FB_ROPE_HALVES}
@@ -396,67 +398,85 @@ ACTIVATIONS = {"none": _lib.FB_ACT_NONE, "relu": _lib.FB_ACT_RELU, "gelu": _lib.
                "gelu_tanh": _lib.FB_ACT_GELU_TANH, "quick_gelu": _lib.FB_ACT_QUICK_GELU, "silu": _lib.FB_ACT_SILU}
 
 
-def _one_device(what: str, *ts: torch.Tensor | None) -> torch.device:
-    """The one CUDA device of all the given tensors."""
-    dev = ts[0].device
+def _raw_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+
+
+def _one_device(what: str, *ts: torch.Tensor | None) -> int:
+    """The index of the one CUDA device of all the given tensors."""
     _cuda(ts[0])
-    for t in ts[1:]:
-        if t is not None and t.device != dev:
-            raise FluxB200Error(f"{what}: every tensor must be on one CUDA device, got {dev} and {t.device}")
-    return dev
+    index = ts[0].get_device()
+    for t in ts:
+        if t is not None and t.get_device() != index:
+            raise FluxB200Error(f"{what}: every tensor must be on one CUDA device, got {ts[0].device} and {t.device}")
+    return index
 
 
-def _launch(dev: torch.device, what: str, flops: float, nbytes: float, call) -> None:
-    """``call(library, stream)`` of the entry point fb_``what`` with ``dev`` the current device, on its current stream."""
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            return _launch(dev, what, flops, nbytes, call)
-    lib = _lib.lib()
-    with _prof.region(what, flops, nbytes):
-        _lib.check(call(lib, _stream()), "fb_" + what)
+def _launch(index: int, entry: str, flops: float, nbytes: float, packed: bytes) -> None:
+    """The C entry ``fb_<entry>`` on the packed arguments, with device ``index`` current, on its current stream."""
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _launch(index, entry, flops, nbytes, packed)
+    fn = getattr(_lib.lib(), "fb_" + entry)
+    if _prof.enabled():
+        with _prof.region(entry, flops, nbytes):
+            rc = fn(packed, _raw_stream(index))
+    else:
+        rc = fn(packed, _raw_stream(index))
+    if rc:
+        _lib.check(rc, "fb_" + entry)
     _count()
 
 
 @functools.lru_cache(maxsize=64)
 def _rope_plan(axes_dim: tuple, theta) -> tuple:
-    """The C arrays of the axes' dims and bases."""
+    """(head_dim, the C struct's theta and axes_dim arrays) for the axes' dims and bases."""
     n = len(axes_dim)
-    thetas = tuple(theta) if isinstance(theta, tuple) else (theta,) * n
-    _need(n >= 1 and len(thetas) == n, "rope_axes: theta is one base, or one per axis")
-    return (ctypes.c_int32 * n)(*axes_dim), (ctypes.c_double * n)(*thetas), sum(axes_dim)
+    thetas = theta if isinstance(theta, tuple) else (theta,) * n
+    _need(1 <= n <= 8, "rope_axes: 1 to 8 axes")
+    _need(len(thetas) == n, "rope_axes: theta is one base, or one per axis")
+    pad = (0,) * (8 - n)
+    return sum(axes_dim), (*(float(t) for t in thetas), *pad, *(int(d) for d in axes_dim), *pad)
 
 
-def _rope(xs: tuple, ids: torch.Tensor, axes_dim, theta, pairs: str, inverse: bool) -> list[torch.Tensor]:
-    x = xs[0]
-    dev = _one_device("rope_axes", *xs, ids)
-    _need(x.dim() == 4 and x.dtype in _DTYPE_CODE, "rope_axes: fp32, bf16 or fp16 [B, H, L, hd] tensors")
-    b, _, l, hd = x.shape
+def _rope(q: torch.Tensor, k: torch.Tensor | None, ids: torch.Tensor, axes_dim, theta, pairs: str, inverse: bool):
+    index = _one_device("rope_axes", q, k, ids)
+    _need(q.dim() == 4 and q.dtype in _DTYPE_CODE, "rope_axes: fp32, bf16 or fp16 [B, H, L, hd] tensors")
+    b, h, l, hd = q.shape
     axes_dim = tuple(axes_dim)
-    dims, thetas, total = _rope_plan(axes_dim, tuple(theta) if isinstance(theta, (tuple, list)) else float(theta))
+    total, arrays = _rope_plan(axes_dim, tuple(theta) if isinstance(theta, (tuple, list)) else theta)
     _need(hd == total, f"rope_axes: the axes' dims {axes_dim} must add up to head_dim {hd}")
     _need(pairs in _PAIRS, f"rope_axes: pairs is 'interleaved' or 'halves', got {pairs!r}")
     _need(ids.dtype in _IDS_CODE, "rope_axes: ids must be fp32, fp64, int32 or int64")
-    _need(ids.dim() in (2, 3) and ids.shape[-1] == len(axes_dim) and ids.shape[-2] == l
-          and (ids.dim() == 2 or ids.shape[0] in (1, b)), f"rope_axes: ids must be [L, axes] or [B, L, axes], got {tuple(ids.shape)}")
-    ib = ids.stride(0) if ids.dim() == 3 and ids.shape[0] > 1 else 0
-    arr, outs = (_lib.FbRopeTensor * len(xs))(), []
-    for t, e in zip(xs, arr):
-        _need(t.dim() == 4 and t.dtype == x.dtype and t.shape[0] == b and t.shape[2] == l and t.shape[3] == hd
-              and (t.stride(3) == 1 or hd == 1), "rope_axes: q and k must be [B, H, L, hd] of one type with unit stride along hd")
-        h = t.shape[1]
-        out = torch.empty(b, h, l, hd, dtype=t.dtype, device=dev)
-        outs.append(out)
-        sb, sh, sl, _ = t.stride()
-        e.x, e.x_stride_b, e.x_stride_h, e.x_stride_l, e.heads = t.data_ptr(), sb, sh, sl, h
-        e.out, e.out_stride_b, e.out_stride_h, e.out_stride_l = out.data_ptr(), h * l * hd, l * hd, hd
-    if b * l == 0:
-        return outs
-    nbytes = 2 * sum(t.numel() for t in outs) * x.element_size()
-    _launch(dev, "rope_axes", 0.0, nbytes, lambda lib, st: lib.fb_rope_axes(
-        ctypes.addressof(arr), len(xs), _DTYPE_CODE[x.dtype], b, l, hd, ids.data_ptr(), _IDS_CODE[ids.dtype], ib,
-        ids.stride(-2), ids.stride(-1), len(axes_dim), ctypes.addressof(dims), ctypes.addressof(thetas), _PAIRS[pairs],
-        int(bool(inverse)), st))
-    return outs
+    ishape, istride = ids.shape, ids.stride()
+    _need(len(ishape) in (2, 3) and ishape[-1] == len(axes_dim) and ishape[-2] == l and (len(ishape) == 2 or ishape[0] in (1, b)),
+          f"rope_axes: ids must be [L, axes] or [B, L, axes], got {tuple(ishape)}")
+    ib = istride[0] if len(ishape) == 3 and ishape[0] > 1 else 0
+    sb, sh, sl, se = q.stride()
+    out_k, tensors, n = None, None, q.numel()
+    _need(se == 1, "rope_axes: q and k must be [B, H, L, hd] of one type with unit stride along hd")
+    out_q = q.new_empty((b, h, l, hd))
+    tensors = (q.data_ptr(), out_q.data_ptr(), sb, sh, sl, h * l * hd, l * hd, hd, h)
+    if k is None:
+        tensors += (0,) * 9
+    else:
+        _need(k.dim() == 4 and k.dtype == q.dtype, "rope_axes: q and k must be [B, H, L, hd] of one type with unit stride along hd")
+        kb, hk, lk, hdk = k.shape
+        sb, sh, sl, se = k.stride()
+        _need(kb == b and lk == l and hdk == hd and se == 1,
+              "rope_axes: q and k must be [B, H, L, hd] of one type with unit stride along hd")
+        out_k = k.new_empty((b, hk, l, hd))
+        tensors += (k.data_ptr(), out_k.data_ptr(), sb, sh, sl, hk * l * hd, l * hd, hd, hk)
+        n += k.numel()
+    if n:
+        code = _DTYPE_CODE[q.dtype]
+        _launch(index, "rope_axes", 0.0, 2 * n * q.element_size(), _lib.pack_rope(
+            *tensors, ids.data_ptr(), ib, istride[-2], istride[-1], *arrays, 1 if k is None else 2, code, b, l, hd,
+            _IDS_CODE[ids.dtype], len(axes_dim), _PAIRS[pairs], bool(inverse)))
+    return out_q, out_k
 
 
 def rope_axes(x: torch.Tensor, ids: torch.Tensor, axes_dim, theta=10000.0, *, pairs: str = "interleaved",
@@ -469,47 +489,44 @@ def rope_axes(x: torch.Tensor, ids: torch.Tensor, axes_dim, theta=10000.0, *, pa
     ``theta`` one base or one per axis. ``pairs``: "interleaved" turns elements (2s, 2s + 1) by slot s, "halves" elements
     (s, s + hd / 2). ``inverse`` turns the other way, which is the gradient: dx = rope_axes(dy, ..., inverse=True).
     Returns a contiguous [B, H, L, hd]."""
-    return _rope((x,), ids, axes_dim, theta, pairs, inverse)[0]
+    return _rope(x, None, ids, axes_dim, theta, pairs, inverse)[0]
 
 
 def rope_axes_qk(q: torch.Tensor, k: torch.Tensor, ids: torch.Tensor, axes_dim, theta=10000.0, *,
                  pairs: str = "interleaved", inverse: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
     """``rope_axes`` of q and k (which may differ in their number of heads) in one launch, each angle computed once."""
-    q, k = _rope((q, k), ids, axes_dim, theta, pairs, inverse)
-    return q, k
+    return _rope(q, k, ids, axes_dim, theta, pairs, inverse)
 
 
 def _outer_inner(what: str, t: torch.Tensor) -> tuple[int, int]:
     """(outer, inner) strides of the rows of t [..., D] seen as [outer, inner, D]."""
-    n = t.dim()
-    _need(t.stride(-1) == 1 or t.shape[-1] == 1, f"{what}: the last dim must have unit stride")
-    if n == 3:
-        return t.stride(0), t.stride(1)
-    if n == 2:
-        return 0, t.stride(0)
-    if n == 1:
-        return 0, 0
-    if t.is_contiguous():
-        return t.stride(-3), t.stride(-2)
-    raise FluxB200Error(f"{what}: a tensor of more than three dims must be contiguous")
+    st = t.stride()
+    n = len(st)
+    _need(st[-1] == 1 or t.shape[-1] == 1, f"{what}: the last dim must have unit stride")
+    if n <= 2:
+        return 0, st[0] if n == 2 else 0
+    if n > 3 and not t.is_contiguous():
+        raise FluxB200Error(f"{what}: a tensor of more than three dims must be contiguous")
+    return st[-3], st[-2]
 
 
-def _norm_args(what: str, x: torch.Tensor, weight, bias, eps: float) -> _lib.FbLayerNormArgs:
-    _need(x.dim() >= 1 and x.dtype in _DTYPE_CODE and x.shape[-1] > 0, f"{what}: x must be fp32, bf16 or fp16 [..., D]")
-    d = x.shape[-1]
-    a = _lib.FbLayerNormArgs()
-    a.x = x.data_ptr()
-    a.x_outer_stride, a.x_inner_stride = _outer_inner(what, x)
-    a.inner = x.shape[-2] if x.dim() > 1 else 1
-    a.outer = math.prod(x.shape[:-2])
-    a.dim, a.x_dtype, a.eps = d, _DTYPE_CODE[x.dtype], eps
+def _norm_rows(what: str, x: torch.Tensor) -> tuple[int, int, int]:
+    """(outer, inner, D) of x [..., D]."""
+    shape = x.shape
+    n = len(shape)
+    _need(n >= 1 and x.dtype in _DTYPE_CODE and shape[-1] > 0, f"{what}: x must be fp32, bf16 or fp16 [..., D]")
+    return math.prod(shape[:-2]), shape[-2] if n > 1 else 1, shape[-1]
+
+
+def _norm_map(what: str, d: int, weight: torch.Tensor | None, bias: torch.Tensor | None) -> tuple[int, int, int]:
+    """(weight, bias, type code) of the affine map."""
+    code = 0
     for name, t in (("weight", weight), ("bias", bias)):
         if t is not None:
             _need(t.dtype in _DTYPE_CODE and t.shape == (d,) and t.is_contiguous(), f"{what}: {name} must be fp32, bf16 or fp16 [D]")
-            _need(weight is None or t.dtype == weight.dtype, f"{what}: weight and bias must share a type")
-            a.w_dtype = _DTYPE_CODE[t.dtype]
-            setattr(a, name, t.data_ptr())
-    return a
+            code = _DTYPE_CODE[t.dtype]
+    _need(weight is None or bias is None or weight.dtype == bias.dtype, f"{what}: weight and bias must share a type")
+    return weight.data_ptr() if weight is not None else 0, bias.data_ptr() if bias is not None else 0, code
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5,
@@ -517,42 +534,50 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dim of x [..., D] (fp32, bf16 or fp16; rows may be
     strided), statistics in fp32, rounded once to ``out_dtype`` (x's by default). weight and bias: [D] of one type, or
     None. Returns a contiguous tensor."""
-    dev = _one_device("layer_norm", x, weight, bias)
-    a = _norm_args("layer_norm", x, weight, bias, eps)
+    index = _one_device("layer_norm", x, weight, bias)
+    outer, inner, d = _norm_rows("layer_norm", x)
+    w, b, w_code = _norm_map("layer_norm", d, weight, bias)
     out_dtype = x.dtype if out_dtype is None else out_dtype
     _need(out_dtype in _DTYPE_CODE, "layer_norm: out_dtype must be fp32, bf16 or fp16")
-    out = torch.empty(x.shape, dtype=out_dtype, device=dev)
-    if out.numel() == 0:
-        return out
-    a.out, a.y_dtype = out.data_ptr(), _DTYPE_CODE[out_dtype]
-    a.out_outer_stride, a.out_inner_stride = a.inner * a.dim, a.dim
-    _launch(dev, "layer_norm", 0.0, x.numel() * (x.element_size() + out.element_size()),
-            lambda lib, st: lib.fb_layer_norm(ctypes.addressof(a), st))
+    xo, xi = _outer_inner("layer_norm", x)
+    out = x.new_empty(x.shape, dtype=out_dtype)
+    if outer * inner:
+        _launch(index, "layer_norm", 0.0, out.numel() * (x.element_size() + out.element_size()), _lib.pack_layer_norm(
+            x.data_ptr(), xo, xi, 0, 0, 0, 0, 0, 0, out.data_ptr(), inner * d, d, w, b, 0, 0, 0, 0, 0, outer, inner, d,
+            _DTYPE_CODE[x.dtype], _DTYPE_CODE[out_dtype], w_code, 0, 0, eps))
     return out
 
 
-def _norm_backward(what: str, a: _lib.FbLayerNormArgs, dev, dy, x, add, sums: bool, groups: int):
+def _norm_backward(what: str, index: int, dy, x, eps: float, weight: int, w_code: int, w_stride: int, plus_one: bool, add,
+                   sums: bool, groups: int):
+    """(dx, dweight, dbias) with one dweight and dbias per group of rows: all rows, or those of an outer index."""
+    outer, inner, d = _norm_rows(what, x)
     _need(dy.dtype in _DTYPE_CODE and dy.shape == x.shape, f"{what}: dy must be fp32, bf16 or fp16 of x's shape")
-    a.dy, a.y_dtype = dy.data_ptr(), _DTYPE_CODE[dy.dtype]
-    a.dy_outer_stride, a.dy_inner_stride = _outer_inner(what, dy)
+    xo, xi = _outer_inner(what, x)
+    yo, yi = _outer_inner(what, dy)
+    ao = ai = 0
     if add is not None:
         _need(add.dtype == x.dtype and add.shape == x.shape, f"{what}: add must be of x's shape and type")
-        a.add = add.data_ptr()
-        a.add_outer_stride, a.add_inner_stride = _outer_inner(what, add)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    a.out, a.out_outer_stride, a.out_inner_stride = dx.data_ptr(), a.inner * a.dim, a.dim
+        ao, ai = _outer_inner(what, add)
+    dx = x.new_empty(x.shape)
     dw = db = None
+    pw = pb = work = need = 0
+    per_outer = groups > 1
     if sums:
-        lib = _lib.load()
-        need = lib.fb_layer_norm_work_floats(a.outer, a.inner, a.dim, a.sum_per_outer)
         # the two gradients and the partial sums in one allocation
-        n = groups * a.dim
-        buf = torch.empty(2 * n + need, dtype=F32, device=dev)
-        dw, db, work = buf[:n], buf[n:2 * n], buf[2 * n:]
-        a.dweight, a.dbias, a.work, a.work_floats = dw.data_ptr(), db.data_ptr(), work.data_ptr(), need
-    if x.numel() or (dw is not None and dw.numel()):
-        _launch(dev, "layer_norm_backward", 0.0, x.numel() * ((2 + (add is not None)) * x.element_size() + dy.element_size()),
-                lambda lib, st: lib.fb_layer_norm_backward(ctypes.addressof(a), st))
+        need = _lib.load().fb_layer_norm_work_floats(outer, inner, d, per_outer)
+        n = groups * d
+        buf = x.new_empty(2 * n + need, dtype=F32)
+        dw, db = buf[:n], buf[n:2 * n]
+        pw = buf.data_ptr()
+        pb, work = pw + 4 * n, pw + 8 * n
+    if outer * inner or (sums and groups):
+        es = x.element_size()
+        _launch(index, "layer_norm_backward", 0.0, dx.numel() * ((2 if add is None else 3) * es + dy.element_size()),
+                _lib.pack_layer_norm(
+                    x.data_ptr(), xo, xi, dy.data_ptr(), yo, yi, 0 if add is None else add.data_ptr(), ao, ai, dx.data_ptr(),
+                    inner * d, d, weight, 0, w_stride, pw, pb, work, need, outer, inner, d, _DTYPE_CODE[x.dtype],
+                    _DTYPE_CODE[dy.dtype], w_code, plus_one, per_outer, eps))
     return dx, dw, db
 
 
@@ -563,38 +588,41 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor 
     type and shape) is added to dx before its one rounding: the gradient that reaches x past the norm, as in a residual
     stream. dx has x's type; dweight = sum of dy * xhat and dbias = sum of dy are fp32 [D], summed in a fixed order;
     ``sums=False`` leaves them out (None)."""
-    dev = _one_device("layer_norm_backward", x, dy, weight, add)
-    a = _norm_args("layer_norm_backward", x, weight, None, eps)
-    return _norm_backward("layer_norm_backward", a, dev, dy, x, add, sums, 1)
+    index = _one_device("layer_norm_backward", x, dy, weight, add)
+    w, _, w_code = _norm_map("layer_norm_backward", _norm_rows("layer_norm_backward", x)[2], weight, None)
+    return _norm_backward("layer_norm_backward", index, dy, x, eps, w, w_code, 0, False, add, sums, 1)
 
 
 def ln_mod_backward(dy: torch.Tensor, x: torch.Tensor, scale: torch.Tensor, *, add: torch.Tensor | None = None,
                     sums: bool = True):
     """The gradients of ``ln_mod`` (bf16(LayerNorm(x) * (1 + scale) + shift), eps 1e-6): (dx, dshift, dscale) for x fp32
-    [B, L, D] (rows may be strided), scale bf16 [B, D] rows as ``ln_mod`` takes them, dy bf16 or fp32 of x's shape. ``add``
-    as in ``layer_norm_backward``. dx fp32; dshift and dscale fp32 [B, D], summed over each image's tokens in a fixed
-    order ([1, D] over all tokens when scale is one row shared by several images)."""
-    dev = _one_device("ln_mod_backward", x, dy, scale, add)
+    [B, L, D] (rows may be strided), scale bf16 [B, D] rows as ``ln_mod`` takes them, dy fp32, bf16 or fp16 of x's shape.
+    ``add`` as in ``layer_norm_backward``. dx fp32; dshift and dscale fp32 [B, D], summed over each image's tokens in a
+    fixed order ([1, D] over all tokens when scale is one row shared by several images)."""
+    index = _one_device("ln_mod_backward", x, dy, scale, add)
     _need(x.dtype == F32 and x.dim() == 3, "ln_mod_backward: x must be fp32 [B, L, D]")
-    a = _norm_args("ln_mod_backward", x, None, None, 1e-6)
     b, _, d = x.shape
     sc, stride = _mod_rows(scale, b, d)
     rows = sc.shape[0]
-    a.weight, a.w_dtype, a.weight_plus_one = sc.data_ptr(), _lib.FB_BF16, 1
-    a.w_outer_stride, a.sum_per_outer = stride, int(rows > 1)
-    dx, dscale, dshift = _norm_backward("ln_mod_backward", a, dev, dy, x, add, sums and rows > 0, rows)
+    dx, dscale, dshift = _norm_backward("ln_mod_backward", index, dy, x, 1e-6, sc.data_ptr(), _lib.FB_BF16, stride, True, add,
+                                        sums and rows > 0, rows)
     if sums and rows == 0:
-        dscale = dshift = torch.empty(0, dtype=F32, device=dev)
+        dscale = dshift = x.new_empty(0)
     if dscale is None:
         return dx, None, None
     return dx, dshift.view(rows, d), dscale.view(rows, d)
 
 
-def _rows(t: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
-    """t [..., cols] as [rows, cols] with unit stride along a row and rows that do not overlap (a copy if it has to be)."""
-    t = t if t.dim() == 2 else t.reshape(rows, cols)
-    ok = (cols <= 1 or t.stride(1) == 1) and (rows <= 1 or t.stride(0) >= cols)
-    return t if ok else t.contiguous()
+def _rows(t: torch.Tensor, rows: int, cols: int) -> tuple[torch.Tensor, int]:
+    """t [..., cols] as [rows, cols] with unit stride along a row and rows that do not overlap (a copy if it has to be),
+    and its row stride."""
+    if t.dim() != 2:
+        t = t.reshape(rows, cols)
+    ld, one = t.stride()
+    if (one != 1 and cols > 1) or (ld < cols and rows > 1):
+        t = t.contiguous()
+        ld = cols
+    return t, ld if rows > 1 else cols
 
 
 def linear_act(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, act: str = "none",
@@ -605,39 +633,42 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = Non
     their type or fp32; ``act`` one of ``ACTIVATIONS``. Any number of rows from one up, any K and N; operands whose rows
     do not start on 16 bytes (K or a row stride not a multiple of 8) are copied to such rows on the way. Unlike
     ``linear`` with its fused epilogues, nothing is rounded before the activation and the residual."""
-    dev = _one_device("linear_act", x, w, bias, residual)
-    _need(x.dtype in (BF16, torch.float16) and w.dtype == x.dtype, "linear_act: x and w must both be bf16 or both fp16")
-    _need(x.dim() >= 1 and w.dim() == 2 and x.shape[-1] == w.shape[1], f"linear_act: K mismatch {tuple(x.shape)} x {tuple(w.shape)}")
+    index = _one_device("linear_act", x, w, bias, residual)
+    dt = x.dtype
+    _need(dt in (BF16, torch.float16) and w.dtype == dt, "linear_act: x and w must both be bf16 or both fp16")
+    shape = x.shape
+    _need(len(shape) >= 1 and w.dim() == 2 and shape[-1] == w.shape[1], f"linear_act: K mismatch {tuple(shape)} x {tuple(w.shape)}")
     _need(act in ACTIVATIONS, f"linear_act: act must be one of {sorted(ACTIVATIONS)}, got {act!r}")
-    out_dtype = x.dtype if out_dtype is None else out_dtype
-    _need(out_dtype in (x.dtype, F32), "linear_act: out_dtype must be x's type or fp32")
+    out_dtype = dt if out_dtype is None else out_dtype
+    _need(out_dtype in (dt, F32), "linear_act: out_dtype must be x's type or fp32")
     n, k = w.shape
     _need(n >= 1, "linear_act: w needs at least one row")
-    m = math.prod(x.shape[:-1])
-    x2, w = _rows(x, m, k), _rows(w, n, k)
-    a = _lib.FbLinearActArgs()
-    r2 = None
+    lead = shape[:-1]
+    m = math.prod(lead)
+    x, ldx = _rows(x, m, k)
+    w, ldw = _rows(w, n, k)
+    r = ldr = b = 0
+    res_code = 0
     if residual is not None:
-        _need(residual.dtype in (x.dtype, F32) and residual.shape[:-1] == x.shape[:-1] and residual.shape[-1] == n,
+        _need(residual.dtype in (dt, F32) and residual.shape[:-1] == lead and residual.shape[-1] == n,
               "linear_act: residual must be [..., N] of x's type or fp32")
-        r2 = _rows(residual, m, n)
-        a.residual, a.ld_residual, a.residual_dtype = r2.data_ptr(), r2.stride(0) if m > 1 else n, _DTYPE_CODE[r2.dtype]
+        residual, ldr = _rows(residual, m, n)
+        r, res_code = residual.data_ptr(), _DTYPE_CODE[residual.dtype]
     if bias is not None:
-        _need(bias.dtype == x.dtype and bias.shape == (n,) and bias.is_contiguous(), "linear_act: bias must be [N] of x's type")
-        a.bias = bias.data_ptr()
-    out = torch.empty(*x.shape[:-1], n, dtype=out_dtype, device=dev)
+        _need(bias.dtype == dt and bias.shape == (n,) and bias.is_contiguous(), "linear_act: bias must be [N] of x's type")
+        b = bias.data_ptr()
+    out = x.new_empty((*lead, n), dtype=out_dtype)
     if m == 0:
         return out
-    a.x, a.ldx, a.w, a.ldw = x2.data_ptr(), x2.stride(0) if m > 1 else k, w.data_ptr(), w.stride(0) if n > 1 else k
-    a.out, a.ld_out, a.m, a.n, a.k = out.data_ptr(), n, m, n, k
-    a.dtype, a.out_dtype, a.act = _DTYPE_CODE[x.dtype], _DTYPE_CODE[out_dtype], ACTIVATIONS[act]
-    need = _lib.load().fb_linear_act_work_bytes(ctypes.addressof(a))
-    work = None
-    if need:
-        work = torch.empty(need, dtype=torch.uint8, device=dev)
-        a.work, a.work_bytes = work.data_ptr(), need
-    _launch(dev, "linear_act", 2.0 * m * n * k, (m * k + n * k) * 2 + m * n * out.element_size(),
-            lambda lib, st: lib.fb_linear_act(ctypes.addressof(a), st))
+    px, pw = x.data_ptr(), w.data_ptr()
+    work = need = 0
+    if (px | pw) % 16 or (ldx | ldw) % 8:
+        need = _lib.load().fb_linear_act_work_bytes(_lib.pack_linear_act(px, ldx, pw, ldw, *(0,) * 7, m, n, k, 0, 0, 0, 0))
+        copies = x.new_empty(need, dtype=torch.uint8)
+        work = copies.data_ptr()
+    _launch(index, "linear_act", 2.0 * m * n * k, (m * k + n * k) * 2 + m * n * out.element_size(), _lib.pack_linear_act(
+        px, ldx, pw, ldw, b, r, ldr, out.data_ptr(), n, work, need, m, n, k, _DTYPE_CODE[dt], res_code,
+        _DTYPE_CODE[out_dtype], ACTIVATIONS[act]))
     return out
 
 

@@ -609,15 +609,19 @@ def test_c_entries_refuse():
     t = _lib.FbRopeTensor(x.data_ptr(), x.data_ptr(), 64, 64, 64, 64, 64, 64, 1)
 
     def rope(count=1, dtype=_lib.FB_BF16, batch=1, seq=1, hd=64, ids=x.data_ptr(), idt=0, axes=1, dims=(64,), theta=(1e4,), pairs=0, tensor=t):
-        d, th = (ctypes.c_int32 * len(dims))(*dims), (ctypes.c_double * len(theta))(*theta)
-        return lib.fb_rope_axes(ctypes.addressof(tensor), count, dtype, batch, seq, hd, ids, idt, 0, 1, 1, axes, ctypes.addressof(d),
-                                ctypes.addressof(th), pairs, 0, None)
+        a = _lib.FbRopeArgs()
+        a.tensor[0] = a.tensor[1] = tensor
+        a.ids, a.ids_stride_l, a.ids_stride_a, a.ids_type = ids, 1, 1, idt
+        a.axes_dim[:len(dims)], a.theta[:len(theta)] = dims, theta
+        a.count, a.dtype, a.batch, a.seq, a.head_dim, a.axes, a.pairs = count, dtype, batch, seq, hd, axes, pairs
+        return lib.fb_rope_axes(ctypes.addressof(a), None)
 
     for kw in (dict(count=0), dict(count=3), dict(dtype=3), dict(batch=-1), dict(hd=32), dict(ids=None), dict(idt=4), dict(axes=0), dict(axes=9),
                dict(dims=(63,), hd=63), dict(dims=(0,), hd=0), dict(theta=(0.0,)), dict(theta=(float("nan"),)), dict(pairs=2), dict(hd=514, dims=(514,)),
                dict(batch=1 << 16, seq=1 << 16), dict(tensor=_lib.FbRopeTensor(None, x.data_ptr(), 64, 64, 64, 64, 64, 64, 1)),
                dict(tensor=_lib.FbRopeTensor(x.data_ptr(), x.data_ptr(), 64, 64, 64, 64, 64, 64, 0))):
         assert rope(**kw) != 0, kw
+    assert lib.fb_rope_axes(None, None) != 0
     torch.cuda.synchronize()
     assert not x.any()
 

@@ -35,7 +35,8 @@ def no_launch(monkeypatch):
     monkeypatch.setattr(ops, "_launch", launched)
 
 
-@pytest.mark.parametrize("struct,name", [(_lib.FbRopeTensor, "fb_rope_tensor"), (_lib.FbLayerNormArgs, "fb_layer_norm_args"),
+@pytest.mark.parametrize("struct,name", [(_lib.FbRopeTensor, "fb_rope_tensor"), (_lib.FbRopeArgs, "fb_rope_args"),
+                                         (_lib.FbLayerNormArgs, "fb_layer_norm_args"),
                                          (_lib.FbLinearActArgs, "fb_linear_act_args")])
 def test_struct_layouts_match_c(tmp_path, struct, name):
     fields = [f[0] for f in struct._fields_]
@@ -50,6 +51,24 @@ def test_struct_layouts_match_c(tmp_path, struct, name):
     assert int(got["size"]) == ctypes.sizeof(struct)
     for f in fields:
         assert int(got[f]) == getattr(struct, f).offset, f
+
+
+@pytest.mark.parametrize("struct,pack,n", [(_lib.FbRopeArgs, _lib.pack_rope, 47), (_lib.FbLayerNormArgs, _lib.pack_layer_norm, 28),
+                                           (_lib.FbLinearActArgs, _lib.pack_linear_act, 18)])
+def test_packed_arguments_fill_the_struct(struct, pack, n):
+    """Numbers 1..n packed in order land in the fields in order."""
+    def leaves(s):
+        for name, t in s._fields_:
+            v = getattr(s, name)
+            if isinstance(v, ctypes.Array):
+                for e in v:
+                    yield from leaves(e) if isinstance(e, ctypes.Structure) else (e,)
+            else:
+                yield v
+
+    raw = pack(*range(1, n + 1))
+    assert len(raw) == ctypes.sizeof(struct)
+    assert [int(v) for v in leaves(struct.from_buffer_copy(raw))] == list(range(1, n + 1))
 
 
 def test_cpu_tensors_are_refused():

@@ -76,6 +76,7 @@ DeviceState* current_device(std::string& err) {
   std::string msg = gemm_setup();
   if (msg.empty()) msg = attention_setup();
   if (msg.empty()) msg = linear_act_setup();
+  if (msg.empty()) msg = layer_norm_setup();
   if (!msg.empty()) {
     err = msg;
     return nullptr;

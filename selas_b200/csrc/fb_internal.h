@@ -88,5 +88,6 @@ int64_t linear_act_work_bytes(const fb_linear_act_args& args);
 std::string gemm_setup();
 std::string attention_setup();
 std::string linear_act_setup();
+std::string layer_norm_setup();
 
 }  // namespace fb

@@ -11,6 +11,8 @@
 // column sums dw and db stay in registers too (a thread owns the same columns of every row it takes), are joined
 // across the block's groups in shared memory, and go out as one fp32 partial row per block; a second kernel adds the
 // partials in a fixed order, so results do not depend on the order in which blocks run.
+#include <type_traits>
+
 #include "fb_internal.h"
 
 namespace fb {
@@ -29,6 +31,7 @@ struct Args {
   int64_t inner;                           // row = outer * inner + index
   int dim;
   int x_type, y_type, w_type;              // fb_dtype; y_type: y (forward) or dy
+  int depth, stage_bytes;                  // rows on their way to shared memory, and the bytes of one
   float w_plus;                            // w is read as w_plus + w (1 for adaLN's scale)
   float eps;
 };
@@ -94,6 +97,23 @@ __device__ __forceinline__ void store_chunk(void* p, int type, int64_t at, const
   }
 }
 
+// Widens CH elements that lie in shared memory or registers as raw bytes.
+__device__ __forceinline__ void widen4(const uint8_t* p, int type, float* f) {
+  if (type == FB_F32) {
+    const float4 v = *reinterpret_cast<const float4*>(p);
+    f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
+  } else if (type == FB_BF16) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    f[0] = __uint_as_float(u.x << 16), f[1] = __uint_as_float(u.x & 0xFFFF0000u);
+    f[2] = __uint_as_float(u.y << 16), f[3] = __uint_as_float(u.y & 0xFFFF0000u);
+  } else {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
+    const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+    f[0] = lo.x, f[1] = lo.y, f[2] = hi.x, f[3] = hi.y;
+  }
+}
+
 // The elements of a row that one thread of its group holds: NCH chunks of CH, chunk c at column CH * (t + GT * c);
 // zeros past the end. The type branch is outside the loop, so the loads of a row go out together.
 template <int GT, int NCH, int CH>
@@ -137,6 +157,63 @@ __device__ __forceinline__ void store_row(void* p, int type, int64_t base, int t
   }
 }
 
+// Asynchronous copy of a thread's own chunks of a row to its own places in shared memory, chunk c at
+// dst + c * T * bytes(chunk): no other thread reads them, so waiting for the copies needs no barrier.
+template <int GT, int NCH, int T>
+__device__ __forceinline__ void fetch_row(uint32_t dst, const void* p, int type, int64_t base, int t, int dim) {
+  if (type == FB_F32) {
+    const float* s = static_cast<const float*>(p) + base;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      const int col = 4 * (t + GT * c);
+      if (col < dim) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + c * T * 16), "l"(s + col) : "memory");
+    }
+  } else {
+    const uint16_t* s = static_cast<const uint16_t*>(p) + base;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      const int col = 4 * (t + GT * c);
+      if (col < dim) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst + c * T * 8), "l"(s + col) : "memory");
+    }
+  }
+}
+
+// The fetched row, widened.
+template <int GT, int NCH, int T>
+__device__ __forceinline__ void take_row(const uint8_t* src, int type, int t, int dim, float (&f)[NCH * 4]) {
+  auto each = [&](int ty, int bytes) {
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      if (4 * (t + GT * c) < dim) {
+        widen4(src + c * T * bytes, ty, f + 4 * c);
+      } else {
+        f[4 * c] = f[4 * c + 1] = f[4 * c + 2] = f[4 * c + 3] = 0.f;
+      }
+    }
+  };
+  if (type == FB_F32) {
+    each(FB_F32, 16);
+  } else if (type == FB_BF16) {
+    each(FB_BF16, 8);
+  } else {
+    each(FB_F16, 8);
+  }
+}
+
+__device__ __forceinline__ void commit_fetch() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Waits until at most `newer` of this thread's newest fetches are on their way (0..3).
+__device__ __forceinline__ void wait_fetch(int newer) {
+  if (newer == 0) {
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+  } else if (newer == 1) {
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+  } else if (newer == 2) {
+    asm volatile("cp.async.wait_group 2;" ::: "memory");
+  } else {
+    asm volatile("cp.async.wait_group 3;" ::: "memory");
+  }
+}
+
 // Sums of two values over a group of GT threads (all of them get both). One warp: shuffles. More: one entry per warp
 // in shared memory and a barrier of the group's own; `buf` alternates between calls, so one barrier per sum is enough.
 template <int GT>
@@ -164,111 +241,196 @@ constexpr int block_threads() {
   return GT < 256 ? 256 : GT;
 }
 
-// Forward: one group per row at a time.
-template <int GT, int NCH, int CH>
-__global__ void __launch_bounds__(block_threads<GT>()) fwd_kernel(const __grid_constant__ Args a) {
-  constexpr int E = NCH * CH, NG = block_threads<GT>() / GT;
-  __shared__ float2 slots[2 * NG * (GT / 32)];
-  const int group = threadIdx.x / GT, t = threadIdx.x % GT;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * NG + group;
-  if (row >= a.rows) return;  // whole groups
-  int buf = 0;
-  const int64_t o = row / a.inner, i = row - o * a.inner;
-  float x[E];
-  load_row<GT, NCH, CH>(a.x, a.x_type, o * a.xo + i * a.xi, t, a.dim, x);
-  const float inv = 1.0f / static_cast<float>(a.dim);
-  float s = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) s += x[e];
-  const float mean = group_sum2<GT>(s, 0.f, group, slots, buf).x * inv;
-  float q = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int col = CH * (t + GT * (e / CH));
-    x[e] = col < a.dim ? x[e] - mean : 0.f;
-    q += x[e] * x[e];
-  }
-  const float rstd = 1.0f / sqrtf(group_sum2<GT>(q, 0.f, group, slots, buf).x * inv + a.eps);
-  if (a.w != nullptr) {
-    float w[E];
-    load_row<GT, NCH, CH>(a.w, a.w_type, o * a.w_stride, t, a.dim, w);
-#pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = x[e] * rstd * (a.w_plus + w[e]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < E; ++e) x[e] *= rstd;
-  }
-  if (a.b != nullptr) {
-    float b[E];
-    load_row<GT, NCH, CH>(a.b, a.w_type, o * a.w_stride, t, a.dim, b);
-#pragma unroll
-    for (int e = 0; e < E; ++e) x[e] += b[e];
-  }
-  store_row<GT, NCH, CH>(a.out, a.y_type, o * a.oo + i * a.oi, t, a.dim, x);
+// Blocks per SM that a kernel is compiled (registers) and its grid and shared memory are sized for.
+template <int GT, int NCH, int CH, bool BWD>
+constexpr int blocks_per_sm() {
+  return GT >= 512 ? (GT == 512 && !BWD ? 2 : 1) : NCH * CH <= 8 ? 4 : NCH * CH <= 12 ? 3 : 2;
 }
 
-// Backward: block p of sum group blockIdx.y takes every (gridDim.x * groups)-th row of it.
+// One row of up to GT * NCH * CH elements per group of GT threads at a time; a group walks over rows
+// blockIdx.x * NG + group, + gridDim.x * NG, ... of sum group blockIdx.y, the next `depth` rows on their way to shared
+// memory while it works on one (CH == 4; the rows of odd sizes and alignments, CH == 1, are loaded where they are used).
 template <int GT, int NCH, int CH>
-__global__ void __launch_bounds__(block_threads<GT>()) bwd_kernel(const __grid_constant__ Args a) {
-  constexpr int E = NCH * CH, T = block_threads<GT>(), NG = T / GT;
+struct Walk {
+  static constexpr int T = block_threads<GT>(), NG = T / GT, E = NCH * CH;
+};
+
+template <int GT, int NCH, int CH>
+__global__ void __launch_bounds__(block_threads<GT>(), blocks_per_sm<GT, NCH, CH, false>())
+    fwd_kernel(const __grid_constant__ Args a) {
+  using W = Walk<GT, NCH, CH>;
+  constexpr int E = W::E, T = W::T, NG = W::NG;
+  extern __shared__ __align__(16) uint8_t ring[];
   __shared__ float2 slots[2 * NG * (GT / 32)];
-  __shared__ float join[NG > 1 ? T * E : 1];
   const int group = threadIdx.x / GT, t = threadIdx.x % GT;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * NG;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * NG + group;
+  const int xb = a.x_type == FB_F32 ? 16 : 8;  // bytes of a chunk
+  const uint8_t* mine = ring + threadIdx.x * xb;
+  auto fetch = [&](int64_t row, int stage) {
+    if (row < a.rows) {
+      const int64_t o = row / a.inner, i = row - o * a.inner;
+      fetch_row<GT, NCH, T>(smem_u32(mine) + stage * a.stage_bytes, a.x, a.x_type, o * a.xo + i * a.xi, t, a.dim);
+    }
+    commit_fetch();
+  };
+  if constexpr (CH == 4) {
+    for (int k = 0; k < a.depth; ++k) fetch(row0 + k * step, k);
+  }
   const float inv = 1.0f / static_cast<float>(a.dim);
-  int buf = 0;
-  float dw[E], db[E];
+  float w[E], b[E];
+  int64_t have = -1;  // the outer index whose w and b are in registers
+  int buf = 0, stage = 0;
+  for (int64_t row = row0; row < a.rows; row += step) {
+    const int64_t o = row / a.inner, i = row - o * a.inner;
+    if (have < 0 || (a.w_stride != 0 && have != o)) {
+      have = o;
+      if (a.w != nullptr) {
+        load_row<GT, NCH, CH>(a.w, a.w_type, o * a.w_stride, t, a.dim, w);
+#pragma unroll
+        for (int e = 0; e < E; ++e) w[e] += a.w_plus;
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) w[e] = 1.f;
+      }
+      if (a.b != nullptr) {
+        load_row<GT, NCH, CH>(a.b, a.w_type, o * a.w_stride, t, a.dim, b);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) b[e] = 0.f;
+      }
+    }
+    float x[E];
+    if constexpr (CH == 4) {
+      wait_fetch(a.depth - 1);
+      take_row<GT, NCH, T>(mine + stage * a.stage_bytes, a.x_type, t, a.dim, x);
+    } else {
+      load_row<GT, NCH, CH>(a.x, a.x_type, o * a.xo + i * a.xi, t, a.dim, x);
+    }
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) s += x[e];
+    const float mean = group_sum2<GT>(s, 0.f, group, slots, buf).x * inv;
+    if constexpr (CH == 4) {
+      fetch(row + a.depth * step, stage);  // the stage's values are in registers
+      if (++stage == a.depth) stage = 0;
+    }
+    float q = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int col = CH * (t + GT * (e / CH));
+      x[e] = col < a.dim ? x[e] - mean : 0.f;
+      q += x[e] * x[e];
+    }
+    const float rstd = 1.0f / sqrtf(group_sum2<GT>(q, 0.f, group, slots, buf).x * inv + a.eps);
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = (x[e] * rstd) * w[e] + b[e];
+    store_row<GT, NCH, CH>(a.out, a.y_type, o * a.oo + i * a.oi, t, a.dim, x);
+  }
+}
+
+template <int GT, int NCH, int CH>
+__global__ void __launch_bounds__(block_threads<GT>(), blocks_per_sm<GT, NCH, CH, true>())
+    bwd_kernel(const __grid_constant__ Args a) {
+  using W = Walk<GT, NCH, CH>;
+  constexpr int E = W::E, T = W::T, NG = W::NG;
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ float2 slots[2 * NG * (GT / 32)];
+  const int group = threadIdx.x / GT, t = threadIdx.x % GT;
+  const int64_t first = static_cast<int64_t>(blockIdx.y) * a.rows;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * NG;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * NG + group;
+  // a stage holds the block's chunks of x, then of dy, then of add
+  const int xb = a.x_type == FB_F32 ? 16 : 8, yb = a.y_type == FB_F32 ? 16 : 8;
+  const uint8_t* mx = ring + threadIdx.x * xb;
+  const uint8_t* my = ring + NCH * T * xb + threadIdx.x * yb;
+  const uint8_t* ma = ring + NCH * T * (xb + yb) + threadIdx.x * xb;
+  auto fetch = [&](int64_t r, int stage) {
+    if (r < a.rows) {
+      const int64_t row = first + r, o = row / a.inner, i = row - o * a.inner;
+      const int off = stage * a.stage_bytes;
+      fetch_row<GT, NCH, T>(smem_u32(mx) + off, a.x, a.x_type, o * a.xo + i * a.xi, t, a.dim);
+      fetch_row<GT, NCH, T>(smem_u32(my) + off, a.dy, a.y_type, o * a.yo + i * a.yi, t, a.dim);
+      if (a.add != nullptr) fetch_row<GT, NCH, T>(smem_u32(ma) + off, a.add, a.x_type, o * a.ao + i * a.ai, t, a.dim);
+    }
+    commit_fetch();
+  };
+  if constexpr (CH == 4) {
+    for (int k = 0; k < a.depth; ++k) fetch(r0 + k * step, k);
+  }
+  const float inv = 1.0f / static_cast<float>(a.dim);
+  int buf = 0, stage = 0;
+  float dw[E], db[E], w[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.f;
-  const int64_t first = static_cast<int64_t>(blockIdx.y) * a.rows;
-  for (int64_t r = static_cast<int64_t>(blockIdx.x) * NG + group; r < a.rows; r += static_cast<int64_t>(gridDim.x) * NG) {
+  int64_t have = -1;  // the outer index whose w is in registers
+  for (int64_t r = r0; r < a.rows; r += step) {
     const int64_t row = first + r, o = row / a.inner, i = row - o * a.inner;
+    if (have < 0 || (a.w_stride != 0 && have != o)) {
+      have = o;
+      if (a.w != nullptr) {
+        load_row<GT, NCH, CH>(a.w, a.w_type, o * a.w_stride, t, a.dim, w);
+#pragma unroll
+        for (int e = 0; e < E; ++e) w[e] += a.w_plus;
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) w[e] = 1.f;
+      }
+    }
     float x[E], g[E];
-    load_row<GT, NCH, CH>(a.x, a.x_type, o * a.xo + i * a.xi, t, a.dim, x);
-    load_row<GT, NCH, CH>(a.dy, a.y_type, o * a.yo + i * a.yi, t, a.dim, g);
-    float w[E];
-    if (a.w != nullptr) {
-      load_row<GT, NCH, CH>(a.w, a.w_type, o * a.w_stride, t, a.dim, w);
-#pragma unroll
-      for (int e = 0; e < E; ++e) w[e] += a.w_plus;
+    if constexpr (CH == 4) {
+      wait_fetch(a.depth - 1);
+      take_row<GT, NCH, T>(mx + stage * a.stage_bytes, a.x_type, t, a.dim, x);
+      take_row<GT, NCH, T>(my + stage * a.stage_bytes, a.y_type, t, a.dim, g);
     } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) w[e] = 1.f;
+      load_row<GT, NCH, CH>(a.x, a.x_type, o * a.xo + i * a.xi, t, a.dim, x);
+      load_row<GT, NCH, CH>(a.dy, a.y_type, o * a.yo + i * a.yi, t, a.dim, g);
     }
     float sx = 0.f, sg = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) sx += x[e], sg += g[e] * w[e];
     const float2 m = group_sum2<GT>(sx, sg, group, slots, buf);
-    const float mean = m.x * inv, gmean = m.y * inv;
+    const float mean = m.x * inv;
     float qx = 0.f, qg = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int col = CH * (t + GT * (e / CH));
       x[e] = col < a.dim ? x[e] - mean : 0.f;
       qx += x[e] * x[e];
-      qg += g[e] * w[e] * x[e];
+      qg += (g[e] * w[e]) * x[e];
     }
     const float2 v = group_sum2<GT>(qx, qg, group, slots, buf);
     const float rstd = 1.0f / sqrtf(v.x * inv + a.eps);
-    const float gx = v.y * inv * rstd;  // mean(g * xhat)
-    float dx[E];
+    // dx = rstd (g w - mean(g w) - xhat mean(g w xhat)), xhat = x rstd
+    const float k0 = rstd * m.y * inv, k1 = rstd * (v.y * inv * rstd);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const float h = x[e] * rstd;
+      x[e] = g[e] * w[e] * rstd - (k0 + h * k1);
       dw[e] += g[e] * h;
       db[e] += g[e];
-      dx[e] = rstd * (g[e] * w[e] - gmean - h * gx);
     }
     if (a.add != nullptr) {
       float ad[E];
-      load_row<GT, NCH, CH>(a.add, a.x_type, o * a.ao + i * a.ai, t, a.dim, ad);
+      if constexpr (CH == 4) {
+        take_row<GT, NCH, T>(ma + stage * a.stage_bytes, a.x_type, t, a.dim, ad);
+      } else {
+        load_row<GT, NCH, CH>(a.add, a.x_type, o * a.ao + i * a.ai, t, a.dim, ad);
+      }
 #pragma unroll
-      for (int e = 0; e < E; ++e) dx[e] += ad[e];
+      for (int e = 0; e < E; ++e) x[e] += ad[e];
     }
-    store_row<GT, NCH, CH>(a.out, a.x_type, o * a.oo + i * a.oi, t, a.dim, dx);
+    store_row<GT, NCH, CH>(a.out, a.x_type, o * a.oo + i * a.oi, t, a.dim, x);
+    if constexpr (CH == 4) {
+      fetch(r + a.depth * step, stage);  // every value of the stage has been used
+      if (++stage == a.depth) stage = 0;
+    }
   }
-  if (a.part == nullptr && a.dw == nullptr) return;
+  if (a.dw == nullptr) return;
+  if constexpr (CH == 4) wait_fetch(0);  // the ring is free
   // join the groups' sums, in the order of the groups
   if constexpr (NG > 1) {
+    float* join = reinterpret_cast<float*>(ring);
     for (int k = 0; k < 2; ++k) {
       __syncthreads();
 #pragma unroll
@@ -385,7 +547,7 @@ __global__ void __launch_bounds__(1024) bwd_wide_kernel(const __grid_constant__ 
     g += at(a.dy, a.y_type, yb + c) * weight(c) * d;
   });
   const float rstd = 1.0f / sqrtf(v.x * inv + a.eps), gx = v.y * inv * rstd;
-  if (threadIdx.x == 0 && a.part) a.part[2 * row] = mean, a.part[2 * row + 1] = rstd;
+  if (threadIdx.x == 0 && a.dw) a.part[2 * row] = mean, a.part[2 * row + 1] = rstd;
   for (int c = threadIdx.x; c < a.dim; c += 1024) {
     const float h = (at(a.x, a.x_type, xb + c) - mean) * rstd;
     float dx = rstd * (at(a.dy, a.y_type, yb + c) * weight(c) - gmean - h * gx);
@@ -422,33 +584,52 @@ __global__ void __launch_bounds__(256) sums_wide_kernel(const __grid_constant__ 
 
 // ---------------------------------------------------------------------------------------------- host
 
-// The group of threads for a row of `dim` elements: at most 16 elements a thread.
-static int group_threads(int dim) {
+static int size_of(int t) { return t == FB_F32 ? 4 : 2; }
+
+// The group of threads for a row of `dim` elements, and the chunks a thread holds: at most 5 chunks of 4 (vectors), or
+// 16 single elements. Fewer threads per row mean fewer barriers and more rows at once; more elements per thread than
+// 20 no longer leave registers for two blocks per SM in the backward pass.
+static int group_threads(int dim, bool vec) {
   int gt = 32;
-  while (gt * 16 < dim) gt *= 2;
+  while (gt * (vec ? 20 : 16) < dim && gt < 1024) gt *= 2;
   return gt;
 }
+static int block_groups(int gt) { return std::max(1, 256 / gt); }
+static int elements(int dim, int gt, bool vec) { return vec ? 4 * ((dim + 4 * gt - 1) / (4 * gt)) : 16; }
 
-// Blocks per sum group of the backward pass: enough groups of threads for every row, at most `kBwdBlocks` in all.
-constexpr int kBwdBlocks = 2 * kNumSms;
-static int64_t bwd_blocks(int64_t rows, int dim, int64_t sum_groups) {
-  const int gt = group_threads(dim), ng = std::max(1, 256 / gt);
-  const int64_t need = std::max<int64_t>(1, (rows + ng - 1) / ng);
-  return std::max<int64_t>(1, std::min(need, kBwdBlocks / std::max<int64_t>(1, sum_groups)));
+// Blocks per sum group of the backward pass: as many as are resident at once, so that each walks over its share of the
+// rows and leaves one partial sum; fewer where there are fewer rows than groups of threads.
+static int64_t bwd_blocks(int64_t rows, int dim, int64_t sum_groups, bool vec) {
+  const int gt = group_threads(dim, vec), e = elements(dim, gt, vec);
+  const int per_sm = gt >= 512 ? 1 : e <= 8 ? 4 : e <= 12 ? 3 : 2;
+  const int64_t need = std::max<int64_t>(1, (rows + block_groups(gt) - 1) / block_groups(gt));
+  return std::max<int64_t>(1, std::min<int64_t>(need, per_sm * kNumSms / std::max<int64_t>(1, sum_groups)));
 }
 
+constexpr int kRingPerSm = 200 * 1024;  // shared memory of an SM that the rows on their way may take
+
 template <int GT, int NCH, int CH>
-static cudaError_t go(const Args& a, bool bwd, int64_t sum_groups, cudaStream_t st) {
+static cudaError_t go(Args a, bool bwd, int64_t sum_groups, cudaStream_t st) {
   constexpr int T = block_threads<GT>(), NG = T / GT;
+  const int per_sm = bwd ? blocks_per_sm<GT, NCH, CH, true>() : blocks_per_sm<GT, NCH, CH, false>();
+  int smem = 0;
+  if (CH == 4) {
+    const int xb = size_of(a.x_type), yb = size_of(a.y_type);
+    a.stage_bytes = 4 * NCH * T * (bwd ? xb + yb + (a.add ? xb : 0) : xb);
+    a.depth = std::max(1, std::min(4, kRingPerSm / per_sm / a.stage_bytes));
+    smem = a.depth * a.stage_bytes;
+  }
+  if (bwd && NG > 1) smem = std::max(smem, NCH * CH * T * 4);  // the groups' sums
   if (!bwd) {
-    fwd_kernel<GT, NCH, CH><<<static_cast<unsigned>((a.rows + NG - 1) / NG), T, 0, st>>>(a);
+    const int64_t need = (a.rows + NG - 1) / NG;
+    fwd_kernel<GT, NCH, CH><<<static_cast<unsigned>(std::min<int64_t>(need, per_sm * kNumSms)), T, smem, st>>>(a);
     return cudaGetLastError();
   }
-  const int64_t blocks = bwd_blocks(a.rows, a.dim, sum_groups);
+  const int64_t blocks = bwd_blocks(a.rows, a.dim, sum_groups, CH == 4);
   const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(sum_groups));
-  bwd_kernel<GT, NCH, CH><<<grid, T, 0, st>>>(a);
+  bwd_kernel<GT, NCH, CH><<<grid, T, smem, st>>>(a);
   cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess && a.part != nullptr && blocks > 1) {
+  if (e == cudaSuccess && a.dw != nullptr && blocks > 1) {
     const dim3 jg(static_cast<unsigned>((2ll * a.dim + 31) / 32), static_cast<unsigned>(sum_groups));
     join_kernel<<<jg, 256, 0, st>>>(a.part, static_cast<int>(blocks), a.dim, a.dw, a.db);
     e = cudaGetLastError();
@@ -456,14 +637,23 @@ static cudaError_t go(const Args& a, bool bwd, int64_t sum_groups, cudaStream_t 
   return e;
 }
 
-template <int GT>
-static cudaError_t go_gt(const Args& a, bool bwd, int64_t sum_groups, bool vec, cudaStream_t st) {
-  if (!vec) return go<GT, 16, 1>(a, bwd, sum_groups, st);
-  switch ((a.dim + 4 * GT - 1) / (4 * GT)) {
-    case 1: return go<GT, 1, 4>(a, bwd, sum_groups, st);
-    case 2: return go<GT, 2, 4>(a, bwd, sum_groups, st);
-    case 3: return go<GT, 3, 4>(a, bwd, sum_groups, st);
-    default: return go<GT, 4, 4>(a, bwd, sum_groups, st);
+// Raises the shared-memory limits of one instance (ring of up to kRingPerSm bytes).
+template <int GT, int NCH, int CH>
+static cudaError_t setup_one() {
+  const cudaError_t e = cudaFuncSetAttribute(fwd_kernel<GT, NCH, CH>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingPerSm);
+  return e != cudaSuccess ? e : cudaFuncSetAttribute(bwd_kernel<GT, NCH, CH>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingPerSm);
+}
+
+template <int GT, typename F>
+static cudaError_t with_chunks(int dim, bool vec, F f) {
+  if (!vec) return f(std::integral_constant<int, 16>(), std::integral_constant<int, 1>());
+  using Four = std::integral_constant<int, 4>;
+  switch ((dim + 4 * GT - 1) / (4 * GT)) {
+    case 1: return f(std::integral_constant<int, 1>(), Four());
+    case 2: return f(std::integral_constant<int, 2>(), Four());
+    case 3: return f(std::integral_constant<int, 3>(), Four());
+    case 4: return f(std::integral_constant<int, 4>(), Four());
+    default: return f(std::integral_constant<int, GT < 1024 ? 5 : 4>(), Four());  // 1024 threads hold kMaxDimRegs in 4
   }
 }
 
@@ -475,24 +665,40 @@ static cudaError_t dispatch(const Args& a, bool bwd, int64_t sum_groups, bool ve
     }
     bwd_wide_kernel<<<static_cast<unsigned>(a.rows * sum_groups), 1024, 0, st>>>(a);
     cudaError_t e = cudaGetLastError();
-    if (e == cudaSuccess && a.part != nullptr) {
+    if (e == cudaSuccess && a.dw != nullptr) {
       sums_wide_kernel<<<dim3((a.dim + 31) / 32, static_cast<unsigned>(sum_groups)), 256, 0, st>>>(a);
       e = cudaGetLastError();
     }
     return e;
   }
-  switch (group_threads(a.dim)) {
-    case 32: return go_gt<32>(a, bwd, sum_groups, vec, st);
-    case 64: return go_gt<64>(a, bwd, sum_groups, vec, st);
-    case 128: return go_gt<128>(a, bwd, sum_groups, vec, st);
-    case 256: return go_gt<256>(a, bwd, sum_groups, vec, st);
-    case 512: return go_gt<512>(a, bwd, sum_groups, vec, st);
-    default: return go_gt<1024>(a, bwd, sum_groups, vec, st);
+  auto run = [&](auto gt) {
+    constexpr int GT = decltype(gt)::value;
+    return with_chunks<GT>(a.dim, vec, [&](auto nch, auto ch) {
+      return go<GT, decltype(nch)::value, decltype(ch)::value>(a, bwd, sum_groups, st);
+    });
+  };
+  switch (group_threads(a.dim, vec)) {
+    case 32: return run(std::integral_constant<int, 32>());
+    case 64: return run(std::integral_constant<int, 64>());
+    case 128: return run(std::integral_constant<int, 128>());
+    case 256: return run(std::integral_constant<int, 256>());
+    case 512: return run(std::integral_constant<int, 512>());
+    default: return run(std::integral_constant<int, 1024>());
   }
 }
 
+template <int GT>
+static cudaError_t setup_gt() {
+  cudaError_t e = setup_one<GT, 16, 1>();
+  if (e == cudaSuccess) e = setup_one<GT, 1, 4>();
+  if (e == cudaSuccess) e = setup_one<GT, 2, 4>();
+  if (e == cudaSuccess) e = setup_one<GT, 3, 4>();
+  if (e == cudaSuccess) e = setup_one<GT, 4, 4>();
+  if constexpr (GT < 1024) e = e == cudaSuccess ? setup_one<GT, 5, 4>() : e;
+  return e;
+}
+
 static bool is_dtype(int t) { return t == FB_F32 || t == FB_F16 || t == FB_BF16; }
-static int size_of(int t) { return t == FB_F32 ? 4 : 2; }
 // Whether chunks of four elements of this tensor are aligned vectors.
 static bool vec4(const void* p, int type, std::initializer_list<int64_t> strides) {
   if (reinterpret_cast<uintptr_t>(p) % (4 * size_of(type)) != 0) return false;
@@ -504,11 +710,23 @@ static bool misaligned(const void* p, int type) { return reinterpret_cast<uintpt
 
 }  // namespace norm
 
+std::string layer_norm_setup() {
+  cudaError_t e = norm::setup_gt<32>();
+  if (e == cudaSuccess) e = norm::setup_gt<64>();
+  if (e == cudaSuccess) e = norm::setup_gt<128>();
+  if (e == cudaSuccess) e = norm::setup_gt<256>();
+  if (e == cudaSuccess) e = norm::setup_gt<512>();
+  if (e == cudaSuccess) e = norm::setup_gt<1024>();
+  return e == cudaSuccess ? std::string() : std::string("cudaFuncSetAttribute(layer_norm): ") + cudaGetErrorString(e);
+}
+
 int64_t layer_norm_work_floats(int64_t outer, int64_t inner, int32_t dim, int32_t per_outer) {
   const int64_t rows = per_outer ? inner : outer * inner, groups = per_outer ? outer : 1;
   if (rows <= 0 || groups <= 0 || dim <= 0) return 0;
   if (dim > norm::kMaxDimRegs) return 2 * rows * groups;
-  const int64_t blocks = norm::bwd_blocks(rows, dim, groups);
+  // which of the two layouts runs depends on alignments that are not known here: room for either
+  const int64_t blocks = std::max(norm::bwd_blocks(rows, dim, groups, false),
+                                  dim % 4 == 0 ? norm::bwd_blocks(rows, dim, groups, true) : 1);
   return blocks > 1 ? groups * blocks * 2 * dim : 0;
 }
 
@@ -571,7 +789,7 @@ int launch_layer_norm(const fb_layer_norm_args& p, bool bwd, cudaStream_t st, st
   if (sums) {
     const int64_t need = layer_norm_work_floats(p.outer, p.inner, p.dim, p.sum_per_outer);
     if (p.work_floats < need || (need > 0 && !p.work)) return bad(FB_ERR_ARG, "workspace too small");
-    a.part = need > 0 ? p.work : nullptr;
+    a.part = p.work;
     a.dw = p.dweight;
     a.db = p.dbias;
   }

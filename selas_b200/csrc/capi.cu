@@ -77,6 +77,7 @@ DeviceState* current_device(std::string& err) {
   if (msg.empty()) msg = attention_setup();
   if (msg.empty()) msg = linear_act_setup();
   if (msg.empty()) msg = layer_norm_setup();
+  if (msg.empty()) msg = rope_axes_setup();
   if (!msg.empty()) {
     err = msg;
     return nullptr;

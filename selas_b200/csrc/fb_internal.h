@@ -89,5 +89,6 @@ std::string gemm_setup();
 std::string attention_setup();
 std::string linear_act_setup();
 std::string layer_norm_setup();
+std::string rope_axes_setup();
 
 }  // namespace fb

@@ -27,14 +27,69 @@ struct Args {
   float *part, *dw, *db;  // partials [sum group][block][2][dim]; with one block per group dw and db are written directly
   int64_t xo, xi, yo, yi, ao, ai, oo, oi;  // strides of x, dy, add, out: outer index, inner index (elements)
   int64_t w_stride;                        // of w and b per outer index (0: shared)
-  int64_t rows;                            // rows of a sum group (forward: all rows)
-  int64_t inner;                           // row = outer * inner + index
+  int rows;                                // rows of a sum group (forward: all rows)
+  int inner;                               // row = outer * inner + index
   int dim;
   int x_type, y_type, w_type;              // fb_dtype; y_type: y (forward) or dy
   int depth, stage_bytes;                  // rows on their way to shared memory, and the bytes of one
+  int add_staged;                          // add is one of what comes that way
   float w_plus;                            // w is read as w_plus + w (1 for adaLN's scale)
   float eps;
 };
+
+// Two fp32 values in one 64-bit register: Blackwell's packed arithmetic does both in one instruction, and the norms'
+// inner loops are bound by instruction issue before they are by the arithmetic.
+typedef uint64_t f2;
+__device__ __forceinline__ f2 pack2(float lo, float hi) {
+  f2 v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ float2 unpack2(f2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ float total(f2 v) {
+  const float2 r = unpack2(v);
+  return r.x + r.y;
+}
+
+// Where a group is in its walk over rows: row = outer * inner + index, advanced by a fixed step without divisions.
+struct Place {
+  int row, o, i;
+};
+__device__ __forceinline__ Place place_of(const Args& a, int first, int row) {
+  const int all = first + row;
+  return {row, all / a.inner, all % a.inner};
+}
+struct Step {
+  int rows, o, i;
+};
+__device__ __forceinline__ void advance(Place& p, const Step& s, int inner) {
+  p.row += s.rows;
+  p.o += s.o;
+  p.i += s.i;
+  if (p.i >= inner) {
+    p.i -= inner;
+    ++p.o;
+  }
+}
 
 // CH consecutive elements (4: one vector access, 1: any alignment) widened to fp32.
 template <int CH>
@@ -244,7 +299,7 @@ constexpr int block_threads() {
 // Blocks per SM that a kernel is compiled (registers) and its grid and shared memory are sized for.
 template <int GT, int NCH, int CH, bool BWD>
 constexpr int blocks_per_sm() {
-  return GT >= 512 ? (GT == 512 && !BWD ? 2 : 1) : NCH * CH <= 8 ? 4 : NCH * CH <= 12 ? 3 : 2;
+  return GT >= 512 ? (GT == 512 && !BWD ? 2 : 1) : NCH * CH <= 4 ? 4 : NCH * CH <= 12 ? 3 : 2;
 }
 
 // One row of up to GT * NCH * CH elements per group of GT threads at a time; a group walks over rows
@@ -252,80 +307,125 @@ constexpr int blocks_per_sm() {
 // memory while it works on one (CH == 4; the rows of odd sizes and alignments, CH == 1, are loaded where they are used).
 template <int GT, int NCH, int CH>
 struct Walk {
-  static constexpr int T = block_threads<GT>(), NG = T / GT, E = NCH * CH;
+  static constexpr int T = block_threads<GT>(), NG = T / GT, E = NCH * CH, P = E / 2;
+  // Pair k of a thread's elements lies in the chunks of columns 2k .. 2k + 1; both are inside the row or both past its
+  // end for chunks of four, each by itself for single elements.
+  static __device__ __forceinline__ int column(int t, int e) { return CH * (t + GT * (e / CH)) + e % CH; }
+  static __device__ __forceinline__ f2 inside(int t, int k, int dim, float v) {
+    if constexpr (CH == 4) {
+      const float m = column(t, 2 * k) < dim ? v : 0.f;
+      return pack2(m, m);
+    } else {
+      return pack2(column(t, 2 * k) < dim ? v : 0.f, column(t, 2 * k + 1) < dim ? v : 0.f);
+    }
+  }
+  static __device__ __forceinline__ void pairs(const float (&f)[E], f2 (&v)[P]) {
+#pragma unroll
+    for (int k = 0; k < P; ++k) v[k] = pack2(f[2 * k], f[2 * k + 1]);
+  }
+  static __device__ __forceinline__ void load(const void* p, int type, int64_t base, int t, int dim, f2 (&v)[P]) {
+    float f[E];
+    load_row<GT, NCH, CH>(p, type, base, t, dim, f);
+    pairs(f, v);
+  }
+  static __device__ __forceinline__ void take(const uint8_t* src, int type, int t, int dim, f2 (&v)[P]) {
+    if constexpr (CH == 4) {
+      float f[E];
+      take_row<GT, NCH, T>(src, type, t, dim, f);
+      pairs(f, v);
+    }
+  }
+  static __device__ __forceinline__ void store(void* p, int type, int64_t base, int t, int dim, const f2 (&v)[P]) {
+    float f[E];
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+      const float2 r = unpack2(v[k]);
+      f[2 * k] = r.x, f[2 * k + 1] = r.y;
+    }
+    store_row<GT, NCH, CH>(p, type, base, t, dim, f);
+  }
+  // A thread's own pairs in shared memory, two to a 16-byte place.
+  static __device__ __forceinline__ void keep(ulonglong2* at, const f2 (&v)[P]) {
+#pragma unroll
+    for (int k = 0; k < P; k += 2) at[(k / 2) * T] = make_ulonglong2(v[k], v[k + 1]);
+  }
+  // w of outer index o, as it multiplies: w_plus + w, or ones
+  static __device__ __forceinline__ void weight(const Args& a, int o, int t, f2 (&w)[P]) {
+    if (a.w != nullptr) {
+      load(a.w, a.w_type, o * a.w_stride, t, a.dim, w);
+      const f2 plus = pack2(a.w_plus, a.w_plus);
+#pragma unroll
+      for (int k = 0; k < P; ++k) w[k] = add2(w[k], plus);
+    } else {
+#pragma unroll
+      for (int k = 0; k < P; ++k) w[k] = pack2(1.f, 1.f);
+    }
+  }
 };
 
 template <int GT, int NCH, int CH>
 __global__ void __launch_bounds__(block_threads<GT>(), blocks_per_sm<GT, NCH, CH, false>())
     fwd_kernel(const __grid_constant__ Args a) {
   using W = Walk<GT, NCH, CH>;
-  constexpr int E = W::E, T = W::T, NG = W::NG;
+  constexpr int P = W::P, T = W::T, NG = W::NG;
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ float2 slots[2 * NG * (GT / 32)];
   const int group = threadIdx.x / GT, t = threadIdx.x % GT;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * NG;
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * NG + group;
-  const int xb = a.x_type == FB_F32 ? 16 : 8;  // bytes of a chunk
-  const uint8_t* mine = ring + threadIdx.x * xb;
-  auto fetch = [&](int64_t row, int stage) {
-    if (row < a.rows) {
-      const int64_t o = row / a.inner, i = row - o * a.inner;
-      fetch_row<GT, NCH, T>(smem_u32(mine) + stage * a.stage_bytes, a.x, a.x_type, o * a.xo + i * a.xi, t, a.dim);
+  const int rows_step = gridDim.x * NG;
+  const Step step = {rows_step, rows_step / a.inner, rows_step % a.inner};
+  const uint8_t* mine = ring + threadIdx.x * (a.x_type == FB_F32 ? 16 : 8);
+  Place at = place_of(a, 0, blockIdx.x * NG + group), ahead = at;
+  auto fetch = [&](int stage) {
+    if (ahead.row < a.rows) {
+      fetch_row<GT, NCH, T>(smem_u32(mine) + stage * a.stage_bytes, a.x, a.x_type, ahead.o * a.xo + ahead.i * a.xi, t, a.dim);
     }
     commit_fetch();
+    advance(ahead, step, a.inner);
   };
   if constexpr (CH == 4) {
-    for (int k = 0; k < a.depth; ++k) fetch(row0 + k * step, k);
+    for (int k = 0; k < a.depth; ++k) fetch(k);
   }
   const float inv = 1.0f / static_cast<float>(a.dim);
-  float w[E], b[E];
-  int64_t have = -1;  // the outer index whose w and b are in registers
+  f2 w[P], b[P];
+  int have = -1;  // the outer index whose w and b are in registers
   int buf = 0, stage = 0;
-  for (int64_t row = row0; row < a.rows; row += step) {
-    const int64_t o = row / a.inner, i = row - o * a.inner;
-    if (have < 0 || (a.w_stride != 0 && have != o)) {
-      have = o;
-      if (a.w != nullptr) {
-        load_row<GT, NCH, CH>(a.w, a.w_type, o * a.w_stride, t, a.dim, w);
-#pragma unroll
-        for (int e = 0; e < E; ++e) w[e] += a.w_plus;
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) w[e] = 1.f;
-      }
+  for (; at.row < a.rows; advance(at, step, a.inner)) {
+    if (have < 0 || (a.w_stride != 0 && have != at.o)) {
+      have = at.o;
+      W::weight(a, at.o, t, w);
       if (a.b != nullptr) {
-        load_row<GT, NCH, CH>(a.b, a.w_type, o * a.w_stride, t, a.dim, b);
+        W::load(a.b, a.w_type, at.o * a.w_stride, t, a.dim, b);
       } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e) b[e] = 0.f;
+        for (int k = 0; k < P; ++k) b[k] = pack2(0.f, 0.f);
       }
     }
-    float x[E];
+    f2 x[P];
     if constexpr (CH == 4) {
       wait_fetch(a.depth - 1);
-      take_row<GT, NCH, T>(mine + stage * a.stage_bytes, a.x_type, t, a.dim, x);
+      W::take(mine + stage * a.stage_bytes, a.x_type, t, a.dim, x);
     } else {
-      load_row<GT, NCH, CH>(a.x, a.x_type, o * a.xo + i * a.xi, t, a.dim, x);
+      W::load(a.x, a.x_type, at.o * a.xo + at.i * a.xi, t, a.dim, x);
     }
-    float s = 0.f;
+    f2 s = pack2(0.f, 0.f);
 #pragma unroll
-    for (int e = 0; e < E; ++e) s += x[e];
-    const float mean = group_sum2<GT>(s, 0.f, group, slots, buf).x * inv;
+    for (int k = 0; k < P; ++k) s = add2(s, x[k]);
+    const float mean = group_sum2<GT>(total(s), 0.f, group, slots, buf).x * inv;
     if constexpr (CH == 4) {
-      fetch(row + a.depth * step, stage);  // the stage's values are in registers
+      fetch(stage);  // the stage's values are in registers
       if (++stage == a.depth) stage = 0;
     }
-    float q = 0.f;
+    f2 q = pack2(0.f, 0.f);
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int col = CH * (t + GT * (e / CH));
-      x[e] = col < a.dim ? x[e] - mean : 0.f;
-      q += x[e] * x[e];
+    for (int k = 0; k < P; ++k) {
+      x[k] = add2(x[k], W::inside(t, k, a.dim, -mean));
+      q = fma2(x[k], x[k], q);
     }
-    const float rstd = 1.0f / sqrtf(group_sum2<GT>(q, 0.f, group, slots, buf).x * inv + a.eps);
+    const float rstd = 1.0f / sqrtf(group_sum2<GT>(total(q), 0.f, group, slots, buf).x * inv + a.eps);
+    const f2 r = pack2(rstd, rstd);
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = (x[e] * rstd) * w[e] + b[e];
-    store_row<GT, NCH, CH>(a.out, a.y_type, o * a.oo + i * a.oi, t, a.dim, x);
+    for (int k = 0; k < P; ++k) x[k] = fma2(mul2(x[k], r), w[k], b[k]);
+    W::store(a.out, a.y_type, at.o * a.oo + at.i * a.oi, t, a.dim, x);
   }
 }
 
@@ -333,96 +433,105 @@ template <int GT, int NCH, int CH>
 __global__ void __launch_bounds__(block_threads<GT>(), blocks_per_sm<GT, NCH, CH, true>())
     bwd_kernel(const __grid_constant__ Args a) {
   using W = Walk<GT, NCH, CH>;
-  constexpr int E = W::E, T = W::T, NG = W::NG;
+  constexpr int E = W::E, P = W::P, T = W::T, NG = W::NG;
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ float2 slots[2 * NG * (GT / 32)];
   const int group = threadIdx.x / GT, t = threadIdx.x % GT;
-  const int64_t first = static_cast<int64_t>(blockIdx.y) * a.rows;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * NG;
-  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * NG + group;
+  const int rows_step = gridDim.x * NG;
+  const Step step = {rows_step, rows_step / a.inner, rows_step % a.inner};
   // a stage holds the block's chunks of x, then of dy, then of add
   const int xb = a.x_type == FB_F32 ? 16 : 8, yb = a.y_type == FB_F32 ? 16 : 8;
   const uint8_t* mx = ring + threadIdx.x * xb;
   const uint8_t* my = ring + NCH * T * xb + threadIdx.x * yb;
   const uint8_t* ma = ring + NCH * T * (xb + yb) + threadIdx.x * xb;
-  auto fetch = [&](int64_t r, int stage) {
-    if (r < a.rows) {
-      const int64_t row = first + r, o = row / a.inner, i = row - o * a.inner;
+  Place at = place_of(a, blockIdx.y * a.rows, blockIdx.x * NG + group), ahead = at;
+  auto fetch = [&](int stage) {
+    if (ahead.row < a.rows) {
       const int off = stage * a.stage_bytes;
-      fetch_row<GT, NCH, T>(smem_u32(mx) + off, a.x, a.x_type, o * a.xo + i * a.xi, t, a.dim);
-      fetch_row<GT, NCH, T>(smem_u32(my) + off, a.dy, a.y_type, o * a.yo + i * a.yi, t, a.dim);
-      if (a.add != nullptr) fetch_row<GT, NCH, T>(smem_u32(ma) + off, a.add, a.x_type, o * a.ao + i * a.ai, t, a.dim);
+      fetch_row<GT, NCH, T>(smem_u32(mx) + off, a.x, a.x_type, ahead.o * a.xo + ahead.i * a.xi, t, a.dim);
+      fetch_row<GT, NCH, T>(smem_u32(my) + off, a.dy, a.y_type, ahead.o * a.yo + ahead.i * a.yi, t, a.dim);
+      if (a.add_staged)
+        fetch_row<GT, NCH, T>(smem_u32(ma) + off, a.add, a.x_type, ahead.o * a.ao + ahead.i * a.ai, t, a.dim);
     }
     commit_fetch();
+    advance(ahead, step, a.inner);
   };
   if constexpr (CH == 4) {
-    for (int k = 0; k < a.depth; ++k) fetch(r0 + k * step, k);
+    for (int k = 0; k < a.depth; ++k) fetch(k);
   }
   const float inv = 1.0f / static_cast<float>(a.dim);
   int buf = 0, stage = 0;
-  float dw[E], db[E], w[E];
+  f2 dw[P], db[P];
 #pragma unroll
-  for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.f;
-  int64_t have = -1;  // the outer index whose w is in registers
-  for (int64_t r = r0; r < a.rows; r += step) {
-    const int64_t row = first + r, o = row / a.inner, i = row - o * a.inner;
-    if (have < 0 || (a.w_stride != 0 && have != o)) {
-      have = o;
-      if (a.w != nullptr) {
-        load_row<GT, NCH, CH>(a.w, a.w_type, o * a.w_stride, t, a.dim, w);
-#pragma unroll
-        for (int e = 0; e < E; ++e) w[e] += a.w_plus;
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) w[e] = 1.f;
-      }
+  for (int k = 0; k < P; ++k) dw[k] = db[k] = pack2(0.f, 0.f);
+  // w waits in shared memory: the sums need its registers
+  ulonglong2* ws = reinterpret_cast<ulonglong2*>(ring + (CH == 4 ? a.depth * a.stage_bytes : 0)) + threadIdx.x;
+  int have = -1;  // the outer index whose w that is
+  for (; at.row < a.rows; advance(at, step, a.inner)) {
+    if (have < 0 || (a.w_stride != 0 && have != at.o)) {
+      have = at.o;
+      f2 w[P];
+      W::weight(a, at.o, t, w);
+      W::keep(ws, w);
     }
-    float x[E], g[E];
+    f2 x[P], g[P];
     if constexpr (CH == 4) {
       wait_fetch(a.depth - 1);
-      take_row<GT, NCH, T>(mx + stage * a.stage_bytes, a.x_type, t, a.dim, x);
-      take_row<GT, NCH, T>(my + stage * a.stage_bytes, a.y_type, t, a.dim, g);
+      W::take(mx + stage * a.stage_bytes, a.x_type, t, a.dim, x);
+      W::take(my + stage * a.stage_bytes, a.y_type, t, a.dim, g);
     } else {
-      load_row<GT, NCH, CH>(a.x, a.x_type, o * a.xo + i * a.xi, t, a.dim, x);
-      load_row<GT, NCH, CH>(a.dy, a.y_type, o * a.yo + i * a.yi, t, a.dim, g);
+      W::load(a.x, a.x_type, at.o * a.xo + at.i * a.xi, t, a.dim, x);
+      W::load(a.dy, a.y_type, at.o * a.yo + at.i * a.yi, t, a.dim, g);
     }
-    float sx = 0.f, sg = 0.f;
+    f2 sx = pack2(0.f, 0.f), sg = sx;
 #pragma unroll
-    for (int e = 0; e < E; ++e) sx += x[e], sg += g[e] * w[e];
-    const float2 m = group_sum2<GT>(sx, sg, group, slots, buf);
+    for (int k = 0; k < P; k += 2) {
+      const ulonglong2 w = ws[(k / 2) * T];
+      sx = add2(add2(sx, x[k]), x[k + 1]);
+      sg = fma2(g[k + 1], w.y, fma2(g[k], w.x, sg));
+    }
+    const float2 m = group_sum2<GT>(total(sx), total(sg), group, slots, buf);
     const float mean = m.x * inv;
-    float qx = 0.f, qg = 0.f;
+    f2 qx = pack2(0.f, 0.f), qg = qx;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int col = CH * (t + GT * (e / CH));
-      x[e] = col < a.dim ? x[e] - mean : 0.f;
-      qx += x[e] * x[e];
-      qg += (g[e] * w[e]) * x[e];
+    for (int k = 0; k < P; k += 2) {
+      const ulonglong2 w = ws[(k / 2) * T];
+#pragma unroll
+      for (int j = k; j < k + 2; ++j) {
+        x[j] = add2(x[j], W::inside(t, j, a.dim, -mean));
+        qx = fma2(x[j], x[j], qx);
+        qg = fma2(mul2(g[j], j == k ? w.x : w.y), x[j], qg);
+      }
     }
-    const float2 v = group_sum2<GT>(qx, qg, group, slots, buf);
+    const float2 v = group_sum2<GT>(total(qx), total(qg), group, slots, buf);
     const float rstd = 1.0f / sqrtf(v.x * inv + a.eps);
     // dx = rstd (g w - mean(g w) - xhat mean(g w xhat)), xhat = x rstd
-    const float k0 = rstd * m.y * inv, k1 = rstd * (v.y * inv * rstd);
+    const float c0 = -rstd * m.y * inv, c1 = -rstd * (v.y * inv * rstd);
+    const f2 r = pack2(rstd, rstd), k0 = pack2(c0, c0), k1 = pack2(c1, c1);
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float h = x[e] * rstd;
-      x[e] = g[e] * w[e] * rstd - (k0 + h * k1);
-      dw[e] += g[e] * h;
-      db[e] += g[e];
+    for (int k = 0; k < P; k += 2) {
+      const ulonglong2 w = ws[(k / 2) * T];
+#pragma unroll
+      for (int j = k; j < k + 2; ++j) {
+        const f2 h = mul2(x[j], r);
+        x[j] = fma2(mul2(g[j], j == k ? w.x : w.y), r, fma2(h, k1, k0));
+        dw[j] = fma2(g[j], h, dw[j]);
+        db[j] = add2(db[j], g[j]);
+      }
     }
     if (a.add != nullptr) {
-      float ad[E];
-      if constexpr (CH == 4) {
-        take_row<GT, NCH, T>(ma + stage * a.stage_bytes, a.x_type, t, a.dim, ad);
+      f2 ad[P];
+      if (CH == 4 && a.add_staged) {
+        W::take(ma + stage * a.stage_bytes, a.x_type, t, a.dim, ad);
       } else {
-        load_row<GT, NCH, CH>(a.add, a.x_type, o * a.ao + i * a.ai, t, a.dim, ad);
+        W::load(a.add, a.x_type, at.o * a.ao + at.i * a.ai, t, a.dim, ad);
       }
 #pragma unroll
-      for (int e = 0; e < E; ++e) x[e] += ad[e];
+      for (int k = 0; k < P; ++k) x[k] = add2(x[k], ad[k]);
     }
-    store_row<GT, NCH, CH>(a.out, a.x_type, o * a.oo + i * a.oi, t, a.dim, x);
+    W::store(a.out, a.x_type, at.o * a.oo + at.i * a.oi, t, a.dim, x);
     if constexpr (CH == 4) {
-      fetch(r + a.depth * step, stage);  // every value of the stage has been used
+      fetch(stage);  // every value of the stage has been used
       if (++stage == a.depth) stage = 0;
     }
   }
@@ -430,18 +539,18 @@ __global__ void __launch_bounds__(block_threads<GT>(), blocks_per_sm<GT, NCH, CH
   if constexpr (CH == 4) wait_fetch(0);  // the ring is free
   // join the groups' sums, in the order of the groups
   if constexpr (NG > 1) {
-    float* join = reinterpret_cast<float*>(ring);
-    for (int k = 0; k < 2; ++k) {
+    f2* join = reinterpret_cast<f2*>(ring);
+    for (int s = 0; s < 2; ++s) {
       __syncthreads();
 #pragma unroll
-      for (int e = 0; e < E; ++e) join[e * T + threadIdx.x] = k ? db[e] : dw[e];
+      for (int k = 0; k < P; ++k) join[k * T + threadIdx.x] = s ? db[k] : dw[k];
       __syncthreads();
       if (group == 0) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          float s = 0.f;
-          for (int n = 0; n < NG; ++n) s += join[e * T + n * GT + t];
-          (k ? db[e] : dw[e]) = s;
+        for (int k = 0; k < P; ++k) {
+          f2 v = join[k * T + t];
+          for (int n = 1; n < NG; ++n) v = add2(v, join[k * T + n * GT + t]);
+          (s ? db[k] : dw[k]) = v;
         }
       }
     }
@@ -457,8 +566,9 @@ __global__ void __launch_bounds__(block_threads<GT>(), blocks_per_sm<GT, NCH, CH
   }
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const int col = CH * (t + GT * (e / CH)) + e % CH;
-    if (col < a.dim) pw[col] = dw[e], pb[col] = db[e];
+    const int col = W::column(t, e);
+    const float2 vw = unpack2(dw[e / 2]), vb = unpack2(db[e / 2]);
+    if (col < a.dim) pw[col] = e % 2 ? vw.y : vw.x, pb[col] = e % 2 ? vb.y : vb.x;
   }
 }
 
@@ -601,12 +711,12 @@ static int elements(int dim, int gt, bool vec) { return vec ? 4 * ((dim + 4 * gt
 // rows and leaves one partial sum; fewer where there are fewer rows than groups of threads.
 static int64_t bwd_blocks(int64_t rows, int dim, int64_t sum_groups, bool vec) {
   const int gt = group_threads(dim, vec), e = elements(dim, gt, vec);
-  const int per_sm = gt >= 512 ? 1 : e <= 8 ? 4 : e <= 12 ? 3 : 2;
+  const int per_sm = gt >= 512 ? 1 : e <= 4 ? 4 : e <= 12 ? 3 : 2;
   const int64_t need = std::max<int64_t>(1, (rows + block_groups(gt) - 1) / block_groups(gt));
   return std::max<int64_t>(1, std::min<int64_t>(need, per_sm * kNumSms / std::max<int64_t>(1, sum_groups)));
 }
 
-constexpr int kRingPerSm = 200 * 1024;  // shared memory of an SM that the rows on their way may take
+constexpr int kRingPerSm = 208 * 1024;  // shared memory of an SM that the rows on their way (and w) may take
 
 template <int GT, int NCH, int CH>
 static cudaError_t go(Args a, bool bwd, int64_t sum_groups, cudaStream_t st) {
@@ -615,13 +725,17 @@ static cudaError_t go(Args a, bool bwd, int64_t sum_groups, cudaStream_t st) {
   int smem = 0;
   if (CH == 4) {
     const int xb = size_of(a.x_type), yb = size_of(a.y_type);
-    a.stage_bytes = 4 * NCH * T * (bwd ? xb + yb + (a.add ? xb : 0) : xb);
-    a.depth = std::max(1, std::min(4, kRingPerSm / per_sm / a.stage_bytes));
+    const int w_bytes = bwd ? NCH * CH * T * 4 : 0;
+    const int two = 4 * NCH * T * (bwd ? xb + yb : xb), three = two + 4 * NCH * T * xb;
+    a.add_staged = bwd && a.add && three + w_bytes <= kRingPerSm / per_sm;
+    a.stage_bytes = a.add_staged ? three : two;
+    a.depth = std::max(1, std::min(4, (kRingPerSm / per_sm - w_bytes) / a.stage_bytes));
     smem = a.depth * a.stage_bytes;
   }
+  if (bwd) smem += NCH * CH * T * 4;  // w
   if (bwd && NG > 1) smem = std::max(smem, NCH * CH * T * 4);  // the groups' sums
   if (!bwd) {
-    const int64_t need = (a.rows + NG - 1) / NG;
+    const int64_t need = (static_cast<int64_t>(a.rows) + NG - 1) / NG;
     fwd_kernel<GT, NCH, CH><<<static_cast<unsigned>(std::min<int64_t>(need, per_sm * kNumSms)), T, smem, st>>>(a);
     return cudaGetLastError();
   }
@@ -663,7 +777,7 @@ static cudaError_t dispatch(const Args& a, bool bwd, int64_t sum_groups, bool ve
       fwd_wide_kernel<<<static_cast<unsigned>(a.rows), 1024, 0, st>>>(a);
       return cudaGetLastError();
     }
-    bwd_wide_kernel<<<static_cast<unsigned>(a.rows * sum_groups), 1024, 0, st>>>(a);
+    bwd_wide_kernel<<<static_cast<unsigned>(a.rows) * static_cast<unsigned>(sum_groups), 1024, 0, st>>>(a);
     cudaError_t e = cudaGetLastError();
     if (e == cudaSuccess && a.dw != nullptr) {
       sums_wide_kernel<<<dim3((a.dim + 31) / 32, static_cast<unsigned>(sum_groups)), 256, 0, st>>>(a);
@@ -743,7 +857,7 @@ int launch_layer_norm(const fb_layer_norm_args& p, bool bwd, cudaStream_t st, st
   const bool sums = bwd && (p.dweight || p.dbias);
   if (sums && (!p.dweight || !p.dbias)) return bad(FB_ERR_ARG, "dweight and dbias come together");
   const int64_t rows_all = (p.inner > 0 && p.outer > (1ll << 31) / p.inner) ? (1ll << 40) : p.outer * p.inner;
-  if (rows_all > 0x7FFFFFFFll) return bad(FB_ERR_UNSUPPORTED, "at most 2^31 - 1 rows per call");
+  if (rows_all > (1ll << 30)) return bad(FB_ERR_UNSUPPORTED, "at most 2^30 rows per call");
   const bool per_outer = sums && p.sum_per_outer;
   const int64_t groups = per_outer ? p.outer : 1;
   if (groups > 65535) return bad(FB_ERR_UNSUPPORTED, "at most 65535 gradients of their own per call");
@@ -765,6 +879,11 @@ int launch_layer_norm(const fb_layer_norm_args& p, bool bwd, cudaStream_t st, st
       (p.weight && norm::misaligned(p.weight, p.w_dtype)) || (p.bias && norm::misaligned(p.bias, p.w_dtype)) ||
       norm::misaligned(p.dweight, FB_F32) || norm::misaligned(p.dbias, FB_F32) || norm::misaligned(p.work, FB_F32))
     return bad(FB_ERR_ALIGN, "a pointer is not aligned to its elements");
+  std::string derr;
+  if (!current_device(derr)) {  // raises the kernels' shared-memory limits on this device
+    err = derr;
+    return FB_ERR_INIT;
+  }
   norm::Args a;
   memset(&a, 0, sizeof(a));
   a.x = p.x;
@@ -778,8 +897,8 @@ int launch_layer_norm(const fb_layer_norm_args& p, bool bwd, cudaStream_t st, st
   a.ao = p.add_outer_stride, a.ai = p.add_inner_stride;
   a.oo = p.out_outer_stride, a.oi = p.out_inner_stride;
   a.w_stride = p.w_outer_stride;
-  a.inner = p.inner;
-  a.rows = per_outer ? p.inner : rows_all;
+  a.inner = static_cast<int>(p.inner);
+  a.rows = static_cast<int>(per_outer ? p.inner : rows_all);
   a.dim = p.dim;
   a.x_type = p.x_dtype;
   a.y_type = p.y_dtype;

@@ -9,9 +9,9 @@
 // Angles: phi / 2 pi is formed in 64 bits (one multiply by omega / 2 pi, minus its nearest whole number), which
 // keeps positions of millions exact to ~1e-9 turns, and only the fraction in [-1/2, 1/2] goes to sincospif in 32 bits.
 //
-// Bound: HBM, every element read once and written once. A group of threads owns one token: each thread keeps the
-// sines and cosines of its own slots in registers and walks over the heads of q and of k, 16 bytes at a time, so no
-// table is read and an angle is computed once for all the heads that a thread takes.
+// Bound: HBM, every element read once and written once. A group of threads owns a token and up to twelve of its heads, of q and
+// of k alike: each thread keeps the sines and cosines of its own slots in registers for all of them, so no table is read
+// from memory.
 #include "fb_internal.h"
 
 namespace fb {
@@ -33,10 +33,10 @@ struct Args {
   int heads;        // of all tensors; head h of tensor 1 is number t[0].heads + h
   int seq;
   uint32_t tokens;  // batch * seq
-  uint32_t items;   // tokens * splits
-  int per_item;     // consecutive heads of one work item
+  uint32_t items;   // tokens * runs of heads
+  int per_item;     // consecutive heads of a work item
   int half;         // head_dim / 2
-  int tpr;          // threads per token
+  int tpr;          // threads per head row
   int inverse;
   const void* ids;
   int ids_type;     // fb_ids_type
@@ -54,106 +54,152 @@ __device__ __forceinline__ double load_id(const Args& a, int64_t at) {
   }
 }
 
-template <typename T>
-__device__ __forceinline__ float to_f32(T v);
-template <>
-__device__ __forceinline__ float to_f32<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
-template <>
-__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T>
-__device__ __forceinline__ T from_f32(float v);
-template <>
-__device__ __forceinline__ float from_f32<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
-// V consecutive elements: one 16-byte access where V elements are 16 bytes, else element by element.
+// V consecutive elements of type T. Wide: the 16 bytes of one vector access, worked on as 32-bit words (two 16-bit values
+// are widened and rounded as a pair); else element by element.
 template <typename T, int V>
-struct alignas(V * sizeof(T) == 16 ? 16 : sizeof(T)) Chunk {
-  T e[V];
+struct Chunk;
+template <>
+struct Chunk<float, 4> {
+  float4 v;
+  __device__ __forceinline__ void get(float (&f)[4]) const { f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w; }
+  __device__ __forceinline__ void set(const float (&f)[4]) { v = make_float4(f[0], f[1], f[2], f[3]); }
+};
+template <>
+struct Chunk<__nv_bfloat16, 8> {
+  uint4 v;
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+  }
+  __device__ __forceinline__ void set(const float (&f)[8]) {
+    v = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+  }
+};
+template <>
+struct Chunk<__half, 8> {
+  uint4 v;
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      f[2 * i] = p.x, f[2 * i + 1] = p.y;
+    }
+  }
+  __device__ __forceinline__ void set(const float (&f)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    v = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+template <typename T>
+struct Chunk<T, 1> {
+  T e;
+  __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = static_cast<float>(e); }
+  __device__ __forceinline__ void set(const float (&f)[1]) { e = static_cast<T>(f[0]); }
+};
+template <typename T>
+struct Chunk<T, 2> {
+  T e[2];
+  __device__ __forceinline__ void get(float (&f)[2]) const { f[0] = static_cast<float>(e[0]), f[1] = static_cast<float>(e[1]); }
+  __device__ __forceinline__ void set(const float (&f)[2]) { e[0] = static_cast<T>(f[0]), e[1] = static_cast<T>(f[1]); }
 };
 
-constexpr int kInFlight = 8;  // head rows a thread loads before it turns the first
+// Shared memory of a block of 256 threads for the rows on their way: 12 chunks of 16 bytes a thread, four blocks per SM.
+constexpr int kRows = 12;
 
-// A thread's share of one head row: one chunk of V elements (interleaved: V / 2 slots), or two chunks half a row
-// apart (halves: V slots).
+// A work item is one token and a run of heads: a group of `tpr` threads turns its rows, a thread's share of a row being
+// one chunk of V elements (interleaved: V / 2 slots), or two chunks half a row apart (halves: V slots). Wide rows are
+// all put on their way to shared memory first (each thread its own chunks, so nothing is waited for together) and the
+// angles are worked out while they come.
 template <typename T, int V, bool HALVES>
-__global__ void __launch_bounds__(kThreads) rope_axes_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kThreads, 4) rope_axes_kernel(const __grid_constant__ Args a) {
   constexpr int S = HALVES ? V : V / 2;  // slots of a thread
-  constexpr int U = HALVES ? kInFlight / 2 : kInFlight;
+  constexpr bool WIDE = V * sizeof(T) == 16;
+  using C = Chunk<T, V>;
+  extern __shared__ __align__(16) uint8_t staged[];
   // The slots' constants are read by different lanes at different places, which the constant cache serves one by one:
   // from shared memory they come at once.
   __shared__ double turns[kMaxSlots];
   __shared__ uint8_t axis[kMaxSlots];
+  const int groups = kThreads / a.tpr;
+  const int g = threadIdx.x / a.tpr;
+  const int r = threadIdx.x - g * a.tpr;
+  const uint32_t item = blockIdx.x * static_cast<uint32_t>(groups) + g;
+  const bool works = g < groups && item < a.items;
+  const uint32_t split = item / a.tokens;
+  const uint32_t token = item - split * a.tokens;
+  const uint32_t b = token / a.seq, l = token - b * a.seq;
+  const int n0 = a.t[0].heads;
+  const int h0 = static_cast<int>(split) * a.per_item;
+  const int rows = works ? min(a.heads - h0, a.per_item) : 0;
+  const T* x0 = static_cast<const T*>(a.t[0].x) + b * a.t[0].xb + l * a.t[0].xl + h0 * a.t[0].xh + r * V;
+  const T* x1 = static_cast<const T*>(a.t[1].x) + b * a.t[1].xb + l * a.t[1].xl + (h0 - n0) * a.t[1].xh + r * V;
+  C* mine = reinterpret_cast<C*>(staged) + threadIdx.x;
+  if constexpr (WIDE) {
+    for (int k = 0; k < rows; ++k) {
+      const T* at = h0 + k < n0 ? x0 + k * a.t[0].xh : x1 + k * a.t[1].xh;
+      const uint32_t dst = smem_u32(mine) + k * (HALVES ? 2 : 1) * kThreads * 16;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(at) : "memory");
+      if constexpr (HALVES)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + kThreads * 16), "l"(at + a.half) : "memory");
+    }
+  }
   for (int i = threadIdx.x; i < a.half; i += kThreads) {
     turns[i] = a.turns[i];
     axis[i] = a.axis[i];
   }
   __syncthreads();
-  const int groups = kThreads / a.tpr;
-  const int g = threadIdx.x / a.tpr;
-  const int r = threadIdx.x - g * a.tpr;
-  const uint32_t item = blockIdx.x * static_cast<uint32_t>(groups) + g;
-  if (g >= groups || item >= a.items) return;
-  const uint32_t split = item / a.tokens;
-  const uint32_t token = item - split * a.tokens;
-  const uint32_t b = token / a.seq, l = token - b * a.seq;
-
-  using C = Chunk<T, V>;
-  const T* x[2];
-  T* o[2];
-#pragma unroll
-  for (int n = 0; n < 2; ++n) {
-    // head h of tensor 1 counts from t[0].heads
-    const int64_t h0 = n ? -static_cast<int64_t>(a.t[0].heads) : 0;
-    x[n] = static_cast<const T*>(a.t[n].x) + b * a.t[n].xb + l * a.t[n].xl + h0 * a.t[n].xh + r * V;
-    o[n] = static_cast<T*>(a.t[n].out) + b * a.t[n].ob + l * a.t[n].ol + h0 * a.t[n].oh + r * V;
-  }
-  const int h_end = min(a.heads, static_cast<int>(split + 1) * a.per_item);
-  int h = static_cast<int>(split) * a.per_item;
-
+  if (!works) return;
   float c[S], s[S];
-  for (; h < h_end; h += U) {
-    C p[U], q[HALVES ? U : 1];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (h + u < h_end) {
-        const int n = h + u >= a.t[0].heads;
-        const T* at = (n ? x[1] : x[0]) + (h + u) * (n ? a.t[1].xh : a.t[0].xh);
-        p[u] = *reinterpret_cast<const C*>(at);
-        if constexpr (HALVES) q[u] = *reinterpret_cast<const C*>(at + a.half);
-      }
+  for (int j = 0; j < S; ++j) {
+    const int slot = r * S + j;
+    double t = load_id(a, b * a.ib + l * a.il + axis[slot] * a.ia) * turns[slot];
+    t -= rint(t);
+    sincospif(2.0f * static_cast<float>(t), &s[j], &c[j]);
+    if (a.inverse) s[j] = -s[j];
+  }
+  if constexpr (WIDE) asm volatile("cp.async.wait_all;" ::: "memory");
+  T* o0 = static_cast<T*>(a.t[0].out) + b * a.t[0].ob + l * a.t[0].ol + h0 * a.t[0].oh + r * V;
+  T* o1 = static_cast<T*>(a.t[1].out) + b * a.t[1].ob + l * a.t[1].ol + (h0 - n0) * a.t[1].oh + r * V;
+#pragma unroll 4
+  for (int k = 0; k < rows; ++k) {
+    const bool first = h0 + k < n0;
+    C p, q;
+    if constexpr (WIDE) {
+      p = mine[k * (HALVES ? 2 : 1) * kThreads];
+      if constexpr (HALVES) q = mine[(2 * k + 1) * kThreads];
+    } else {
+      const T* at = first ? x0 + k * a.t[0].xh : x1 + k * a.t[1].xh;
+      p = *reinterpret_cast<const C*>(at);
+      if constexpr (HALVES) q = *reinterpret_cast<const C*>(at + a.half);
     }
-    if (h == static_cast<int>(split) * a.per_item) {  // the first rows are on their way: the angles meanwhile
+    float f[V], e[V];
+    p.get(f);
+    if constexpr (HALVES) q.get(e);
 #pragma unroll
-      for (int i = 0; i < S; ++i) {
-        const int slot = r * S + i;
-        double t = load_id(a, b * a.ib + l * a.il + axis[slot] * a.ia) * turns[slot];
-        t -= rint(t);
-        sincospif(2.0f * static_cast<float>(t), &s[i], &c[i]);
-        if (a.inverse) s[i] = -s[i];
-      }
+    for (int j = 0; j < S; ++j) {
+      float& va = HALVES ? f[j] : f[2 * j];
+      float& vb = HALVES ? e[j] : f[2 * j + 1];
+      const float ta = va * c[j] - vb * s[j];
+      vb = va * s[j] + vb * c[j];
+      va = ta;
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (h + u < h_end) {
-#pragma unroll
-        for (int i = 0; i < S; ++i) {
-          T& ea = HALVES ? p[u].e[i] : p[u].e[2 * i];
-          T& eb = HALVES ? q[u].e[i] : p[u].e[2 * i + 1];
-          const float va = to_f32<T>(ea), vb = to_f32<T>(eb);
-          ea = from_f32<T>(va * c[i] - vb * s[i]);
-          eb = from_f32<T>(va * s[i] + vb * c[i]);
-        }
-        const int n = h + u >= a.t[0].heads;
-        T* at = (n ? o[1] : o[0]) + (h + u) * (n ? a.t[1].oh : a.t[0].oh);
-        *reinterpret_cast<C*>(at) = p[u];
-        if constexpr (HALVES) *reinterpret_cast<C*>(at + a.half) = q[u];
-      }
+    T* at = first ? o0 + k * a.t[0].oh : o1 + k * a.t[1].oh;
+    p.set(f);
+    *reinterpret_cast<C*>(at) = p;
+    if constexpr (HALVES) {
+      q.set(e);
+      *reinterpret_cast<C*>(at + a.half) = q;
     }
   }
 }
@@ -162,15 +208,17 @@ template <typename T, int V, bool HALVES>
 static cudaError_t go(Args& a, cudaStream_t st) {
   a.tpr = HALVES ? a.half / V : 2 * a.half / V;
   const int groups = kThreads / a.tpr;
-  // Cut the heads of q and k into enough runs to fill the GPU (about eight blocks per SM), of whole batches of loads
-  // where tokens are many; a single token spreads over as many groups as there are heads.
-  constexpr int U = HALVES ? kInFlight / 2 : kInFlight;
-  const int64_t want = (static_cast<int64_t>(kNumSms) * 8 * groups + a.tokens - 1) / a.tokens;
-  a.per_item = static_cast<int>(std::max<int64_t>(1, a.heads / want));
-  if (a.per_item > U) a.per_item = (a.per_item + U - 1) / U * U;
+  // Runs of up to kRows chunks, shorter where that would leave some of the four blocks per SM without work: a single
+  // token's heads all go to different groups.
+  constexpr int most = HALVES ? kRows / 2 : kRows;
+  const int64_t room = 4ll * kNumSms * groups;
+  const int64_t fair = (static_cast<int64_t>(a.tokens) * a.heads + room - 1) / room;
+  const int64_t runs = (a.heads + most - 1) / most;
+  a.per_item = static_cast<int>(std::min<int64_t>(fair, (a.heads + runs - 1) / runs));
   a.items = a.tokens * static_cast<uint32_t>((a.heads + a.per_item - 1) / a.per_item);
   const unsigned grid = (a.items + groups - 1) / groups;
-  rope_axes_kernel<T, V, HALVES><<<grid, kThreads, 0, st>>>(a);
+  const int smem = V * sizeof(T) == 16 ? a.per_item * (HALVES ? 2 : 1) * kThreads * 16 : 0;
+  rope_axes_kernel<T, V, HALVES><<<grid, kThreads, smem, st>>>(a);
   return cudaGetLastError();
 }
 
@@ -212,6 +260,22 @@ static void fill_slots(int axes, const int32_t* dims, const double* theta, Args&
 
 }  // namespace rope
 
+std::string rope_axes_setup() {
+  using namespace rope;
+  const int bytes = kRows * kThreads * 16;
+  cudaError_t e = cudaSuccess;
+  auto raise = [&](auto kernel) {
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  };
+  raise(rope_axes_kernel<float, 4, false>);
+  raise(rope_axes_kernel<float, 4, true>);
+  raise(rope_axes_kernel<__half, 8, false>);
+  raise(rope_axes_kernel<__half, 8, true>);
+  raise(rope_axes_kernel<__nv_bfloat16, 8, false>);
+  raise(rope_axes_kernel<__nv_bfloat16, 8, true>);
+  return e == cudaSuccess ? std::string() : std::string("cudaFuncSetAttribute(rope_axes): ") + cudaGetErrorString(e);
+}
+
 int launch_rope_axes(const fb_rope_args& p, cudaStream_t st, std::string& err) {
   const int count = p.count, dtype = p.dtype, head_dim = p.head_dim, axes = p.axes, pairs = p.pairs;
   const fb_rope_tensor* ts = p.tensor;
@@ -244,6 +308,11 @@ int launch_rope_axes(const fb_rope_args& p, cudaStream_t st, std::string& err) {
       err = "fb_rope_axes: 1 to 65536 heads";
       return FB_ERR_ARG;
     }
+  }
+  std::string derr;
+  if (!current_device(derr)) {  // raises the kernels' shared-memory limits on this device
+    err = derr;
+    return FB_ERR_INIT;
   }
   const int64_t tokens = static_cast<int64_t>(p.batch) * p.seq;
   if (tokens == 0) return FB_OK;

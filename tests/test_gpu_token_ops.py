@@ -158,6 +158,20 @@ def test_rope_strides(pairs, dt):
     check_rope(ops().rope_axes(same, ids, axes, pairs=pairs), same, ids, axes, pairs=pairs)
 
 
+@pytest.mark.parametrize("pairs", ["interleaved", "halves"])
+@pytest.mark.parametrize("dt,h,kv,axes,l", [(BF16, 24, 24, (16, 56, 56), 4608), (F32, 16, 4, (16, 24, 24), 3001), (F16, 40, 1, (22, 20, 22), 5000),
+                                            (BF16, 7, 3, (10, 30, 40), 9001), (F16, 3, 2, (2, 4), 40001)])
+def test_rope_many_tokens(pairs, dt, h, kv, axes, l):
+    """Enough tokens that a thread takes a run of heads, across the border of q and k, with a run left over."""
+    g = gen(7)
+    hd = sum(axes)
+    q, k = randn(g, 2, h, l, hd, dtype=dt), randn(g, 2, l, kv, hd, dtype=dt).transpose(1, 2)
+    ids = grid_ids(g, l, len(axes), F32, 300)
+    qo, ko = ops().rope_axes_qk(q, k, ids, axes, pairs=pairs, inverse=True)
+    check_rope(qo, q, ids, axes, pairs=pairs, inverse=True)
+    check_rope(ko, k, ids, axes, pairs=pairs, inverse=True)
+
+
 def test_rope_gradient_by_differences():
     """sum(g * rope(x)) along random directions: central differences in fp32 (the map is linear, so a step of one is
     exact up to rounding) against the inverse turn of g."""

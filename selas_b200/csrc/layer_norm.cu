@@ -83,12 +83,9 @@ struct Step {
 };
 __device__ __forceinline__ void advance(Place& p, const Step& s, int inner) {
   p.row += s.rows;
-  p.o += s.o;
   p.i += s.i;
-  if (p.i >= inner) {
-    p.i -= inner;
-    ++p.o;
-  }
+  p.o += s.o + (p.i >= inner);
+  if (p.i >= inner) p.i -= inner;
 }
 
 // CH consecutive elements (4: one vector access, 1: any alignment) widened to fp32.
@@ -170,14 +167,14 @@ __device__ __forceinline__ void widen4(const uint8_t* p, int type, float* f) {
 }
 
 // The elements of a row that one thread of its group holds: NCH chunks of CH, chunk c at column CH * (t + GT * c);
-// zeros past the end. The type branch is outside the loop, so the loads of a row go out together.
-template <int GT, int NCH, int CH>
+// zeros past the end (FULL: the row ends with the last thread's last chunk). The type branch is outside the loop, so the loads of a row go out together.
+template <int GT, int NCH, int CH, bool FULL>
 __device__ __forceinline__ void load_row(const void* p, int type, int64_t base, int t, int dim, float (&f)[NCH * CH]) {
   auto each = [&](int ty) {
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
       const int col = CH * (t + GT * c);
-      if (col < dim) {
+      if (FULL || col < dim) {
         load_chunk<CH>(p, ty, base + col, f + CH * c);
       } else {
 #pragma unroll
@@ -194,13 +191,13 @@ __device__ __forceinline__ void load_row(const void* p, int type, int64_t base, 
   }
 }
 
-template <int GT, int NCH, int CH>
+template <int GT, int NCH, int CH, bool FULL>
 __device__ __forceinline__ void store_row(void* p, int type, int64_t base, int t, int dim, const float (&f)[NCH * CH]) {
   auto each = [&](int ty) {
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
       const int col = CH * (t + GT * c);
-      if (col < dim) store_chunk<CH>(p, ty, base + col, f + CH * c);
+      if (FULL || col < dim) store_chunk<CH>(p, ty, base + col, f + CH * c);
     }
   };
   if (type == FB_F32) {
@@ -214,32 +211,32 @@ __device__ __forceinline__ void store_row(void* p, int type, int64_t base, int t
 
 // Asynchronous copy of a thread's own chunks of a row to its own places in shared memory, chunk c at
 // dst + c * T * bytes(chunk): no other thread reads them, so waiting for the copies needs no barrier.
-template <int GT, int NCH, int T>
+template <int GT, int NCH, int T, bool FULL>
 __device__ __forceinline__ void fetch_row(uint32_t dst, const void* p, int type, int64_t base, int t, int dim) {
   if (type == FB_F32) {
     const float* s = static_cast<const float*>(p) + base;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
       const int col = 4 * (t + GT * c);
-      if (col < dim) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + c * T * 16), "l"(s + col) : "memory");
+      if (FULL || col < dim) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + c * T * 16), "l"(s + col) : "memory");
     }
   } else {
     const uint16_t* s = static_cast<const uint16_t*>(p) + base;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
       const int col = 4 * (t + GT * c);
-      if (col < dim) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst + c * T * 8), "l"(s + col) : "memory");
+      if (FULL || col < dim) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst + c * T * 8), "l"(s + col) : "memory");
     }
   }
 }
 
 // The fetched row, widened.
-template <int GT, int NCH, int T>
+template <int GT, int NCH, int T, bool FULL>
 __device__ __forceinline__ void take_row(const uint8_t* src, int type, int t, int dim, float (&f)[NCH * 4]) {
   auto each = [&](int ty, int bytes) {
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-      if (4 * (t + GT * c) < dim) {
+      if (FULL || 4 * (t + GT * c) < dim) {
         widen4(src + c * T * bytes, ty, f + 4 * c);
       } else {
         f[4 * c] = f[4 * c + 1] = f[4 * c + 2] = f[4 * c + 3] = 0.f;
@@ -273,17 +270,17 @@ __device__ __forceinline__ void wait_fetch(int newer) {
 // in shared memory and a barrier of the group's own; `buf` alternates between calls, so one barrier per sum is enough.
 template <int GT>
 __device__ __forceinline__ float2 group_sum2(float a, float b, int group, float2* slots, int& buf) {
+  // the lower half of the warp adds up a, the upper half b
+  const bool upper = threadIdx.x & 16;
+  float v = (upper ? b : a) + __shfl_xor_sync(0xffffffffu, upper ? a : b, 16);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    a += __shfl_xor_sync(0xffffffffu, a, o);
-    b += __shfl_xor_sync(0xffffffffu, b, o);
-  }
-  if constexpr (GT == 32) return make_float2(a, b);
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if constexpr (GT == 32) return make_float2(__shfl_sync(0xffffffffu, v, 0), __shfl_sync(0xffffffffu, v, 16));
   constexpr int W = GT / 32;
   float2* s = slots + (buf * (blockDim.x / GT) + group) * W;
   buf ^= 1;
   const int warp = (threadIdx.x % GT) >> 5;
-  if ((threadIdx.x & 31) == 0) s[warp] = make_float2(a, b);
+  if ((threadIdx.x & 15) == 0) (upper ? s[warp].y : s[warp].x) = v;
   asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(GT) : "memory");
   float2 r = s[0];
 #pragma unroll
@@ -291,28 +288,26 @@ __device__ __forceinline__ float2 group_sum2(float a, float b, int group, float2
   return r;
 }
 
-template <int GT>
-constexpr int block_threads() {
-  return GT < 256 ? 256 : GT;
-}
-
-// Blocks per SM that a kernel is compiled (registers) and its grid and shared memory are sized for.
-template <int GT, int NCH, int CH, bool BWD>
-constexpr int blocks_per_sm() {
-  return GT >= 512 ? (GT == 512 && !BWD ? 2 : 1) : NCH * CH <= 4 ? 4 : NCH * CH <= 12 ? 3 : 2;
-}
+// Threads of a block, and blocks per SM that a kernel is compiled for (registers) and its grid and shared memory are
+// sized for. Forward: blocks of 256 threads, as many as their registers allow. Backward: one block per SM, so that the
+// groups' column sums are joined in shared memory and one partial row per SM goes to memory.
+constexpr int fwd_threads(int gt) { return gt < 256 ? 256 : gt; }
+constexpr int fwd_blocks(int gt, int e) { return gt >= 512 ? (gt == 512 ? 2 : 1) : e <= 4 ? 4 : e <= 12 ? 3 : 2; }
+constexpr int bwd_threads(int gt, int e) { return gt >= 512 ? gt : e <= 4 ? 1024 : e <= 12 ? 768 : 512; }
 
 // One row of up to GT * NCH * CH elements per group of GT threads at a time; a group walks over rows
 // blockIdx.x * NG + group, + gridDim.x * NG, ... of sum group blockIdx.y, the next `depth` rows on their way to shared
 // memory while it works on one (CH == 4; the rows of odd sizes and alignments, CH == 1, are loaded where they are used).
-template <int GT, int NCH, int CH>
+template <int GT, int NCH, int CH, bool FULL, int THREADS>
 struct Walk {
-  static constexpr int T = block_threads<GT>(), NG = T / GT, E = NCH * CH, P = E / 2;
+  static constexpr int T = THREADS, NG = T / GT, E = NCH * CH, P = E / 2;
   // Pair k of a thread's elements lies in the chunks of columns 2k .. 2k + 1; both are inside the row or both past its
   // end for chunks of four, each by itself for single elements.
   static __device__ __forceinline__ int column(int t, int e) { return CH * (t + GT * (e / CH)) + e % CH; }
   static __device__ __forceinline__ f2 inside(int t, int k, int dim, float v) {
-    if constexpr (CH == 4) {
+    if constexpr (FULL) {
+      return pack2(v, v);
+    } else if constexpr (CH == 4) {
       const float m = column(t, 2 * k) < dim ? v : 0.f;
       return pack2(m, m);
     } else {
@@ -325,13 +320,13 @@ struct Walk {
   }
   static __device__ __forceinline__ void load(const void* p, int type, int64_t base, int t, int dim, f2 (&v)[P]) {
     float f[E];
-    load_row<GT, NCH, CH>(p, type, base, t, dim, f);
+    load_row<GT, NCH, CH, FULL>(p, type, base, t, dim, f);
     pairs(f, v);
   }
   static __device__ __forceinline__ void take(const uint8_t* src, int type, int t, int dim, f2 (&v)[P]) {
     if constexpr (CH == 4) {
       float f[E];
-      take_row<GT, NCH, T>(src, type, t, dim, f);
+      take_row<GT, NCH, T, FULL>(src, type, t, dim, f);
       pairs(f, v);
     }
   }
@@ -342,7 +337,7 @@ struct Walk {
       const float2 r = unpack2(v[k]);
       f[2 * k] = r.x, f[2 * k + 1] = r.y;
     }
-    store_row<GT, NCH, CH>(p, type, base, t, dim, f);
+    store_row<GT, NCH, CH, FULL>(p, type, base, t, dim, f);
   }
   // A thread's own pairs in shared memory, two to a 16-byte place.
   static __device__ __forceinline__ void keep(ulonglong2* at, const f2 (&v)[P]) {
@@ -363,10 +358,9 @@ struct Walk {
   }
 };
 
-template <int GT, int NCH, int CH>
-__global__ void __launch_bounds__(block_threads<GT>(), blocks_per_sm<GT, NCH, CH, false>())
-    fwd_kernel(const __grid_constant__ Args a) {
-  using W = Walk<GT, NCH, CH>;
+template <int GT, int NCH, int CH, bool FULL>
+__global__ void __launch_bounds__(fwd_threads(GT), fwd_blocks(GT, NCH* CH)) fwd_kernel(const __grid_constant__ Args a) {
+  using W = Walk<GT, NCH, CH, FULL, fwd_threads(GT)>;
   constexpr int P = W::P, T = W::T, NG = W::NG;
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ float2 slots[2 * NG * (GT / 32)];
@@ -377,7 +371,7 @@ __global__ void __launch_bounds__(block_threads<GT>(), blocks_per_sm<GT, NCH, CH
   Place at = place_of(a, 0, blockIdx.x * NG + group), ahead = at;
   auto fetch = [&](int stage) {
     if (ahead.row < a.rows) {
-      fetch_row<GT, NCH, T>(smem_u32(mine) + stage * a.stage_bytes, a.x, a.x_type, ahead.o * a.xo + ahead.i * a.xi, t, a.dim);
+      fetch_row<GT, NCH, T, FULL>(smem_u32(mine) + stage * a.stage_bytes, a.x, a.x_type, ahead.o * a.xo + ahead.i * a.xi, t, a.dim);
     }
     commit_fetch();
     advance(ahead, step, a.inner);
@@ -421,7 +415,7 @@ __global__ void __launch_bounds__(block_threads<GT>(), blocks_per_sm<GT, NCH, CH
       x[k] = add2(x[k], W::inside(t, k, a.dim, -mean));
       q = fma2(x[k], x[k], q);
     }
-    const float rstd = 1.0f / sqrtf(group_sum2<GT>(total(q), 0.f, group, slots, buf).x * inv + a.eps);
+    const float rstd = rsqrtf(group_sum2<GT>(total(q), 0.f, group, slots, buf).x * inv + a.eps);
     const f2 r = pack2(rstd, rstd);
 #pragma unroll
     for (int k = 0; k < P; ++k) x[k] = fma2(mul2(x[k], r), w[k], b[k]);
@@ -429,10 +423,9 @@ __global__ void __launch_bounds__(block_threads<GT>(), blocks_per_sm<GT, NCH, CH
   }
 }
 
-template <int GT, int NCH, int CH>
-__global__ void __launch_bounds__(block_threads<GT>(), blocks_per_sm<GT, NCH, CH, true>())
-    bwd_kernel(const __grid_constant__ Args a) {
-  using W = Walk<GT, NCH, CH>;
+template <int GT, int NCH, int CH, bool FULL>
+__global__ void __launch_bounds__(bwd_threads(GT, NCH* CH), 1) bwd_kernel(const __grid_constant__ Args a) {
+  using W = Walk<GT, NCH, CH, FULL, bwd_threads(GT, NCH * CH)>;
   constexpr int E = W::E, P = W::P, T = W::T, NG = W::NG;
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ float2 slots[2 * NG * (GT / 32)];
@@ -448,10 +441,10 @@ __global__ void __launch_bounds__(block_threads<GT>(), blocks_per_sm<GT, NCH, CH
   auto fetch = [&](int stage) {
     if (ahead.row < a.rows) {
       const int off = stage * a.stage_bytes;
-      fetch_row<GT, NCH, T>(smem_u32(mx) + off, a.x, a.x_type, ahead.o * a.xo + ahead.i * a.xi, t, a.dim);
-      fetch_row<GT, NCH, T>(smem_u32(my) + off, a.dy, a.y_type, ahead.o * a.yo + ahead.i * a.yi, t, a.dim);
+      fetch_row<GT, NCH, T, FULL>(smem_u32(mx) + off, a.x, a.x_type, ahead.o * a.xo + ahead.i * a.xi, t, a.dim);
+      fetch_row<GT, NCH, T, FULL>(smem_u32(my) + off, a.dy, a.y_type, ahead.o * a.yo + ahead.i * a.yi, t, a.dim);
       if (a.add_staged)
-        fetch_row<GT, NCH, T>(smem_u32(ma) + off, a.add, a.x_type, ahead.o * a.ao + ahead.i * a.ai, t, a.dim);
+        fetch_row<GT, NCH, T, FULL>(smem_u32(ma) + off, a.add, a.x_type, ahead.o * a.ao + ahead.i * a.ai, t, a.dim);
     }
     commit_fetch();
     advance(ahead, step, a.inner);
@@ -504,7 +497,7 @@ __global__ void __launch_bounds__(block_threads<GT>(), blocks_per_sm<GT, NCH, CH
       }
     }
     const float2 v = group_sum2<GT>(total(qx), total(qg), group, slots, buf);
-    const float rstd = 1.0f / sqrtf(v.x * inv + a.eps);
+    const float rstd = rsqrtf(v.x * inv + a.eps);
     // dx = rstd (g w - mean(g w) - xhat mean(g w xhat)), xhat = x rstd
     const float c0 = -rstd * m.y * inv, c1 = -rstd * (v.y * inv * rstd);
     const f2 r = pack2(rstd, rstd), k0 = pack2(c0, c0), k1 = pack2(c1, c1);
@@ -568,14 +561,15 @@ __global__ void __launch_bounds__(block_threads<GT>(), blocks_per_sm<GT, NCH, CH
   for (int e = 0; e < E; ++e) {
     const int col = W::column(t, e);
     const float2 vw = unpack2(dw[e / 2]), vb = unpack2(db[e / 2]);
-    if (col < a.dim) pw[col] = e % 2 ? vw.y : vw.x, pb[col] = e % 2 ? vb.y : vb.x;
+    if (FULL || col < a.dim) pw[col] = e % 2 ? vw.y : vw.x, pb[col] = e % 2 ? vb.y : vb.x;
   }
 }
 
 // dw, db [sum group][dim] = the partials' sums. 32 columns x 8 runs of the partials per block, joined in order.
-__global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ part, int blocks, int dim,
+__global__ void __launch_bounds__(256) join_kernel(const float* part, int blocks, int dim,
                                                    float* __restrict__ dw, float* __restrict__ db) {
   __shared__ float s[8][32];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 31, run = threadIdx.x >> 5;
   const int64_t n2 = 2ll * dim;
   const int64_t col = static_cast<int64_t>(blockIdx.x) * 32 + lane;  // over dw, then db
@@ -704,58 +698,64 @@ static int group_threads(int dim, bool vec) {
   while (gt * (vec ? 20 : 16) < dim && gt < 1024) gt *= 2;
   return gt;
 }
-static int block_groups(int gt) { return std::max(1, 256 / gt); }
 static int elements(int dim, int gt, bool vec) { return vec ? 4 * ((dim + 4 * gt - 1) / (4 * gt)) : 16; }
 
-// Blocks per sum group of the backward pass: as many as are resident at once, so that each walks over its share of the
-// rows and leaves one partial sum; fewer where there are fewer rows than groups of threads.
+// Blocks per sum group of the backward pass: the SMs shared out over the groups, fewer where there are fewer rows than
+// groups of threads.
 static int64_t bwd_blocks(int64_t rows, int dim, int64_t sum_groups, bool vec) {
-  const int gt = group_threads(dim, vec), e = elements(dim, gt, vec);
-  const int per_sm = gt >= 512 ? 1 : e <= 4 ? 4 : e <= 12 ? 3 : 2;
-  const int64_t need = std::max<int64_t>(1, (rows + block_groups(gt) - 1) / block_groups(gt));
-  return std::max<int64_t>(1, std::min<int64_t>(need, per_sm * kNumSms / std::max<int64_t>(1, sum_groups)));
+  const int gt = group_threads(dim, vec), ng = bwd_threads(gt, elements(dim, gt, vec)) / gt;
+  const int64_t need = std::max<int64_t>(1, (rows + ng - 1) / ng);
+  return std::max<int64_t>(1, std::min<int64_t>(need, kNumSms / std::max<int64_t>(1, sum_groups)));
 }
 
 constexpr int kRingPerSm = 208 * 1024;  // shared memory of an SM that the rows on their way (and w) may take
 
-template <int GT, int NCH, int CH>
+template <int GT, int NCH, int CH, bool FULL>
 static cudaError_t go(Args a, bool bwd, int64_t sum_groups, cudaStream_t st) {
-  constexpr int T = block_threads<GT>(), NG = T / GT;
-  const int per_sm = bwd ? blocks_per_sm<GT, NCH, CH, true>() : blocks_per_sm<GT, NCH, CH, false>();
+  constexpr int TF = fwd_threads(GT), TB = bwd_threads(GT, NCH * CH), E = NCH * CH;
+  const int T = bwd ? TB : TF, per_sm = bwd ? 1 : fwd_blocks(GT, E);
+  const int w_bytes = bwd ? E * T * 4 : 0;
   int smem = 0;
   if (CH == 4) {
     const int xb = size_of(a.x_type), yb = size_of(a.y_type);
-    const int w_bytes = bwd ? NCH * CH * T * 4 : 0;
     const int two = 4 * NCH * T * (bwd ? xb + yb : xb), three = two + 4 * NCH * T * xb;
     a.add_staged = bwd && a.add && three + w_bytes <= kRingPerSm / per_sm;
     a.stage_bytes = a.add_staged ? three : two;
     a.depth = std::max(1, std::min(4, (kRingPerSm / per_sm - w_bytes) / a.stage_bytes));
     smem = a.depth * a.stage_bytes;
   }
-  if (bwd) smem += NCH * CH * T * 4;  // w
-  if (bwd && NG > 1) smem = std::max(smem, NCH * CH * T * 4);  // the groups' sums
+  smem += w_bytes;  // after the walk, the groups' sums take this much too
   if (!bwd) {
+    constexpr int NG = TF / GT;
     const int64_t need = (static_cast<int64_t>(a.rows) + NG - 1) / NG;
-    fwd_kernel<GT, NCH, CH><<<static_cast<unsigned>(std::min<int64_t>(need, per_sm * kNumSms)), T, smem, st>>>(a);
+    fwd_kernel<GT, NCH, CH, FULL><<<static_cast<unsigned>(std::min<int64_t>(need, per_sm * kNumSms)), TF, smem, st>>>(a);
     return cudaGetLastError();
   }
   const int64_t blocks = bwd_blocks(a.rows, a.dim, sum_groups, CH == 4);
   const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(sum_groups));
-  bwd_kernel<GT, NCH, CH><<<grid, T, smem, st>>>(a);
+  bwd_kernel<GT, NCH, CH, FULL><<<grid, TB, smem, st>>>(a);
   cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess && a.dw != nullptr && blocks > 1) {
-    const dim3 jg(static_cast<unsigned>((2ll * a.dim + 31) / 32), static_cast<unsigned>(sum_groups));
-    join_kernel<<<jg, 256, 0, st>>>(a.part, static_cast<int>(blocks), a.dim, a.dw, a.db);
-    e = cudaGetLastError();
+    // launched while the last blocks of the walk still run; it waits for them before it reads
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>((2ll * a.dim + 31) / 32), static_cast<unsigned>(sum_groups));
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, join_kernel, static_cast<const float*>(a.part), static_cast<int>(blocks), a.dim, a.dw, a.db);
   }
   return e;
 }
 
 // Raises the shared-memory limits of one instance (ring of up to kRingPerSm bytes).
-template <int GT, int NCH, int CH>
+template <int GT, int NCH, int CH, bool FULL>
 static cudaError_t setup_one() {
-  const cudaError_t e = cudaFuncSetAttribute(fwd_kernel<GT, NCH, CH>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingPerSm);
-  return e != cudaSuccess ? e : cudaFuncSetAttribute(bwd_kernel<GT, NCH, CH>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingPerSm);
+  const cudaError_t e = cudaFuncSetAttribute(fwd_kernel<GT, NCH, CH, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingPerSm);
+  return e != cudaSuccess ? e : cudaFuncSetAttribute(bwd_kernel<GT, NCH, CH, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingPerSm);
 }
 
 template <int GT, typename F>
@@ -788,7 +788,9 @@ static cudaError_t dispatch(const Args& a, bool bwd, int64_t sum_groups, bool ve
   auto run = [&](auto gt) {
     constexpr int GT = decltype(gt)::value;
     return with_chunks<GT>(a.dim, vec, [&](auto nch, auto ch) {
-      return go<GT, decltype(nch)::value, decltype(ch)::value>(a, bwd, sum_groups, st);
+      constexpr int NCH = decltype(nch)::value, CH = decltype(ch)::value;
+      if (CH == 4 && a.dim == 4 * GT * NCH) return go<GT, NCH, CH, CH == 4>(a, bwd, sum_groups, st);
+      return go<GT, NCH, CH, false>(a, bwd, sum_groups, st);
     });
   };
   switch (group_threads(a.dim, vec)) {
@@ -801,14 +803,19 @@ static cudaError_t dispatch(const Args& a, bool bwd, int64_t sum_groups, bool ve
   }
 }
 
+template <int GT, int NCH>
+static cudaError_t setup_both() {
+  const cudaError_t e = setup_one<GT, NCH, 4, false>();
+  return e != cudaSuccess ? e : setup_one<GT, NCH, 4, true>();
+}
 template <int GT>
 static cudaError_t setup_gt() {
-  cudaError_t e = setup_one<GT, 16, 1>();
-  if (e == cudaSuccess) e = setup_one<GT, 1, 4>();
-  if (e == cudaSuccess) e = setup_one<GT, 2, 4>();
-  if (e == cudaSuccess) e = setup_one<GT, 3, 4>();
-  if (e == cudaSuccess) e = setup_one<GT, 4, 4>();
-  if constexpr (GT < 1024) e = e == cudaSuccess ? setup_one<GT, 5, 4>() : e;
+  cudaError_t e = setup_one<GT, 16, 1, false>();
+  if (e == cudaSuccess) e = setup_both<GT, 1>();
+  if (e == cudaSuccess) e = setup_both<GT, 2>();
+  if (e == cudaSuccess) e = setup_both<GT, 3>();
+  if (e == cudaSuccess) e = setup_both<GT, 4>();
+  if constexpr (GT < 1024) e = e == cudaSuccess ? setup_both<GT, 5>() : e;
   return e;
 }
 

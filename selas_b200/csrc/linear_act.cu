@@ -16,9 +16,9 @@
 //  * many_kernel, for the rest: 256 tokens x 256 features per CTA pair (tcgen05.mma.cta_group::2), persistent over tiles.
 //
 // Precision: the tensor core adds into its accumulator with less care than an fp32 add (over K = 12288 the error grew to
-// 1.3e-5 of the result's norm), so an accumulator takes 512 of K at most; the epilogue warps then add it to fp32
-// registers, which are the sum proper, while the other TMEM buffer takes the next 512. That costs no time, and holds
-// the error of an fp32 output below 1e-6.
+// 1.3e-5 of the result's norm), so an accumulator takes 1024 of K at most; the epilogue warps then add it to fp32
+// registers, which are the sum proper, while the other TMEM buffer takes the next 1024. That costs 2 % of the time at
+// most (every 512 cost 10 %) and holds the error of an fp32 output near 1e-6.
 #include <type_traits>
 
 #include "gemm_common.cuh"
@@ -45,13 +45,30 @@ struct Args {
 
 // The kernels are instances per activation: with all of them behind a switch in every unrolled place, the code of an
 // epilogue outgrew the instruction caches (a 256 x 256 tile took 80 us).
+//
+// The erf of GELU is Abramowitz and Stegun's 7.1.26 for erfc(|x|), x = z / sqrt 2, off by at most 1.5e-7: y = z h for
+// z < 0 and z - z h otherwise, h = erfc(|x|) / 2, which keeps the small values of the negative side. With CUDA's erff the
+// epilogue of a 256 x 256 tile at K = 3072 took longer than its products. The sigmoids divide by 1 + exp with the
+// hardware's exp2 and division (2 ulp); tanh(u) = 2 sigmoid(2u) - 1.
 template <int ACT>
 __device__ __forceinline__ float activate(float z) {
   if constexpr (ACT == FB_ACT_RELU) return z < 0.f ? 0.f : z;  // keeps a NaN
-  if constexpr (ACT == FB_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-  if constexpr (ACT == FB_ACT_GELU_TANH) return gelu_tanh_f32(z);
-  if constexpr (ACT == FB_ACT_QUICK_GELU) return z / (1.0f + expf(-1.702f * z));
-  if constexpr (ACT == FB_ACT_SILU) return z / (1.0f + expf(-z));
+  if constexpr (ACT == FB_ACT_GELU) {
+    const float x = fabsf(z) * 0.70710678118654752f;
+    const float t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
+    float h = fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
+    h = fmaf(h, t, 0.5f * 1.421413741f);
+    h = fmaf(h, t, 0.5f * -0.284496736f);
+    h = fmaf(h, t, 0.5f * 0.254829592f);
+    const float zh = z * (h * t * __expf(-x * x));
+    return z < 0.f ? zh : z - zh;
+  }
+  if constexpr (ACT == FB_ACT_GELU_TANH) {
+    const float u = 0.7978845608028654f * fmaf(0.044715f * z * z, z, z);  // sqrt(2 / pi) (z + 0.044715 z^3)
+    return __fdividef(z, 1.0f + __expf(-2.0f * u));
+  }
+  if constexpr (ACT == FB_ACT_QUICK_GELU) return __fdividef(z, 1.0f + __expf(-1.702f * z));
+  if constexpr (ACT == FB_ACT_SILU) return __fdividef(z, 1.0f + __expf(-z));
   return z;
 }
 
@@ -142,7 +159,7 @@ __device__ __forceinline__ void promote(uint32_t taddr, bool first, float (&v)[N
 // ---------------------------------------------------------------------------------------------- few rows
 
 constexpr int kFeat = 128;       // output features of a tile
-constexpr int kChunkBlocks = 8;  // K blocks of 64 that one accumulator takes
+constexpr int kChunkBlocks = 16;  // K blocks of 64 that one accumulator takes
 
 // warp 0 loads, warp 1 issues the MMAs, the others promote the accumulator (TMEM lane = feature, column = token; at 128
 // tokens two warps share a lane quarter, so that a thread holds at most 64 sums); all of them write the outputs.
@@ -184,6 +201,11 @@ __global__ void __launch_bounds__(Few<BT>::kThreads, 2) few_kernel(const __grid_
   const int kb0 = static_cast<int>(static_cast<int64_t>(a.num_kb) * rank / a.splits);
   const int kb1 = static_cast<int>(static_cast<int64_t>(a.num_kb) * (rank + 1) / a.splits);
 
+  auto load = [&](int stage, int kb) {
+    mbar_arrive_expect_tx(&full[stage], C::kStageBytes);
+    tma_load_2d(&a.tma_w, &full[stage], sW + stage * C::kWBytes, kb * BK, f0);
+    tma_load_2d(&a.tma_x, &full[stage], sX + stage * C::kXBytes, kb * BK, t0);
+  };
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(&full[s], 1);
@@ -196,14 +218,34 @@ __global__ void __launch_bounds__(Few<BT>::kThreads, 2) few_kernel(const __grid_
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbar_init();
-  }
-  if (warp == 0 && lane == 0) {
-    tma_prefetch_desc(&a.tma_w);
-    tma_prefetch_desc(&a.tma_x);
+    // this thread's barriers are ready: the first loads do not wait for the rest of the set-up
+    for (int s = 0; s < C::kStages && kb0 + s < kb1; ++s) load(s, kb0 + s);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, C::kTmemCols);
     tmem_relinquish();
+  }
+  // This CTA's share of the tile's tokens. Its bias and residuals are fetched now, not when the sums are there.
+  const int live = min(BT, a.m - t0);
+  const int j0 = live * rank / a.splits, j1 = live * (rank + 1) / a.splits;
+  const bool whole = a.vec && f0 + kFeat <= a.n;  // every lane's four consecutive features are aligned vectors
+  if (a.residual != nullptr) {
+    const int line = a.res_f32 ? 32 : 64, lines = kFeat / line;  // features in 128 bytes
+    for (int i = threadIdx.x; i < (j1 - j0) * lines; i += C::kThreads) {
+      const int n = f0 + (i % lines) * line;
+      const int64_t at = static_cast<int64_t>(t0 + j0 + i / lines) * a.ld_res + n;
+      if (n < a.n)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint8_t*>(a.residual) + (a.res_f32 ? 4 : 2) * at));
+    }
+  }
+  float4 b;  // of features f0 + 4 lane + 0 .. 3, or f0 + lane + 32 * 0 .. 3
+  if (whole) {
+    b = bias4(a, f0 + 4 * lane);
+  } else {
+    b.x = f0 + lane < a.n ? bias1(a, f0 + lane) : 0.f;
+    b.y = f0 + lane + 32 < a.n ? bias1(a, f0 + lane + 32) : 0.f;
+    b.z = f0 + lane + 64 < a.n ? bias1(a, f0 + lane + 64) : 0.f;
+    b.w = f0 + lane + 96 < a.n ? bias1(a, f0 + lane + 96) : 0.f;
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -213,17 +255,15 @@ __global__ void __launch_bounds__(Few<BT>::kThreads, 2) few_kernel(const __grid_
   if (warp == 0) {
     if (lane == 0) {
       int stage = 0;
-      uint32_t phase = 0, issued[C::kStages];
-      for (int s = 0; s < C::kStages; ++s) issued[s] = 0xFFFFFFFFu;
+      uint32_t phase = 1, issued[C::kStages];
+      for (int s = 0; s < C::kStages; ++s) issued[s] = kb0 + s < kb1 ? 0u : 0xFFFFFFFFu;
       bool ok = true;
-      for (int kb = kb0; kb < kb1; ++kb) {
+      for (int kb = kb0 + C::kStages; kb < kb1; ++kb) {
         if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, a.status, FB_DEV_TIMEOUT_MMA)) {
           ok = false;
           break;
         }
-        mbar_arrive_expect_tx(&full[stage], C::kStageBytes);
-        tma_load_2d(&a.tma_w, &full[stage], sW + stage * C::kWBytes, kb * BK, f0);
-        tma_load_2d(&a.tma_x, &full[stage], sX + stage * C::kXBytes, kb * BK, t0);
+        load(stage, kb);
         issued[stage] = phase;
         if (++stage == C::kStages) {
           stage = 0;
@@ -299,34 +339,31 @@ __global__ void __launch_bounds__(Few<BT>::kThreads, 2) few_kernel(const __grid_
     __syncthreads();
   }
 
-  // This CTA's share of the tile's tokens, U tokens per warp at a time: a lane finishes four consecutive features of
-  // each (vectors), or features lane, lane + 32, .. (rows of any alignment).
-  const int live = min(BT, a.m - t0);
-  const int j1 = live * (rank + 1) / a.splits;
-  constexpr int U = 4;
+  // U tokens per warp at a time: a lane finishes four features of each.
+  constexpr int U = 2;
   const uint32_t base = smem_u32(tile);
-  const bool tail = !a.vec || f0 + kFeat > a.n;  // any lane's four features may end early
-  if (!tail) {
+  if (whole) {
     const int n0 = f0 + 4 * lane;
-    const float4 b = bias4(a, n0);
 #pragma unroll 1
-    for (int j = live * rank / a.splits + warp; j < j1; j += U * C::kWarps) {
+    for (int j = j0 + warp; j < j1; j += U * C::kWarps) {
       float4 r[U], z[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (j + u * C::kWarps < j1) r[u] = residual4(a, t0 + j + u * C::kWarps, n0);
-#pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int ju = min(j + u * C::kWarps, BT - 1);
-        z[u] = a.splits > 1 ? ld_shared_cluster_f4(mapa_shared(base + (ju * kFeat + 4 * lane) * 4, 0))
-                            : *reinterpret_cast<const float4*>(tile + ju * kFeat + 4 * lane);
+        const int ju = min(j + u * C::kWarps, BT - 1);  // past the share: read, not written
+        z[u] = *reinterpret_cast<const float4*>(tile + ju * kFeat + 4 * lane);
+        if (j + u * C::kWarps < j1) r[u] = residual4(a, t0 + j + u * C::kWarps, n0);
       }
-      for (int s = 1; s < a.splits; ++s) {
+      if (a.splits > 1) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int ju = min(j + u * C::kWarps, BT - 1);
-          const float4 p = ld_shared_cluster_f4(mapa_shared(base + (ju * kFeat + 4 * lane) * 4, s));
-          z[u].x += p.x, z[u].y += p.y, z[u].z += p.z, z[u].w += p.w;
+        for (int u = 0; u < U; ++u) z[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int s = 0; s < a.splits; ++s) {
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int ju = min(j + u * C::kWarps, BT - 1);
+            const float4 p = ld_shared_cluster_f4(mapa_shared(base + (ju * kFeat + 4 * lane) * 4, s));
+            z[u].x += p.x, z[u].y += p.y, z[u].z += p.z, z[u].w += p.w;
+          }
         }
       }
 #pragma unroll
@@ -334,14 +371,12 @@ __global__ void __launch_bounds__(Few<BT>::kThreads, 2) few_kernel(const __grid_
         if (j + u * C::kWarps < j1) finish4<ACT>(a, t0 + j + u * C::kWarps, n0, z[u], b, r[u]);
     }
   } else {
-    float b[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) b[i] = f0 + lane + 32 * i < a.n ? bias1(a, f0 + lane + 32 * i) : 0.f;
+    const float bs[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll 1
-    for (int j = live * rank / a.splits + warp; j < j1; j += 2 * C::kWarps) {
-      float r[2][4], z[2][4];
+    for (int j = j0 + warp; j < j1; j += U * C::kWarps) {
+      float r[U][4], z[U][4];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int u = 0; u < U; ++u) {
         const int ju = j + u * C::kWarps;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -350,9 +385,10 @@ __global__ void __launch_bounds__(Few<BT>::kThreads, 2) few_kernel(const __grid_
           z[u][i] = 0.f;
         }
       }
+#pragma unroll 2
       for (int s = 0; s < a.splits; ++s) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < U; ++u) {
           const int ju = min(j + u * C::kWarps, BT - 1);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -370,17 +406,19 @@ __global__ void __launch_bounds__(Few<BT>::kThreads, 2) few_kernel(const __grid_
         }
       }
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int n = f0 + lane + 32 * i;
-          if (j + u * C::kWarps < j1 && n < a.n) finish1<ACT>(a, t0 + j + u * C::kWarps, n, z[u][i], b[i], r[u][i]);
+          if (j + u * C::kWarps < j1 && n < a.n) finish1<ACT>(a, t0 + j + u * C::kWarps, n, z[u][i], bs[i], r[u][i]);
         }
     }
   }
   __syncwarp();
   if (a.splits > 1) {
-    cluster_sync_all();  // nobody reads this CTA's tile any more
+    // Nobody reads this CTA's tile any more: what was read has been used, so this barrier orders no memory (with
+    // release semantics it would also wait for the outputs to reach L2).
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
   } else {
     __syncthreads();
   }
@@ -394,7 +432,7 @@ __global__ void __launch_bounds__(Few<BT>::kThreads, 2) few_kernel(const __grid_
 
 // A cluster of two CTAs per 256 x 256 tile: each loads its own 128 token rows and 128 of the 256 weight rows, the leader
 // issues M = 256, N = 256 MMAs that read both, and each CTA's TMEM gets its 128 rows (256 columns, two accumulators).
-// An operand stage is 128 of K (two 64-wide boxes of each operand, 64 KB per CTA), an accumulator takes four stages.
+// An operand stage is 128 of K (two 64-wide boxes of each operand, 64 KB per CTA), an accumulator takes eight stages.
 // Eight epilogue warps, two per TMEM lane quarter, hold the 128 sums of their half row in registers; a finished tile
 // goes through 4 KB of shared memory per warp, 32 x 32 values at a time, so that residuals and outputs are contiguous
 // accesses, while the tensor core already works on the next tile.
@@ -407,7 +445,7 @@ constexpr int kThreads = 128 + 32 * kEpiWarps;
 constexpr int kLeanRegs = 40, kEpiRegs = 232;
 constexpr int kSub = 2;
 constexpr int kStages = 3;
-constexpr int kChunkStages = 4;
+constexpr int kChunkStages = 8;
 constexpr int kBoxBytes = 128 * BK * 2;
 constexpr int kOpBytes = kSub * kBoxBytes;
 constexpr int kStageBytes = 2 * kOpBytes;
@@ -562,6 +600,14 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
     for (int tile = pair; ok && tile < tiles; tile += npairs) {
       int mb, nb;
       place(a, tile, mb, nb);
+      const int row0 = mb * kTile + 128 * rank + quarter * 32;
+      if (a.residual != nullptr && row0 + lane < a.m) {  // the row's 128 residuals: in L2 by the time the sums are there
+        const int n0 = nb * kTile + part * 128, line = a.res_f32 ? 32 : 64;
+        for (int n = n0; n < min(n0 + 128, a.n); n += line) {
+          const int64_t at = static_cast<int64_t>(row0 + lane) * a.ld_res + n;
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint8_t*>(a.residual) + (a.res_f32 ? 4 : 2) * at));
+        }
+      }
       float v[128];
       for (int kc = 0; kc < nstage; kc += kChunkStages) {
         if (!mbar_wait(&acc_full[acc], acc_phase, abort_flag, a.status, FB_DEV_TIMEOUT_MMA)) {
@@ -577,7 +623,6 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
         if (acc == 0) acc_phase ^= 1u;
       }
       if (!ok) break;
-      const int row0 = mb * kTile + 128 * rank + quarter * 32;
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         const int n0 = nb * kTile + part * 128 + 32 * c;
@@ -597,20 +642,17 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
           if (a.vec && n0 + 32 <= a.n) {
             const int u = lane & 7, n = n0 + 4 * u;
             const float4 b = bias4(a, n);
-#pragma unroll 1
-            for (int h = 0; h < 2; ++h) {
-              float4 r[4];
+            float4 r[8];
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int row = 16 * h + 4 * i + (lane >> 3);
-                if (row0 + row < a.m) r[i] = residual4(a, row0 + row, n);
-              }
+            for (int i = 0; i < 8; ++i) {
+              const int row = 4 * i + (lane >> 3);
+              if (row0 + row < a.m) r[i] = residual4(a, row0 + row, n);
+            }
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int row = 16 * h + 4 * i + (lane >> 3);
-                const float4 z = *reinterpret_cast<const float4*>(patch + row * 128 + ((u ^ (row & 7)) << 4));
-                if (row0 + row < a.m) finish4<ACT>(a, row0 + row, n, z, b, r[i]);
-              }
+            for (int i = 0; i < 8; ++i) {
+              const int row = 4 * i + (lane >> 3);
+              const float4 z = *reinterpret_cast<const float4*>(patch + row * 128 + ((u ^ (row & 7)) << 4));
+              if (row0 + row < a.m) finish4<ACT>(a, row0 + row, n, z, b, r[i]);
             }
           } else {
             const int n = n0 + lane;
@@ -837,9 +879,9 @@ int launch_linear_act(const fb_linear_act_args& p, cudaStream_t st, std::string&
     a.tiles_t = (p.m + bt - 1) / bt;
     const int64_t tiles = static_cast<int64_t>(a.tiles_f) * a.tiles_t;
     if (tiles > (1ll << 27)) return bad(FB_ERR_UNSUPPORTED, "too many output tiles");
-    // Split K over a cluster while all CTAs still fit the GPU at once (two per SM) and each gets four K blocks.
+    // Split K over a cluster until every SM has a CTA, as long as each gets four K blocks.
     a.splits = 1;
-    while (a.splits < 8 && tiles * (a.splits + 1) <= 2 * kNumSms && a.num_kb >= 4 * (a.splits + 1)) ++a.splits;
+    while (a.splits < 8 && tiles * (a.splits + 1) <= kNumSms && a.num_kb >= 4 * (a.splits + 1)) ++a.splits;
     const int ctas = static_cast<int>(tiles * a.splits);
     e = with_act(p.act, [&](auto c) { return go_few<decltype(c)::value>(a, bt, ctas, st); });
   }

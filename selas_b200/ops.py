@@ -405,13 +405,17 @@ def _raw_stream(index: int) -> int:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
 
 
-def _one_device(what: str, *ts: torch.Tensor | None) -> int:
+def _refuse(msg: str) -> None:
+    raise FluxB200Error(msg)
+
+
+def _one_device(what: str, x: torch.Tensor, *others: torch.Tensor | None) -> int:
     """The index of the one CUDA device of all the given tensors."""
-    _cuda(ts[0])
-    index = ts[0].get_device()
-    for t in ts:
+    _cuda(x)
+    index = x.get_device()
+    for t in others:
         if t is not None and t.get_device() != index:
-            raise FluxB200Error(f"{what}: every tensor must be on one CUDA device, got {ts[0].device} and {t.device}")
+            _refuse(f"{what}: every tensor must be on one CUDA device, got {x.device} and {t.device}")
     return index
 
 
@@ -444,38 +448,53 @@ def _rope_plan(axes_dim: tuple, theta) -> tuple:
 
 def _rope(q: torch.Tensor, k: torch.Tensor | None, ids: torch.Tensor, axes_dim, theta, pairs: str, inverse: bool):
     index = _one_device("rope_axes", q, k, ids)
-    _need(q.dim() == 4 and q.dtype in _DTYPE_CODE, "rope_axes: fp32, bf16 or fp16 [B, H, L, hd] tensors")
+    dtype = q.dtype
+    code = _DTYPE_CODE.get(dtype)
+    if code is None or q.dim() != 4:
+        _refuse("rope_axes: fp32, bf16 or fp16 [B, H, L, hd] tensors")
     b, h, l, hd = q.shape
     axes_dim = tuple(axes_dim)
     total, arrays = _rope_plan(axes_dim, tuple(theta) if isinstance(theta, (tuple, list)) else theta)
-    _need(hd == total, f"rope_axes: the axes' dims {axes_dim} must add up to head_dim {hd}")
-    _need(pairs in _PAIRS, f"rope_axes: pairs is 'interleaved' or 'halves', got {pairs!r}")
-    _need(ids.dtype in _IDS_CODE, "rope_axes: ids must be fp32, fp64, int32 or int64")
-    ishape, istride = ids.shape, ids.stride()
-    _need(len(ishape) in (2, 3) and ishape[-1] == len(axes_dim) and ishape[-2] == l and (len(ishape) == 2 or ishape[0] in (1, b)),
-          f"rope_axes: ids must be [L, axes] or [B, L, axes], got {tuple(ishape)}")
-    ib = istride[0] if len(ishape) == 3 and ishape[0] > 1 else 0
-    sb, sh, sl, se = q.stride()
-    out_k, tensors, n = None, None, q.numel()
-    _need(se == 1, "rope_axes: q and k must be [B, H, L, hd] of one type with unit stride along hd")
-    out_q = q.new_empty((b, h, l, hd))
-    tensors = (q.data_ptr(), out_q.data_ptr(), sb, sh, sl, h * l * hd, l * hd, hd, h)
+    if hd != total:
+        _refuse(f"rope_axes: the axes' dims {axes_dim} must add up to head_dim {hd}")
+    order = _PAIRS.get(pairs)
+    if order is None:
+        _refuse(f"rope_axes: pairs is 'interleaved' or 'halves', got {pairs!r}")
+    ids_code = _IDS_CODE.get(ids.dtype)
+    shape = ids.shape
+    if ids_code is None:
+        _refuse("rope_axes: ids must be fp32, fp64, int32 or int64")
+    if shape == (l, len(axes_dim)):
+        ib = 0
+        il, ia = ids.stride()
+    elif len(shape) == 3 and shape[1:] == (l, len(axes_dim)) and shape[0] in (1, b):
+        ib, il, ia = ids.stride()
+        ib = ib if shape[0] > 1 else 0
+    else:
+        _refuse(f"rope_axes: ids must be [L, axes] or [B, L, axes], got {tuple(shape)}")
+    sb, sh, sl, one = q.stride()
+    if one != 1:
+        _refuse("rope_axes: q and k must be [B, H, L, hd] of one type with unit stride along hd")
+    out_q, out_k, count = q.new_empty((b, h, l, hd)), None, 1
+    rows, heads = l * hd, h
+    tensors = (q.data_ptr(), out_q.data_ptr(), sb, sh, sl, h * rows, rows, hd, h)
     if k is None:
         tensors += (0,) * 9
     else:
-        _need(k.dim() == 4 and k.dtype == q.dtype, "rope_axes: q and k must be [B, H, L, hd] of one type with unit stride along hd")
-        kb, hk, lk, hdk = k.shape
-        sb, sh, sl, se = k.stride()
-        _need(kb == b and lk == l and hdk == hd and se == 1,
-              "rope_axes: q and k must be [B, H, L, hd] of one type with unit stride along hd")
-        out_k = k.new_empty((b, hk, l, hd))
-        tensors += (k.data_ptr(), out_k.data_ptr(), sb, sh, sl, hk * l * hd, l * hd, hd, hk)
-        n += k.numel()
+        if k.dtype != dtype or k.dim() != 4:
+            _refuse("rope_axes: q and k must be [B, H, L, hd] of one type with unit stride along hd")
+        kb, kh, kl, kd = k.shape
+        sb, sh, sl, one = k.stride()
+        if kb != b or kl != l or kd != hd or one != 1:
+            _refuse("rope_axes: q and k must be [B, H, L, hd] of one type with unit stride along hd")
+        out_k, count = k.new_empty((b, kh, l, hd)), 2
+        heads += kh
+        tensors += (k.data_ptr(), out_k.data_ptr(), sb, sh, sl, kh * rows, rows, hd, kh)
+    n = b * heads * rows
     if n:
-        code = _DTYPE_CODE[q.dtype]
-        _launch(index, "rope_axes", 0.0, 2 * n * q.element_size(), _lib.pack_rope(
-            *tensors, ids.data_ptr(), ib, istride[-2], istride[-1], *arrays, 1 if k is None else 2, code, b, l, hd,
-            _IDS_CODE[ids.dtype], len(axes_dim), _PAIRS[pairs], bool(inverse)))
+        _launch(index, "rope_axes", 0.0, 2 * n * (4 if code == _lib.FB_F32 else 2), _lib.pack_rope(
+            *tensors, ids.data_ptr(), ib, il, ia, *arrays, count, code, b, l, hd, ids_code, len(axes_dim), order,
+            1 if inverse else 0))
     return out_q, out_k
 
 
@@ -502,31 +521,35 @@ def _outer_inner(what: str, t: torch.Tensor) -> tuple[int, int]:
     """(outer, inner) strides of the rows of t [..., D] seen as [outer, inner, D]."""
     st = t.stride()
     n = len(st)
-    _need(st[-1] == 1 or t.shape[-1] == 1, f"{what}: the last dim must have unit stride")
+    if st[-1] != 1 and t.shape[-1] != 1:
+        _refuse(f"{what}: the last dim must have unit stride")
+    if n == 3:
+        return st[0], st[1]
     if n <= 2:
         return 0, st[0] if n == 2 else 0
-    if n > 3 and not t.is_contiguous():
-        raise FluxB200Error(f"{what}: a tensor of more than three dims must be contiguous")
+    if not t.is_contiguous():
+        _refuse(f"{what}: a tensor of more than three dims must be contiguous")
     return st[-3], st[-2]
 
 
-def _norm_rows(what: str, x: torch.Tensor) -> tuple[int, int, int]:
-    """(outer, inner, D) of x [..., D]."""
+def _norm_rows(what: str, x: torch.Tensor) -> tuple[int, int, int, int]:
+    """(outer, inner, D, type code) of x [..., D]."""
     shape = x.shape
     n = len(shape)
-    _need(n >= 1 and x.dtype in _DTYPE_CODE and shape[-1] > 0, f"{what}: x must be fp32, bf16 or fp16 [..., D]")
-    return math.prod(shape[:-2]), shape[-2] if n > 1 else 1, shape[-1]
+    code = _DTYPE_CODE.get(x.dtype)
+    if code is None or n < 1 or shape[-1] < 1:
+        _refuse(f"{what}: x must be fp32, bf16 or fp16 [..., D]")
+    if n == 3:
+        return *shape, code
+    return math.prod(shape[:-2]), shape[-2] if n > 1 else 1, shape[-1], code
 
 
-def _norm_map(what: str, d: int, weight: torch.Tensor | None, bias: torch.Tensor | None) -> tuple[int, int, int]:
-    """(weight, bias, type code) of the affine map."""
-    code = 0
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None:
-            _need(t.dtype in _DTYPE_CODE and t.shape == (d,) and t.is_contiguous(), f"{what}: {name} must be fp32, bf16 or fp16 [D]")
-            code = _DTYPE_CODE[t.dtype]
-    _need(weight is None or bias is None or weight.dtype == bias.dtype, f"{what}: weight and bias must share a type")
-    return weight.data_ptr() if weight is not None else 0, bias.data_ptr() if bias is not None else 0, code
+def _norm_vector(what: str, name: str, d: int, t: torch.Tensor) -> tuple[int, int]:
+    """(pointer, type code) of a weight or bias."""
+    code = _DTYPE_CODE.get(t.dtype)
+    if code is None or t.shape != (d,) or not t.is_contiguous():
+        _refuse(f"{what}: {name} must be fp32, bf16 or fp16 [D]")
+    return t.data_ptr(), code
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5,
@@ -535,34 +558,49 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     strided), statistics in fp32, rounded once to ``out_dtype`` (x's by default). weight and bias: [D] of one type, or
     None. Returns a contiguous tensor."""
     index = _one_device("layer_norm", x, weight, bias)
-    outer, inner, d = _norm_rows("layer_norm", x)
-    w, b, w_code = _norm_map("layer_norm", d, weight, bias)
+    outer, inner, d, code = _norm_rows("layer_norm", x)
+    w = b = w_code = 0
+    if weight is not None:
+        w, w_code = _norm_vector("layer_norm", "weight", d, weight)
+    if bias is not None:
+        b, b_code = _norm_vector("layer_norm", "bias", d, bias)
+        if weight is not None and b_code != w_code:
+            _refuse("layer_norm: weight and bias must share a type")
+        w_code = b_code
     out_dtype = x.dtype if out_dtype is None else out_dtype
-    _need(out_dtype in _DTYPE_CODE, "layer_norm: out_dtype must be fp32, bf16 or fp16")
+    out_code = _DTYPE_CODE.get(out_dtype)
+    if out_code is None:
+        _refuse("layer_norm: out_dtype must be fp32, bf16 or fp16")
     xo, xi = _outer_inner("layer_norm", x)
     out = x.new_empty(x.shape, dtype=out_dtype)
-    if outer * inner:
-        _launch(index, "layer_norm", 0.0, out.numel() * (x.element_size() + out.element_size()), _lib.pack_layer_norm(
+    rows = outer * inner
+    if rows:
+        nbytes = rows * d * ((4 if code == _lib.FB_F32 else 2) + (4 if out_code == _lib.FB_F32 else 2))
+        _launch(index, "layer_norm", 0.0, nbytes, _lib.pack_layer_norm(
             x.data_ptr(), xo, xi, 0, 0, 0, 0, 0, 0, out.data_ptr(), inner * d, d, w, b, 0, 0, 0, 0, 0, outer, inner, d,
-            _DTYPE_CODE[x.dtype], _DTYPE_CODE[out_dtype], w_code, 0, 0, eps))
+            code, out_code, w_code, 0, 0, eps))
     return out
 
 
 def _norm_backward(what: str, index: int, dy, x, eps: float, weight: int, w_code: int, w_stride: int, plus_one: bool, add,
                    sums: bool, groups: int):
     """(dx, dweight, dbias) with one dweight and dbias per group of rows: all rows, or those of an outer index."""
-    outer, inner, d = _norm_rows(what, x)
-    _need(dy.dtype in _DTYPE_CODE and dy.shape == x.shape, f"{what}: dy must be fp32, bf16 or fp16 of x's shape")
+    outer, inner, d, code = _norm_rows(what, x)
+    y_code = _DTYPE_CODE.get(dy.dtype)
+    if y_code is None or dy.shape != x.shape:
+        _refuse(f"{what}: dy must be fp32, bf16 or fp16 of x's shape")
     xo, xi = _outer_inner(what, x)
     yo, yi = _outer_inner(what, dy)
-    ao = ai = 0
+    ad = ao = ai = 0
     if add is not None:
-        _need(add.dtype == x.dtype and add.shape == x.shape, f"{what}: add must be of x's shape and type")
+        if add.dtype != x.dtype or add.shape != x.shape:
+            _refuse(f"{what}: add must be of x's shape and type")
         ao, ai = _outer_inner(what, add)
+        ad = add.data_ptr()
     dx = x.new_empty(x.shape)
     dw = db = None
     pw = pb = work = need = 0
-    per_outer = groups > 1
+    per_outer = 1 if groups > 1 else 0
     if sums:
         # the two gradients and the partial sums in one allocation
         need = _lib.load().fb_layer_norm_work_floats(outer, inner, d, per_outer)
@@ -571,13 +609,12 @@ def _norm_backward(what: str, index: int, dy, x, eps: float, weight: int, w_code
         dw, db = buf[:n], buf[n:2 * n]
         pw = buf.data_ptr()
         pb, work = pw + 4 * n, pw + 8 * n
-    if outer * inner or (sums and groups):
-        es = x.element_size()
-        _launch(index, "layer_norm_backward", 0.0, dx.numel() * ((2 if add is None else 3) * es + dy.element_size()),
-                _lib.pack_layer_norm(
-                    x.data_ptr(), xo, xi, dy.data_ptr(), yo, yi, 0 if add is None else add.data_ptr(), ao, ai, dx.data_ptr(),
-                    inner * d, d, weight, 0, w_stride, pw, pb, work, need, outer, inner, d, _DTYPE_CODE[x.dtype],
-                    _DTYPE_CODE[dy.dtype], w_code, plus_one, per_outer, eps))
+    rows = outer * inner
+    if rows or (sums and groups):
+        nbytes = rows * d * ((2 if add is None else 3) * (4 if code == _lib.FB_F32 else 2) + (4 if y_code == _lib.FB_F32 else 2))
+        _launch(index, "layer_norm_backward", 0.0, nbytes, _lib.pack_layer_norm(
+            x.data_ptr(), xo, xi, dy.data_ptr(), yo, yi, ad, ao, ai, dx.data_ptr(), inner * d, d, weight, 0, w_stride, pw,
+            pb, work, need, outer, inner, d, code, y_code, w_code, plus_one, per_outer, eps))
     return dx, dw, db
 
 
@@ -589,7 +626,9 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor 
     stream. dx has x's type; dweight = sum of dy * xhat and dbias = sum of dy are fp32 [D], summed in a fixed order;
     ``sums=False`` leaves them out (None)."""
     index = _one_device("layer_norm_backward", x, dy, weight, add)
-    w, _, w_code = _norm_map("layer_norm_backward", _norm_rows("layer_norm_backward", x)[2], weight, None)
+    w = w_code = 0
+    if weight is not None:
+        w, w_code = _norm_vector("layer_norm_backward", "weight", x.shape[-1] if x.dim() else 0, weight)
     return _norm_backward("layer_norm_backward", index, dy, x, eps, w, w_code, 0, False, add, sums, 1)
 
 
@@ -635,27 +674,34 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = Non
     ``linear`` with its fused epilogues, nothing is rounded before the activation and the residual."""
     index = _one_device("linear_act", x, w, bias, residual)
     dt = x.dtype
-    _need(dt in (BF16, torch.float16) and w.dtype == dt, "linear_act: x and w must both be bf16 or both fp16")
+    if (dt != BF16 and dt != torch.float16) or w.dtype != dt:
+        _refuse("linear_act: x and w must both be bf16 or both fp16")
     shape = x.shape
-    _need(len(shape) >= 1 and w.dim() == 2 and shape[-1] == w.shape[1], f"linear_act: K mismatch {tuple(shape)} x {tuple(w.shape)}")
-    _need(act in ACTIVATIONS, f"linear_act: act must be one of {sorted(ACTIVATIONS)}, got {act!r}")
+    if len(shape) < 1 or w.dim() != 2 or shape[-1] != w.shape[1]:
+        _refuse(f"linear_act: K mismatch {tuple(shape)} x {tuple(w.shape)}")
+    act_code = ACTIVATIONS.get(act)
+    if act_code is None:
+        _refuse(f"linear_act: act must be one of {sorted(ACTIVATIONS)}, got {act!r}")
     out_dtype = dt if out_dtype is None else out_dtype
-    _need(out_dtype in (dt, F32), "linear_act: out_dtype must be x's type or fp32")
+    if out_dtype != dt and out_dtype != F32:
+        _refuse("linear_act: out_dtype must be x's type or fp32")
     n, k = w.shape
-    _need(n >= 1, "linear_act: w needs at least one row")
+    if n < 1:
+        _refuse("linear_act: w needs at least one row")
     lead = shape[:-1]
     m = math.prod(lead)
     x, ldx = _rows(x, m, k)
     w, ldw = _rows(w, n, k)
-    r = ldr = b = 0
-    res_code = 0
+    code = _DTYPE_CODE[dt]
+    r = ldr = b = res_code = 0
     if residual is not None:
-        _need(residual.dtype in (dt, F32) and residual.shape[:-1] == lead and residual.shape[-1] == n,
-              "linear_act: residual must be [..., N] of x's type or fp32")
+        if (residual.dtype != dt and residual.dtype != F32) or residual.shape[:-1] != lead or residual.shape[-1] != n:
+            _refuse("linear_act: residual must be [..., N] of x's type or fp32")
         residual, ldr = _rows(residual, m, n)
         r, res_code = residual.data_ptr(), _DTYPE_CODE[residual.dtype]
     if bias is not None:
-        _need(bias.dtype == dt and bias.shape == (n,) and bias.is_contiguous(), "linear_act: bias must be [N] of x's type")
+        if bias.dtype != dt or bias.shape != (n,) or not bias.is_contiguous():
+            _refuse("linear_act: bias must be [N] of x's type")
         b = bias.data_ptr()
     out = x.new_empty((*lead, n), dtype=out_dtype)
     if m == 0:
@@ -666,9 +712,10 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = Non
         need = _lib.load().fb_linear_act_work_bytes(_lib.pack_linear_act(px, ldx, pw, ldw, *(0,) * 7, m, n, k, 0, 0, 0, 0))
         copies = x.new_empty(need, dtype=torch.uint8)
         work = copies.data_ptr()
-    _launch(index, "linear_act", 2.0 * m * n * k, (m * k + n * k) * 2 + m * n * out.element_size(), _lib.pack_linear_act(
-        px, ldx, pw, ldw, b, r, ldr, out.data_ptr(), n, work, need, m, n, k, _DTYPE_CODE[dt], res_code,
-        _DTYPE_CODE[out_dtype], ACTIVATIONS[act]))
+    out_code = _DTYPE_CODE[out_dtype]
+    _launch(index, "linear_act", 2.0 * m * n * k, (m * k + n * k) * 2 + m * n * (4 if out_code == _lib.FB_F32 else 2),
+            _lib.pack_linear_act(px, ldx, pw, ldw, b, r, ldr, out.data_ptr(), n, work, need, m, n, k, code, res_code, out_code,
+                                 act_code))
     return out
 
 

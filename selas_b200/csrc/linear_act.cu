@@ -19,6 +19,7 @@
 // 1.3e-5 of the result's norm), so an accumulator takes 1024 of K at most; the epilogue warps then add it to fp32
 // registers, which are the sum proper, while the other TMEM buffer takes the next 1024. That costs 2 % of the time at
 // most (every 512 cost 10 %) and holds the error of an fp32 output near 1e-6.
+#include <atomic>
 #include <type_traits>
 
 #include "gemm_common.cuh"
@@ -50,18 +51,28 @@ struct Args {
 // z < 0 and z - z h otherwise, h = erfc(|x|) / 2, which keeps the small values of the negative side. With CUDA's erff the
 // epilogue of a 256 x 256 tile at K = 3072 took longer than its products. The sigmoids divide by 1 + exp with the
 // hardware's exp2 and division (2 ulp); tanh(u) = 2 sigmoid(2u) - 1.
+__device__ __forceinline__ float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 template <int ACT>
 __device__ __forceinline__ float activate(float z) {
   if constexpr (ACT == FB_ACT_RELU) return z < 0.f ? 0.f : z;  // keeps a NaN
   if constexpr (ACT == FB_ACT_GELU) {
-    const float x = fabsf(z) * 0.70710678118654752f;
-    const float t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
+    const float s = fminf(fabsf(z), 30.f);  // past 30 nothing is left of erfc; keeps inf * 0 out
+    const float t = rcp_approx(fmaf(0.3275911f * 0.70710678f, s, 1.0f));
     float h = fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
     h = fmaf(h, t, 0.5f * 1.421413741f);
     h = fmaf(h, t, 0.5f * -0.284496736f);
     h = fmaf(h, t, 0.5f * 0.254829592f);
-    const float zh = z * (h * t * __expf(-x * x));
-    return z < 0.f ? zh : z - zh;
+    const float q = 0.84932180f * z;  // sqrt(log2(e) / 2)
+    return fmaf(-s, h * t * exp2_approx(-q * q), fmaxf(z, 0.f));
   }
   if constexpr (ACT == FB_ACT_GELU_TANH) {
     const float u = 0.7978845608028654f * fmaf(0.044715f * z * z, z, z);  // sqrt(2 / pi) (z + 0.044715 z^3)
@@ -73,14 +84,33 @@ __device__ __forceinline__ float activate(float z) {
 }
 
 // 16-bit value of the operands' type widened to fp32, and back.
-__device__ __forceinline__ float widen(uint32_t v, int half) {
-  return half ? __half2float(__ushort_as_half(static_cast<uint16_t>(v))) : __uint_as_float(v << 16);
+template <bool HALF>
+__device__ __forceinline__ float widen(uint32_t v) {
+  return HALF ? __half2float(__ushort_as_half(static_cast<uint16_t>(v))) : __uint_as_float(v << 16);
 }
-__device__ __forceinline__ uint32_t narrow(float v, int half) {
-  return half ? __half_as_ushort(__float2half_rn(v)) : __bfloat16_as_ushort(__float2bfloat16_rn(v));
+template <bool HALF>
+__device__ __forceinline__ float4 widen4(uint2 u) {
+  if constexpr (HALF) {
+    const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
+    const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+    return make_float4(lo.x, lo.y, hi.x, hi.y);
+  } else {
+    return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16),
+                       __uint_as_float(u.y & 0xFFFF0000u));
+  }
 }
-__device__ __forceinline__ float4 widen4(uint2 u, int half) {
-  return make_float4(widen(u.x & 0xFFFFu, half), widen(u.x >> 16, half), widen(u.y & 0xFFFFu, half), widen(u.y >> 16, half));
+template <bool HALF>
+__device__ __forceinline__ uint2 narrow4(float4 v) {
+  if constexpr (HALF) {
+    const __half2 lo = __floats2half2_rn(v.x, v.y), hi = __floats2half2_rn(v.z, v.w);
+    return make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+  } else {
+    return make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+  }
+}
+template <bool HALF>
+__device__ __forceinline__ uint16_t narrow(float v) {
+  return HALF ? __half_as_ushort(__float2half_rn(v)) : __bfloat16_as_ushort(__float2bfloat16_rn(v));
 }
 
 __device__ __forceinline__ float4 ld_shared_cluster_f4(uint32_t addr) {
@@ -92,46 +122,201 @@ __device__ __forceinline__ float4 ld_shared_cluster_f4(uint32_t addr) {
   return v;
 }
 
-// Four consecutive features n0 .. n0 + 3 of a token as aligned vectors (n0 + 4 <= n), and one feature of any alignment.
+__device__ __forceinline__ float4 ld_shared_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// Four consecutive features n0 .. n0 + 3 as aligned vectors, for N tokens at a time: token + i * step, of which those
+// below `end` exist. What a call's types decide is decided once for all of them: a branch in every step costs more than
+// the step.
 __device__ __forceinline__ float4 bias4(const Args& a, int n0) {
   if (a.bias == nullptr) return make_float4(0.f, 0.f, 0.f, 0.f);
-  return widen4(__ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.bias) + n0)), a.half);
+  const uint2 u = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.bias) + n0));
+  return a.half ? widen4<true>(u) : widen4<false>(u);
 }
-__device__ __forceinline__ float4 residual4(const Args& a, int token, int n0) {
-  if (a.residual == nullptr) return make_float4(0.f, 0.f, 0.f, 0.f);
-  const int64_t at = static_cast<int64_t>(token) * a.ld_res + n0;
-  if (a.res_f32) return *reinterpret_cast<const float4*>(static_cast<const float*>(a.residual) + at);
-  return widen4(*reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.residual) + at), a.half);
-}
-template <int ACT>
-__device__ __forceinline__ void finish4(const Args& a, int token, int n0, float4 z, float4 b, float4 r) {
-  const float y0 = activate<ACT>(z.x + b.x) + r.x, y1 = activate<ACT>(z.y + b.y) + r.y;
-  const float y2 = activate<ACT>(z.z + b.z) + r.z, y3 = activate<ACT>(z.w + b.w) + r.w;
-  const int64_t at = static_cast<int64_t>(token) * a.ld_out + n0;
-  if (a.out_f32) {
-    *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = make_float4(y0, y1, y2, y3);
+template <int N>
+__device__ __forceinline__ void residuals(const Args& a, int token, int step, int end, int n0, float4 (&r)[N]) {
+  const int64_t at = token * a.ld_res + n0, by = step * a.ld_res;
+  if (a.residual == nullptr) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  } else if (a.res_f32) {
+    const float* p = static_cast<const float*>(a.residual) + at;
+#pragma unroll
+    for (int i = 0; i < N; ++i, p += by)
+      if (token + i * step < end) r[i] = *reinterpret_cast<const float4*>(p);
   } else {
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) =
-        make_uint2(narrow(y0, a.half) | narrow(y1, a.half) << 16, narrow(y2, a.half) | narrow(y3, a.half) << 16);
+    const uint16_t* p = static_cast<const uint16_t*>(a.residual) + at;
+    uint2 u[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i, p += by)
+      if (token + i * step < end) u[i] = *reinterpret_cast<const uint2*>(p);
+    if (a.half) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) r[i] = widen4<true>(u[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) r[i] = widen4<false>(u[i]);
+    }
   }
 }
+// z: the sums, overwritten
+template <int ACT, int N>
+__device__ __forceinline__ void finish(const Args& a, int token, int step, int end, int n0, float4 b, const float4 (&r)[N], float4 (&z)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    z[i].x = activate<ACT>(z[i].x + b.x) + r[i].x;
+    z[i].y = activate<ACT>(z[i].y + b.y) + r[i].y;
+    z[i].z = activate<ACT>(z[i].z + b.z) + r[i].z;
+    z[i].w = activate<ACT>(z[i].w + b.w) + r[i].w;
+  }
+  const int64_t at = token * a.ld_out + n0, by = step * a.ld_out;
+  if (a.out_f32) {
+    float* p = static_cast<float*>(a.out) + at;
+#pragma unroll
+    for (int i = 0; i < N; ++i, p += by)
+      if (token + i * step < end) *reinterpret_cast<float4*>(p) = z[i];
+  } else {
+    uint16_t* p = static_cast<uint16_t*>(a.out) + at;
+    if (a.half) {
+#pragma unroll
+      for (int i = 0; i < N; ++i, p += by)
+        if (token + i * step < end) *reinterpret_cast<uint2*>(p) = narrow4<true>(z[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i, p += by)
+        if (token + i * step < end) *reinterpret_cast<uint2*>(p) = narrow4<false>(z[i]);
+    }
+  }
+}
+// One feature of one token, any alignment.
 __device__ __forceinline__ float bias1(const Args& a, int n) {
-  return a.bias == nullptr ? 0.f : widen(__ldg(static_cast<const uint16_t*>(a.bias) + n), a.half);
+  if (a.bias == nullptr) return 0.f;
+  const uint16_t v = __ldg(static_cast<const uint16_t*>(a.bias) + n);
+  return a.half ? widen<true>(v) : widen<false>(v);
 }
-__device__ __forceinline__ float residual1(const Args& a, int token, int n) {
-  if (a.residual == nullptr) return 0.f;
-  const int64_t at = static_cast<int64_t>(token) * a.ld_res + n;
-  return a.res_f32 ? static_cast<const float*>(a.residual)[at] : widen(static_cast<const uint16_t*>(a.residual)[at], a.half);
-}
-template <int ACT>
-__device__ __forceinline__ void finish1(const Args& a, int token, int n, float z, float b, float r) {
-  const float y = activate<ACT>(z + b) + r;
-  const int64_t at = static_cast<int64_t>(token) * a.ld_out + n;
-  if (a.out_f32) {
-    static_cast<float*>(a.out)[at] = y;
+// N values of any alignment: where(i) = token * stride + feature, live(i): it exists.
+template <int N, typename Where, typename Live>
+__device__ __forceinline__ void residuals1(const Args& a, Where where, Live live, float (&r)[N]) {
+  if (a.residual == nullptr) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = 0.f;
+  } else if (a.res_f32) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = live(i) ? static_cast<const float*>(a.residual)[where(i, a.ld_res)] : 0.f;
   } else {
-    static_cast<uint16_t*>(a.out)[at] = static_cast<uint16_t>(narrow(y, a.half));
+    uint16_t u[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) u[i] = live(i) ? static_cast<const uint16_t*>(a.residual)[where(i, a.ld_res)] : 0;
+    if (a.half) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) r[i] = widen<true>(u[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) r[i] = widen<false>(u[i]);
+    }
   }
+}
+// z: the sums with their bias, overwritten
+template <int ACT, int N, typename Where, typename Live>
+__device__ __forceinline__ void finish1(const Args& a, Where where, Live live, const float (&r)[N], float (&z)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) z[i] = activate<ACT>(z[i]) + r[i];
+  if (a.out_f32) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (live(i)) static_cast<float*>(a.out)[where(i, a.ld_out)] = z[i];
+  } else if (a.half) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (live(i)) static_cast<uint16_t*>(a.out)[where(i, a.ld_out)] = narrow<true>(z[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (live(i)) static_cast<uint16_t*>(a.out)[where(i, a.ld_out)] = narrow<false>(z[i]);
+  }
+}
+
+// The bias of a lane's four features of the 128 from f0: f0 + 4 lane + 0 .. 3 (whole), or f0 + lane + 32 * 0 .. 3.
+__device__ __forceinline__ float4 lane_bias(const Args& a, int f0, bool whole, int lane) {
+  if (whole) return bias4(a, f0 + 4 * lane);
+  float b[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) b[i] = f0 + lane + 32 * i < a.n ? bias1(a, f0 + lane + 32 * i) : 0.f;
+  return make_float4(b[0], b[1], b[2], b[3]);
+}
+
+// Finishes tokens j0 + warp, + WARPS, .. below j1 of a tile (token j of the tile is row t0 + j of the output) for the 128
+// features from f0 whose sums lie in shared memory as fp32 rows of ROW floats from `base` on, features from column `col`:
+// in this CTA's (splits == 1), or as partial sums at the same place of the cluster's CTAs first_rank + s * rank_step, added
+// in order of s. SWIZZLE: the 16-byte unit u of row j is at place u ^ (j % 8). Two tokens per warp at a time: a lane
+// finishes four consecutive features of each (whole: aligned vectors), or features lane, lane + 32, .. .
+template <int ACT, int WARPS, int ROW, bool SWIZZLE>
+__device__ __forceinline__ void finish_share(const Args& a, uint32_t base, int col, int rows, int t0, int j0, int j1, int f0, bool whole,
+                                             float4 b, int warp, int lane, int splits, int first_rank, int rank_step) {
+  constexpr int U = 2;
+  if (whole) {
+    const int n0 = f0 + 4 * lane;
+#pragma unroll 1
+    for (int j = j0 + warp; j < j1; j += U * WARPS) {
+      float4 r[U], z[U];
+      residuals<U>(a, t0 + j, WARPS, t0 + j1, n0, r);
+#pragma unroll
+      for (int u = 0; u < U; ++u) z[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int s = 0; s < splits; ++s) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int ju = min(j + u * WARPS, rows - 1);  // past the share: read, not written
+          const uint32_t at = base + ju * ROW * 4 + (((col >> 2) + lane) ^ (SWIZZLE ? ju & 7 : 0)) * 16;
+          const float4 p = splits > 1 ? ld_shared_cluster_f4(mapa_shared(at, first_rank + s * rank_step)) : ld_shared_f4(at);
+          z[u].x += p.x, z[u].y += p.y, z[u].z += p.z, z[u].w += p.w;
+        }
+      }
+      finish<ACT, U>(a, t0 + j, WARPS, t0 + j1, n0, b, r, z);
+    }
+  } else {
+    const float bs[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll 1
+    for (int j = j0 + warp; j < j1; j += U * WARPS) {
+      // value i: token j + (i / 4) * WARPS, feature f0 + lane + 32 (i % 4)
+      auto exists = [&](int i) { return j + (i >> 2) * WARPS < j1 && f0 + lane + 32 * (i & 3) < a.n; };
+      auto where = [&](int i, int64_t ld) {
+        return static_cast<int64_t>(t0 + j + (i >> 2) * WARPS) * ld + f0 + lane + 32 * (i & 3);
+      };
+      float r[4 * U], z[4 * U];
+      residuals1<4 * U>(a, where, exists, r);
+#pragma unroll
+      for (int i = 0; i < 4 * U; ++i) z[i] = bs[i & 3];
+#pragma unroll 2
+      for (int s = 0; s < splits; ++s) {
+#pragma unroll
+        for (int i = 0; i < 4 * U; ++i) {
+          const int ju = min(j + (i >> 2) * WARPS, rows - 1), c = col + lane + 32 * (i & 3);
+          const uint32_t at = base + ju * ROW * 4 + ((c >> 2) ^ (SWIZZLE ? ju & 7 : 0)) * 16 + (c & 3) * 4;
+          float p;
+          if (splits > 1) {
+            asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                         : "=f"(p)
+                         : "r"(mapa_shared(at, first_rank + s * rank_step))
+                         : "memory");
+          } else {
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(p) : "r"(at) : "memory");
+          }
+          z[i] += p;
+        }
+      }
+      finish1<ACT, 4 * U>(a, where, exists, r, z);
+    }
+  }
+}
+
+// A barrier of the cluster that orders no memory: enough where what was read has been used (with release semantics it
+// would also wait for the outputs to reach L2).
+__device__ __forceinline__ void cluster_sync_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 
 // Adds NC accumulator columns at `taddr` (this warp's 32 lanes) to v; the first time they are the sum.
@@ -238,15 +423,7 @@ __global__ void __launch_bounds__(Few<BT>::kThreads, 2) few_kernel(const __grid_
         asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint8_t*>(a.residual) + (a.res_f32 ? 4 : 2) * at));
     }
   }
-  float4 b;  // of features f0 + 4 lane + 0 .. 3, or f0 + lane + 32 * 0 .. 3
-  if (whole) {
-    b = bias4(a, f0 + 4 * lane);
-  } else {
-    b.x = f0 + lane < a.n ? bias1(a, f0 + lane) : 0.f;
-    b.y = f0 + lane + 32 < a.n ? bias1(a, f0 + lane + 32) : 0.f;
-    b.z = f0 + lane + 64 < a.n ? bias1(a, f0 + lane + 64) : 0.f;
-    b.w = f0 + lane + 96 < a.n ? bias1(a, f0 + lane + 96) : 0.f;
-  }
+  const float4 b = lane_bias(a, f0, whole, lane);
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
@@ -339,86 +516,10 @@ __global__ void __launch_bounds__(Few<BT>::kThreads, 2) few_kernel(const __grid_
     __syncthreads();
   }
 
-  // U tokens per warp at a time: a lane finishes four features of each.
-  constexpr int U = 2;
-  const uint32_t base = smem_u32(tile);
-  if (whole) {
-    const int n0 = f0 + 4 * lane;
-#pragma unroll 1
-    for (int j = j0 + warp; j < j1; j += U * C::kWarps) {
-      float4 r[U], z[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int ju = min(j + u * C::kWarps, BT - 1);  // past the share: read, not written
-        z[u] = *reinterpret_cast<const float4*>(tile + ju * kFeat + 4 * lane);
-        if (j + u * C::kWarps < j1) r[u] = residual4(a, t0 + j + u * C::kWarps, n0);
-      }
-      if (a.splits > 1) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) z[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int s = 0; s < a.splits; ++s) {
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            const int ju = min(j + u * C::kWarps, BT - 1);
-            const float4 p = ld_shared_cluster_f4(mapa_shared(base + (ju * kFeat + 4 * lane) * 4, s));
-            z[u].x += p.x, z[u].y += p.y, z[u].z += p.z, z[u].w += p.w;
-          }
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (j + u * C::kWarps < j1) finish4<ACT>(a, t0 + j + u * C::kWarps, n0, z[u], b, r[u]);
-    }
-  } else {
-    const float bs[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll 1
-    for (int j = j0 + warp; j < j1; j += U * C::kWarps) {
-      float r[U][4], z[U][4];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int ju = j + u * C::kWarps;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int n = f0 + lane + 32 * i;
-          r[u][i] = ju < j1 && n < a.n ? residual1(a, t0 + ju, n) : 0.f;
-          z[u][i] = 0.f;
-        }
-      }
-#pragma unroll 2
-      for (int s = 0; s < a.splits; ++s) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int ju = min(j + u * C::kWarps, BT - 1);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float p;
-            if (a.splits > 1) {
-              asm volatile("ld.shared::cluster.f32 %0, [%1];"
-                           : "=f"(p)
-                           : "r"(mapa_shared(base + (ju * kFeat + lane + 32 * i) * 4, s))
-                           : "memory");
-            } else {
-              p = tile[ju * kFeat + lane + 32 * i];
-            }
-            z[u][i] += p;
-          }
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int n = f0 + lane + 32 * i;
-          if (j + u * C::kWarps < j1 && n < a.n) finish1<ACT>(a, t0 + j + u * C::kWarps, n, z[u][i], bs[i], r[u][i]);
-        }
-    }
-  }
+  finish_share<ACT, C::kWarps, kFeat, false>(a, smem_u32(tile), 0, BT, t0, j0, j1, f0, whole, b, warp, lane, a.splits, 0, 1);
   __syncwarp();
   if (a.splits > 1) {
-    // Nobody reads this CTA's tile any more: what was read has been used, so this barrier orders no memory (with
-    // release semantics it would also wait for the outputs to reach L2).
-    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+    cluster_sync_relaxed();  // nobody reads this CTA's tile any more
   } else {
     __syncthreads();
   }
@@ -436,9 +537,16 @@ __global__ void __launch_bounds__(Few<BT>::kThreads, 2) few_kernel(const __grid_
 // Eight epilogue warps, two per TMEM lane quarter, hold the 128 sums of their half row in registers; a finished tile
 // goes through 4 KB of shared memory per warp, 32 x 32 values at a time, so that residuals and outputs are contiguous
 // accesses, while the tensor core already works on the next tile.
+//
+// SPLIT, for fewer tiles than pairs: a cluster of `splits` pairs shares one tile, each pair a run of K. The sums go to shared
+// memory (128 KB, in the place of the operand stages), and every CTA finishes an equal share of its 128 rows by adding the
+// partial sums of the CTAs that hold the same rows. (Against few_kernel's 128 x 128 tiles this halves the operand bytes that
+// an SM has to take in per product: at 512 x 3072 those bytes, not the products, set few_kernel's time.)
 namespace many {
 constexpr int kTile = 256;
+constexpr int kMaxSplits = 4;
 constexpr int kEpiWarps = 8;
+constexpr int kCols = 4 * kTile / kEpiWarps;  // sums of a thread
 // Three warpgroups: loads and MMAs (two of its warps idle), and the two of the epilogue, which take the registers that
 // the first gives back. 128 x 40 + 256 x 232 = 384 x 168, what the block is launched with.
 constexpr int kThreads = 128 + 32 * kEpiWarps;
@@ -453,6 +561,15 @@ constexpr int kPatchBytes = 32 * 32 * 4;
 constexpr int kSmemBytes = kStages * kStageBytes + kEpiWarps * kPatchBytes + 256 + 1024;
 constexpr uint32_t kTmemCols = 512;
 
+// Arrives on the barrier at shared-memory offset `bar` of both CTAs of the pair whose leader has cluster rank `lead` when
+// every MMA issued so far by this thread is complete. (It signals barriers; it loads nothing.)
+__device__ __forceinline__ void commit_pair(uint32_t bar, int lead) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"(static_cast<unsigned short>(3 << lead))
+      : "memory");
+}
+
 // Token tiles in groups of a.group, tokens fastest inside a group: the tiles that run at once share rows of both operands.
 __device__ __forceinline__ void place(const Args& a, int tile, int& mb, int& nb) {
   const int per_group = a.group * a.tiles_f;
@@ -464,7 +581,7 @@ __device__ __forceinline__ void place(const Args& a, int tile, int& mb, int& nb)
   nb = in_group / gm;
 }
 
-template <int ACT>
+template <int ACT, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant__ Args a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -480,7 +597,8 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = warp_id(), lane = lane_id();
-  const int rank = static_cast<int>(cluster_ctarank());
+  const int cta = static_cast<int>(cluster_ctarank());
+  const int rank = cta & 1, lead = cta & ~1, split = SPLIT ? cta >> 1 : 0;  // in the pair, its leader, which run of K
   const bool leader = rank == 0;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -508,9 +626,10 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
   cluster_sync_all();  // both CTAs' barriers exist before either signals the other
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
-  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
   const int tiles = a.tiles_f * a.tiles_t;
-  const int nstage = (a.num_kb + kSub - 1) / kSub;  // a K tail past the end is zero-filled by TMA
+  const int pair = SPLIT ? blockIdx.x / (2 * a.splits) : blockIdx.x >> 1, npairs = SPLIT ? tiles : gridDim.x >> 1;
+  const int stages_all = (a.num_kb + kSub - 1) / kSub;  // a K tail past the end is zero-filled by TMA
+  const int ks0 = SPLIT ? stages_all * split / a.splits : 0, ks1 = SPLIT ? stages_all * (split + 1) / a.splits : stages_all;
 
   if (warp < 4) {
     reg_dealloc<kLeanRegs>();
@@ -522,12 +641,12 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
       for (int tile = pair; ok && tile < tiles; tile += npairs) {
         int mb, nb;
         place(a, tile, mb, nb);
-        for (int ks = 0; ks < nstage; ++ks) {
+        for (int ks = ks0; ks < ks1; ++ks) {
           if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, a.status, FB_DEV_TIMEOUT_MMA)) {
             ok = false;
             break;
           }
-          const uint32_t bar = mapa_shared(smem_u32(&full[stage]), 0);
+          const uint32_t bar = mapa_shared(smem_u32(&full[stage]), lead);
           if (leader) mbar_arrive_expect_tx(&full[stage], 2 * kStageBytes);
 #pragma unroll
           for (int h = 0; h < kSub; ++h) {
@@ -552,14 +671,14 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
       for (int tile = pair; ok && tile < tiles; tile += npairs) {
-        for (int kc = 0; ok && kc < nstage; kc += kChunkStages) {
+        for (int kc = ks0; ok && kc < ks1; kc += kChunkStages) {
           if (!mbar_wait(&acc_empty[acc], acc_phase ^ 1u, abort_flag, a.status, FB_DEV_TIMEOUT_EPI)) {
             ok = false;
             break;
           }
           tc_fence_after_sync();
           const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * kTile);
-          for (int ks = kc; ks < min(kc + kChunkStages, nstage); ++ks) {
+          for (int ks = kc; ks < min(kc + kChunkStages, ks1); ++ks) {
             if (!mbar_wait(&full[stage], phase, abort_flag, a.status, FB_DEV_TIMEOUT_TMA)) {
               ok = false;
               break;
@@ -574,20 +693,25 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
                                   sdesc_kmajor_sw128(w0 + h * kBoxBytes + 32 * k), a.idesc,
                                   (ks > kc || h > 0 || k > 0) ? 1u : 0u);
             }
-            umma_commit_pair_both(smem_u32(&empty[stage]));
+            commit_pair(smem_u32(&empty[stage]), lead);
             if (++stage == kStages) {
               stage = 0;
               phase ^= 1u;
             }
           }
           if (!ok) break;
-          umma_commit_pair_both(smem_u32(&acc_full[acc]));
+          commit_pair(smem_u32(&acc_full[acc]), lead);
           acc ^= 1;
           if (acc == 0) acc_phase ^= 1u;
         }
       }
-      umma_commit_pair(mapa_shared(smem_u32(drain), 0));
+      umma_commit_pair(mapa_shared(smem_u32(drain), lead));
       mbar_wait_quiet(drain, 0, kWaitBudgetNs);
+    }
+    if constexpr (SPLIT) {
+      __syncwarp();
+      cluster_sync_all();      // the partial sums are in shared memory
+      cluster_sync_relaxed();  // and have been read
     }
   } else {
     reg_alloc<kEpiRegs>();
@@ -600,69 +724,104 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
     for (int tile = pair; ok && tile < tiles; tile += npairs) {
       int mb, nb;
       place(a, tile, mb, nb);
-      const int row0 = mb * kTile + 128 * rank + quarter * 32;
-      if (a.residual != nullptr && row0 + lane < a.m) {  // the row's 128 residuals: in L2 by the time the sums are there
-        const int n0 = nb * kTile + part * 128, line = a.res_f32 ? 32 : 64;
-        for (int n = n0; n < min(n0 + 128, a.n); n += line) {
+      const int row0 = mb * kTile + 128 * rank + quarter * 32, col0 = nb * kTile + part * kCols;
+      if (a.residual != nullptr && row0 + lane < a.m) {  // the row's residuals: in L2 by the time the sums are there
+        const int line = a.res_f32 ? 32 : 64;
+        for (int n = col0; n < min(col0 + kCols, a.n); n += line) {
           const int64_t at = static_cast<int64_t>(row0 + lane) * a.ld_res + n;
           asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint8_t*>(a.residual) + (a.res_f32 ? 4 : 2) * at));
         }
       }
-      float v[128];
-      for (int kc = 0; kc < nstage; kc += kChunkStages) {
+      uint2 b[kCols / 32];  // the bias of this lane's four features of each step below
+#pragma unroll
+      for (int c = 0; c < kCols / 32; ++c) {
+        const int n = col0 + 32 * c + 4 * (lane & 7);
+        b[c] = a.vec && a.bias != nullptr && n + 4 <= a.n
+                   ? __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.bias) + n))
+                   : make_uint2(0u, 0u);
+      }
+      float v[kCols];
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) v[j] = 0.f;  // the sum over no K at all
+      for (int kc = ks0; kc < ks1; kc += kChunkStages) {
         if (!mbar_wait(&acc_full[acc], acc_phase, abort_flag, a.status, FB_DEV_TIMEOUT_MMA)) {
           ok = false;
           break;
         }
         tc_fence_after_sync();
-        promote<128, 32>(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * kTile + part * 128, kc == 0, v);
+        promote<kCols, 32>(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * kTile + part * kCols, kc == ks0, v);
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive_remote(mapa_shared(smem_u32(&acc_empty[acc]), 0));
+        if (lane == 0) mbar_arrive_remote(mapa_shared(smem_u32(&acc_empty[acc]), lead));
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1u;
       }
+      if constexpr (SPLIT) {
+        // [128 rows][256 columns]; the tensor core has read every stage. After a wait that gave up the values do not matter.
+        float* sums = reinterpret_cast<float*>(smem);
+        const int row = quarter * 32 + lane;
+#pragma unroll
+        for (int w = 0; w < kCols / 4; ++w)
+          *reinterpret_cast<float4*>(sums + row * kTile + (((part * kCols / 4 + w) ^ (row & 7)) << 2)) =
+              make_float4(v[4 * w], v[4 * w + 1], v[4 * w + 2], v[4 * w + 3]);
+        __syncwarp();
+        cluster_sync_all();
+        const int first = mb * kTile + 128 * rank, live = max(0, min(128, a.m - first));
+        for (int f0 = nb * kTile; f0 < min((nb + 1) * kTile, a.n); f0 += 128) {
+          const bool whole = a.vec && f0 + 128 <= a.n;
+          finish_share<ACT, kEpiWarps, kTile, true>(a, smem_u32(sums), f0 - nb * kTile, 128, first, live * split / a.splits,
+                                                    live * (split + 1) / a.splits, f0, whole, lane_bias(a, f0, whole, lane),
+                                                    warp - 4, lane, a.splits, rank, 2);
+        }
+        __syncwarp();
+        cluster_sync_relaxed();
+        break;
+      }
       if (!ok) break;
+      if (row0 >= a.m) continue;
+      // 32 columns at a time through the patch: row = lane, the 16-byte unit u of a row at place u ^ (row % 8)
 #pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        const int n0 = nb * kTile + part * 128 + 32 * c;
-        if (n0 < a.n && row0 < a.m) {
-          // the patch: row = lane, the 16-byte unit u of a row at place u ^ (row % 8)
-          __syncwarp();
+      for (int c = 0; c < kCols / 32; ++c) {
+        const int n0 = col0 + 32 * c;
+        if (n0 >= a.n) break;
+        const bool whole = a.vec && n0 + 32 <= a.n;  // every lane's four consecutive features are aligned vectors
+        // eight lanes per row, four features each
+        const int u = lane & 7, first = lane >> 3, n = n0 + 4 * u;
+        float4 r[8];
+        if (whole) residuals<8>(a, row0 + first, 4, a.m, n, r);
+        __syncwarp();
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if (c == k) {
+        for (int k = 0; k < kCols / 32; ++k) {
+          if (c == k) {
 #pragma unroll
-              for (int u = 0; u < 8; ++u)
-                *reinterpret_cast<float4*>(patch + lane * 128 + ((u ^ (lane & 7)) << 4)) =
-                    make_float4(v[32 * k + 4 * u], v[32 * k + 4 * u + 1], v[32 * k + 4 * u + 2], v[32 * k + 4 * u + 3]);
-            }
+            for (int w = 0; w < 8; ++w)
+              *reinterpret_cast<float4*>(patch + lane * 128 + ((w ^ (lane & 7)) << 4)) =
+                  make_float4(v[32 * k + 4 * w], v[32 * k + 4 * w + 1], v[32 * k + 4 * w + 2], v[32 * k + 4 * w + 3]);
           }
-          __syncwarp();
-          if (a.vec && n0 + 32 <= a.n) {
-            const int u = lane & 7, n = n0 + 4 * u;
-            const float4 b = bias4(a, n);
-            float4 r[8];
+        }
+        __syncwarp();
+        if (whole) {
+          float4 z[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int row = 4 * i + (lane >> 3);
-              if (row0 + row < a.m) r[i] = residual4(a, row0 + row, n);
-            }
+          for (int i = 0; i < 8; ++i) {
+            const int row = first + 4 * i;
+            z[i] = *reinterpret_cast<const float4*>(patch + row * 128 + ((u ^ (row & 7)) << 4));
+          }
+          const uint2 bc = c == 0 ? b[0] : c == 1 ? b[1] : c == 2 ? b[2] : b[3];
+          finish<ACT, 8>(a, row0 + first, 4, a.m, n, a.half ? widen4<true>(bc) : widen4<false>(bc), r, z);
+        } else {
+          const int n1 = n0 + lane;
+          const float b1 = n1 < a.n ? bias1(a, n1) : 0.f;
+#pragma unroll 1
+          for (int h = 0; h < 32; h += 8) {
+            auto is = [&](int i) { return row0 + h + i < a.m && n1 < a.n; };
+            auto where = [&](int i, int64_t ld) { return static_cast<int64_t>(row0 + h + i) * ld + n1; };
+            float r1[8], z1[8];
+            residuals1<8>(a, where, is, r1);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int row = 4 * i + (lane >> 3);
-              const float4 z = *reinterpret_cast<const float4*>(patch + row * 128 + ((u ^ (row & 7)) << 4));
-              if (row0 + row < a.m) finish4<ACT>(a, row0 + row, n, z, b, r[i]);
-            }
-          } else {
-            const int n = n0 + lane;
-            const float b = n < a.n ? bias1(a, n) : 0.f;
-            const int rows = n < a.n ? min(32, a.m - row0) : 0;
-#pragma unroll 4
-            for (int row = 0; row < rows; ++row) {
-              const float z = *reinterpret_cast<const float*>(patch + row * 128 + (((lane >> 2) ^ (row & 7)) << 4) + 4 * (lane & 3));
-              finish1<ACT>(a, row0 + row, n, z, b, residual1(a, row0 + row, n));
-            }
+            for (int i = 0; i < 8; ++i)
+              z1[i] = *reinterpret_cast<const float*>(patch + (h + i) * 128 + (((lane >> 2) ^ ((h + i) & 7)) << 4) + 4 * (lane & 3)) + b1;
+            finish1<ACT, 8>(a, where, is, r1, z1);
           }
         }
       }
@@ -746,6 +905,10 @@ static int encode_rows(CUtensorMap* map, const void* base, int64_t rows, int64_t
   return FB_OK;
 }
 
+// Clusters of 2 s CTAs of many_kernel that run at once (a cluster stays inside one group of SMs, so fewer than the SMs
+// alone would hold); asked of the driver once, in linear_act_setup.
+static std::atomic<int> g_clusters[many::kMaxSplits + 1];
+
 static int64_t up8(int64_t k) { return (k + 7) / 8 * 8; }
 // A matrix's row stride as TMA sees it: a single row has none, so any will do.
 static int64_t row_stride(int64_t ld, int rows, int k) { return rows == 1 ? up8(k) : ld; }
@@ -769,9 +932,26 @@ std::string linear_act_setup() {
       raise(few_kernel<32, ACT>, Few<32>::kSmemBytes);
       raise(few_kernel<64, ACT>, Few<64>::kSmemBytes);
       raise(few_kernel<128, ACT>, Few<128>::kSmemBytes);
-      raise(many::many_kernel<ACT>, many::kSmemBytes);
+      raise(many::many_kernel<ACT, false>, many::kSmemBytes);
+      raise(many::many_kernel<ACT, true>, many::kSmemBytes);
       return cudaSuccess;
     });
+  }
+  for (int s = 2; e == cudaSuccess && s <= many::kMaxSplits; ++s) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * s * 74, 1, 1);
+    cfg.blockDim = dim3(many::kThreads, 1, 1);
+    cfg.dynamicSmemBytes = many::kSmemBytes;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2 * s;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    e = cudaOccupancyMaxActiveClusters(&n, many::many_kernel<FB_ACT_NONE, true>, &cfg);
+    g_clusters[s].store(n, std::memory_order_relaxed);
   }
   return e == cudaSuccess ? std::string() : std::string("cudaFuncSetAttribute(linear_act): ") + cudaGetErrorString(e);
 }
@@ -816,12 +996,12 @@ int launch_linear_act(const fb_linear_act_args& p, cudaStream_t st, std::string&
   const bool half = p.dtype == FB_F16;
   a.num_kb = (p.k + BK - 1) / BK;
   const int64_t tiles_many = ((p.m + 255ll) / 256) * ((p.n + 255ll) / 256);
-  const int64_t tiles_few = ((p.m + 127ll) / 128) * ((p.n + 127ll) / 128);
-  // many_kernel where 256 x 256 tiles keep the pairs busy.
-  static const int force = getenv("LACT") ? atoi(getenv("LACT")) : 0;
-  const bool many_rows = force ? force == 2 : p.m > 128 && tiles_many >= 37;
+  // many_kernel's larger tiles pay once there is work for them; below, few_kernel is done sooner (no second CTA to meet, a
+  // smaller tile to fill and write). Measured, few against many, each call with a cold L2: 256 x 3072 x 3072 (m x k x n)
+  // 14.7 / 16.6 us, 2048 x 1024 x 1024 12.4 / 14.5, 1024 x 1024 x 4096 14.5 / 14.5, 1024 x 3072 x 3072 26.8 / 24.8,
+  // 8192 x 1024 x 1024 26.8 / 20.7, 4608 x 3072 x 3072 82 / 60; up to 128 rows few_kernel's one token tile is never worse.
+  const bool many_rows = p.m > 128 && static_cast<double>(p.m) * p.n * p.k >= 4294967296.0;
   const int bt = many_rows ? 128 : p.m <= 16 ? 16 : p.m <= 32 ? 32 : p.m <= 64 ? 64 : 128;
-  (void)tiles_few;
   if (p.k > 0) {
     const void *x = p.x, *w = p.w;
     int64_t ldx = row_stride(p.ldx, p.m, p.k), ldw = row_stride(p.ldw, p.n, p.k);
@@ -870,18 +1050,31 @@ int launch_linear_act(const fb_linear_act_args& p, cudaStream_t st, std::string&
     a.tiles_t = (p.m + 255) / 256;
     if (tiles_many > (1ll << 30)) return bad(FB_ERR_UNSUPPORTED, "too many output tiles");
     a.group = a.tiles_f <= 16 ? 4 : 16;
-    const int pairs = static_cast<int>(std::min<int64_t>(tiles_many, dev->sm_count / 2));
+    const int pairs = dev->sm_count / 2;
+    // Pairs that share a tile, as long as each gets two stages of K and the clusters all run at once.
+    a.splits = 1;
+    for (int s = 2; s <= many::kMaxSplits; ++s)
+      if (tiles_many <= g_clusters[s].load(std::memory_order_relaxed) && a.num_kb >= 4 * s) a.splits = s;
     e = with_act(p.act, [&](auto c) {
-      return launch(many::many_kernel<decltype(c)::value>, a, 2 * pairs, 2, many::kThreads, many::kSmemBytes, st);
+      constexpr int ACT = decltype(c)::value;
+      if (a.splits > 1)
+        return launch(many::many_kernel<ACT, true>, a, static_cast<int>(2 * a.splits * tiles_many), 2 * a.splits, many::kThreads,
+                      many::kSmemBytes, st);
+      return launch(many::many_kernel<ACT, false>, a, static_cast<int>(2 * std::min<int64_t>(tiles_many, pairs)), 2, many::kThreads,
+                    many::kSmemBytes, st);
     });
   } else {
     a.tiles_f = (p.n + kFeat - 1) / kFeat;
     a.tiles_t = (p.m + bt - 1) / bt;
     const int64_t tiles = static_cast<int64_t>(a.tiles_f) * a.tiles_t;
     if (tiles > (1ll << 27)) return bad(FB_ERR_UNSUPPORTED, "too many output tiles");
-    // Split K over a cluster until every SM has a CTA, as long as each gets four K blocks.
+    // Split K over a cluster, at most two CTAs per SM and four K blocks at least per CTA, so that the busiest SM has the
+    // least to do: 24 tiles take six CTAs each (144 SMs busy), 96 tiles three (two per SM instead of 96 SMs with one).
     a.splits = 1;
-    while (a.splits < 8 && tiles * (a.splits + 1) <= kNumSms && a.num_kb >= 4 * (a.splits + 1)) ++a.splits;
+    for (int s = 2; s <= 8 && tiles * s <= 2 * kNumSms && a.num_kb >= 4 * s; ++s) {
+      const int64_t now = (tiles * a.splits + kNumSms - 1) / kNumSms, then = (tiles * s + kNumSms - 1) / kNumSms;
+      if (then * a.splits < now * s) a.splits = s;
+    }
     const int ctas = static_cast<int>(tiles * a.splits);
     e = with_act(p.act, [&](auto c) { return go_few<decltype(c)::value>(a, bt, ctas, st); });
   }

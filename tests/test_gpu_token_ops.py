@@ -530,9 +530,10 @@ def test_linear_strides():
     assert torch.equal(ops().linear_act(x1, w, b), ops().linear_act(x1[None], w, b)[0])
 
 
-def test_linear_no_depth_is_bias_and_residual():
-    b, r = torch.linspace(-2, 2, 50, device=DEV).to(BF16), torch.ones(3, 50, device=DEV)
-    got = ops().linear_act(torch.empty(3, 0, dtype=BF16, device=DEV), torch.empty(50, 0, dtype=BF16, device=DEV), b, "relu", r, out_dtype=F32)
+@pytest.mark.parametrize("m,n", [(3, 50), (200, 50), (700, 4000)])
+def test_linear_no_depth_is_bias_and_residual(m, n):
+    b, r = torch.linspace(-2, 2, n, device=DEV).to(BF16), torch.ones(m, n, device=DEV)
+    got = ops().linear_act(torch.empty(m, 0, dtype=BF16, device=DEV), torch.empty(n, 0, dtype=BF16, device=DEV), b, "relu", r, out_dtype=F32)
     assert torch.equal(got, b.float().clamp_min(0) + r)
 
 

@@ -288,12 +288,15 @@ __device__ __forceinline__ float2 group_sum2(float a, float b, int group, float2
   return r;
 }
 
-// Threads of a block, and blocks per SM that a kernel is compiled for (registers) and its grid and shared memory are
-// sized for. Forward: blocks of 256 threads, as many as their registers allow. Backward: one block per SM, so that the
+// Threads of a block (whole groups of GT), and blocks per SM that a kernel is compiled for (registers) and its grid and
+// shared memory are sized for. Forward: blocks of 256 threads, as many as their registers allow. Backward: one block per SM, so that the
 // groups' column sums are joined in shared memory and one partial row per SM goes to memory.
 constexpr int fwd_threads(int gt) { return gt < 256 ? 256 : gt; }
 constexpr int fwd_blocks(int gt, int e) { return gt >= 512 ? (gt == 512 ? 2 : 1) : e <= 4 ? 4 : e <= 12 ? 3 : 2; }
-constexpr int bwd_threads(int gt, int e) { return gt >= 512 ? gt : e <= 4 ? 1024 : e <= 12 ? 768 : 512; }
+constexpr int bwd_threads(int gt, int e) {
+  const int most = e <= 4 ? 1024 : e <= 12 ? 768 : e <= 20 ? 512 : e <= 28 ? 384 : 256;
+  return most < gt ? gt : most / gt * gt;  // whole groups: their barriers count on it
+}
 
 // One row of up to GT * NCH * CH elements per group of GT threads at a time; a group walks over rows
 // blockIdx.x * NG + group, + gridDim.x * NG, ... of sum group blockIdx.y, the next `depth` rows on their way to shared
@@ -301,6 +304,7 @@ constexpr int bwd_threads(int gt, int e) { return gt >= 512 ? gt : e <= 4 ? 1024
 template <int GT, int NCH, int CH, bool FULL, int THREADS>
 struct Walk {
   static constexpr int T = THREADS, NG = T / GT, E = NCH * CH, P = E / 2;
+  static_assert(T % GT == 0 && T <= 1024 && (GT == 32 || NG <= 15), "whole groups, a barrier of its own for each");
   // Pair k of a thread's elements lies in the chunks of columns 2k .. 2k + 1; both are inside the row or both past its
   // end for chunks of four, each by itself for single elements.
   static __device__ __forceinline__ int column(int t, int e) { return CH * (t + GT * (e / CH)) + e % CH; }
@@ -693,9 +697,9 @@ static int size_of(int t) { return t == FB_F32 ? 4 : 2; }
 // The group of threads for a row of `dim` elements, and the chunks a thread holds: at most 5 chunks of 4 (vectors), or
 // 16 single elements. Fewer threads per row mean fewer barriers and more rows at once; more elements per thread than
 // 20 no longer leave registers for two blocks per SM in the backward pass.
-static int group_threads(int dim, bool vec) {
+static int group_threads(int dim, bool vec, bool bwd) {
   int gt = 32;
-  while (gt * (vec ? 20 : 16) < dim && gt < 1024) gt *= 2;
+  while (gt * (vec ? (bwd && dim <= 10240 ? 40 : 20) : 16) < dim && gt < 1024) gt *= 2;
   return gt;
 }
 static int elements(int dim, int gt, bool vec) { return vec ? 4 * ((dim + 4 * gt - 1) / (4 * gt)) : 16; }
@@ -703,7 +707,7 @@ static int elements(int dim, int gt, bool vec) { return vec ? 4 * ((dim + 4 * gt
 // Blocks per sum group of the backward pass: the SMs shared out over the groups, fewer where there are fewer rows than
 // groups of threads.
 static int64_t bwd_blocks(int64_t rows, int dim, int64_t sum_groups, bool vec) {
-  const int gt = group_threads(dim, vec), ng = bwd_threads(gt, elements(dim, gt, vec)) / gt;
+  const int gt = group_threads(dim, vec, true), ng = bwd_threads(gt, elements(dim, gt, vec)) / gt;
   const int64_t need = std::max<int64_t>(1, (rows + ng - 1) / ng);
   return std::max<int64_t>(1, std::min<int64_t>(need, kNumSms / std::max<int64_t>(1, sum_groups)));
 }
@@ -711,29 +715,34 @@ static int64_t bwd_blocks(int64_t rows, int dim, int64_t sum_groups, bool vec) {
 constexpr int kRingPerSm = 208 * 1024;  // shared memory of an SM that the rows on their way (and w) may take
 
 template <int GT, int NCH, int CH, bool FULL>
-static cudaError_t go(Args a, bool bwd, int64_t sum_groups, cudaStream_t st) {
-  constexpr int TF = fwd_threads(GT), TB = bwd_threads(GT, NCH * CH), E = NCH * CH;
-  const int T = bwd ? TB : TF, per_sm = bwd ? 1 : fwd_blocks(GT, E);
-  const int w_bytes = bwd ? E * T * 4 : 0;
+static cudaError_t go_fwd(Args a, cudaStream_t st) {
+  constexpr int T = fwd_threads(GT), NG = T / GT, per_sm = fwd_blocks(GT, NCH * CH);
   int smem = 0;
   if (CH == 4) {
-    const int xb = size_of(a.x_type), yb = size_of(a.y_type);
-    const int two = 4 * NCH * T * (bwd ? xb + yb : xb), three = two + 4 * NCH * T * xb;
-    a.add_staged = bwd && a.add && three + w_bytes <= kRingPerSm / per_sm;
-    a.stage_bytes = a.add_staged ? three : two;
-    a.depth = std::max(1, std::min(4, (kRingPerSm / per_sm - w_bytes) / a.stage_bytes));
+    a.stage_bytes = 4 * NCH * T * size_of(a.x_type);
+    a.depth = std::max(1, std::min(4, kRingPerSm / per_sm / a.stage_bytes));
     smem = a.depth * a.stage_bytes;
   }
-  smem += w_bytes;  // after the walk, the groups' sums take this much too
-  if (!bwd) {
-    constexpr int NG = TF / GT;
-    const int64_t need = (static_cast<int64_t>(a.rows) + NG - 1) / NG;
-    fwd_kernel<GT, NCH, CH, FULL><<<static_cast<unsigned>(std::min<int64_t>(need, per_sm * kNumSms)), TF, smem, st>>>(a);
-    return cudaGetLastError();
+  const int64_t need = (static_cast<int64_t>(a.rows) + NG - 1) / NG;
+  fwd_kernel<GT, NCH, CH, FULL><<<static_cast<unsigned>(std::min<int64_t>(need, per_sm * kNumSms)), T, smem, st>>>(a);
+  return cudaGetLastError();
+}
+
+template <int GT, int NCH, int CH, bool FULL>
+static cudaError_t go_bwd(Args a, int64_t sum_groups, cudaStream_t st) {
+  constexpr int T = bwd_threads(GT, NCH * CH), w_bytes = NCH * CH * T * 4;
+  int smem = w_bytes;  // after the walk, the groups' sums take this much too
+  if (CH == 4) {
+    const int xb = size_of(a.x_type), yb = size_of(a.y_type);
+    const int two = 4 * NCH * T * (xb + yb), three = two + 4 * NCH * T * xb;
+    a.add_staged = a.add && three + w_bytes <= kRingPerSm;
+    a.stage_bytes = a.add_staged ? three : two;
+    a.depth = std::max(1, std::min(4, (kRingPerSm - w_bytes) / a.stage_bytes));
+    smem += a.depth * a.stage_bytes;
   }
   const int64_t blocks = bwd_blocks(a.rows, a.dim, sum_groups, CH == 4);
   const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(sum_groups));
-  bwd_kernel<GT, NCH, CH, FULL><<<grid, TB, smem, st>>>(a);
+  bwd_kernel<GT, NCH, CH, FULL><<<grid, T, smem, st>>>(a);
   cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess && a.dw != nullptr && blocks > 1) {
     // launched while the last blocks of the walk still run; it waits for them before it reads
@@ -751,23 +760,38 @@ static cudaError_t go(Args a, bool bwd, int64_t sum_groups, cudaStream_t st) {
   return e;
 }
 
-// Raises the shared-memory limits of one instance (ring of up to kRingPerSm bytes).
-template <int GT, int NCH, int CH, bool FULL>
-static cudaError_t setup_one() {
-  const cudaError_t e = cudaFuncSetAttribute(fwd_kernel<GT, NCH, CH, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingPerSm);
-  return e != cudaSuccess ? e : cudaFuncSetAttribute(bwd_kernel<GT, NCH, CH, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingPerSm);
+// f(GT, NCH, CH) as integral constants for a row of `dim` elements: every instance there is, and the only ones.
+template <int N>
+using Int = std::integral_constant<int, N>;
+template <int GT, int FROM, int TO, typename F>
+static cudaError_t with_chunks(int chunks, F f) {
+  if constexpr (FROM < TO) {
+    if (chunks > FROM) return with_chunks<GT, FROM + 1, TO>(chunks, f);
+  }
+  return f(Int<GT>(), Int<FROM>(), Int<4>());
 }
-
-template <int GT, typename F>
-static cudaError_t with_chunks(int dim, bool vec, F f) {
-  if (!vec) return f(std::integral_constant<int, 16>(), std::integral_constant<int, 1>());
-  using Four = std::integral_constant<int, 4>;
-  switch ((dim + 4 * GT - 1) / (4 * GT)) {
-    case 1: return f(std::integral_constant<int, 1>(), Four());
-    case 2: return f(std::integral_constant<int, 2>(), Four());
-    case 3: return f(std::integral_constant<int, 3>(), Four());
-    case 4: return f(std::integral_constant<int, 4>(), Four());
-    default: return f(std::integral_constant<int, GT < 1024 ? 5 : 4>(), Four());  // 1024 threads hold kMaxDimRegs in 4
+template <typename F>
+static cudaError_t with_fwd(int dim, bool vec, F f) {
+  const int gt = group_threads(dim, vec, false), chunks = (dim + 4 * gt - 1) / (4 * gt);
+  switch (gt) {
+    case 32: return vec ? with_chunks<32, 1, 5>(chunks, f) : f(Int<32>(), Int<16>(), Int<1>());
+    case 64: return vec ? with_chunks<64, 3, 5>(chunks, f) : f(Int<64>(), Int<16>(), Int<1>());
+    case 128: return vec ? with_chunks<128, 3, 5>(chunks, f) : f(Int<128>(), Int<16>(), Int<1>());
+    case 256: return vec ? with_chunks<256, 3, 5>(chunks, f) : f(Int<256>(), Int<16>(), Int<1>());
+    case 512: return vec ? with_chunks<512, 3, 5>(chunks, f) : f(Int<512>(), Int<16>(), Int<1>());
+    default: return vec ? with_chunks<1024, 3, 4>(chunks, f) : f(Int<1024>(), Int<16>(), Int<1>());
+  }
+}
+template <typename F>
+static cudaError_t with_bwd(int dim, bool vec, F f) {
+  const int gt = group_threads(dim, vec, true), chunks = (dim + 4 * gt - 1) / (4 * gt);
+  switch (gt) {
+    case 32: return vec ? with_chunks<32, 1, 10>(chunks, f) : f(Int<32>(), Int<16>(), Int<1>());
+    case 64: return vec ? with_chunks<64, 6, 10>(chunks, f) : f(Int<64>(), Int<16>(), Int<1>());
+    case 128: return vec ? with_chunks<128, 6, 10>(chunks, f) : f(Int<128>(), Int<16>(), Int<1>());
+    case 256: return vec ? with_chunks<256, 6, 10>(chunks, f) : f(Int<256>(), Int<16>(), Int<1>());
+    case 512: return f(Int<512>(), Int<16>(), Int<1>());
+    default: return vec ? with_chunks<1024, 3, 4>(chunks, f) : f(Int<1024>(), Int<16>(), Int<1>());
   }
 }
 
@@ -785,37 +809,46 @@ static cudaError_t dispatch(const Args& a, bool bwd, int64_t sum_groups, bool ve
     }
     return e;
   }
-  auto run = [&](auto gt) {
-    constexpr int GT = decltype(gt)::value;
-    return with_chunks<GT>(a.dim, vec, [&](auto nch, auto ch) {
-      constexpr int NCH = decltype(nch)::value, CH = decltype(ch)::value;
-      if (CH == 4 && a.dim == 4 * GT * NCH) return go<GT, NCH, CH, CH == 4>(a, bwd, sum_groups, st);
-      return go<GT, NCH, CH, false>(a, bwd, sum_groups, st);
-    });
+  auto run = [&](auto gt, auto nch, auto ch) {
+    constexpr int GT = decltype(gt)::value, NCH = decltype(nch)::value, CH = decltype(ch)::value;
+    if constexpr (CH == 4) {
+      if (a.dim == 4 * GT * NCH) return go_fwd<GT, NCH, CH, true>(a, st);
+    }
+    return go_fwd<GT, NCH, CH, false>(a, st);
   };
-  switch (group_threads(a.dim, vec)) {
-    case 32: return run(std::integral_constant<int, 32>());
-    case 64: return run(std::integral_constant<int, 64>());
-    case 128: return run(std::integral_constant<int, 128>());
-    case 256: return run(std::integral_constant<int, 256>());
-    case 512: return run(std::integral_constant<int, 512>());
-    default: return run(std::integral_constant<int, 1024>());
-  }
+  auto back = [&](auto gt, auto nch, auto ch) {
+    constexpr int GT = decltype(gt)::value, NCH = decltype(nch)::value, CH = decltype(ch)::value;
+    if constexpr (CH == 4) {
+      if (a.dim == 4 * GT * NCH) return go_bwd<GT, NCH, CH, true>(a, sum_groups, st);
+    }
+    return go_bwd<GT, NCH, CH, false>(a, sum_groups, st);
+  };
+  return bwd ? with_bwd(a.dim, vec, back) : with_fwd(a.dim, vec, run);
 }
 
-template <int GT, int NCH>
-static cudaError_t setup_both() {
-  const cudaError_t e = setup_one<GT, NCH, 4, false>();
-  return e != cudaSuccess ? e : setup_one<GT, NCH, 4, true>();
-}
-template <int GT>
-static cudaError_t setup_gt() {
-  cudaError_t e = setup_one<GT, 16, 1, false>();
-  if (e == cudaSuccess) e = setup_both<GT, 1>();
-  if (e == cudaSuccess) e = setup_both<GT, 2>();
-  if (e == cudaSuccess) e = setup_both<GT, 3>();
-  if (e == cudaSuccess) e = setup_both<GT, 4>();
-  if constexpr (GT < 1024) e = e == cudaSuccess ? setup_both<GT, 5>() : e;
+// Raises the shared-memory limits of every instance (ring of up to kRingPerSm bytes).
+static cudaError_t setup() {
+  cudaError_t e = cudaSuccess;
+  auto raise = [&](auto kernel) {
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingPerSm);
+  };
+  auto fwd = [&](auto gt, auto nch, auto ch) {
+    constexpr int GT = decltype(gt)::value, NCH = decltype(nch)::value, CH = decltype(ch)::value;
+    raise(fwd_kernel<GT, NCH, CH, false>);
+    if constexpr (CH == 4) raise(fwd_kernel<GT, NCH, CH, true>);
+    return e;
+  };
+  auto bwd = [&](auto gt, auto nch, auto ch) {
+    constexpr int GT = decltype(gt)::value, NCH = decltype(nch)::value, CH = decltype(ch)::value;
+    raise(bwd_kernel<GT, NCH, CH, false>);
+    if constexpr (CH == 4) raise(bwd_kernel<GT, NCH, CH, true>);
+    return e;
+  };
+  for (int vec = 0; vec < 2; ++vec)
+    for (int dim = 32 * 4; dim <= kMaxDimRegs; dim += 32 * 4) {
+      with_fwd(dim, vec, fwd);
+      with_bwd(dim, vec, bwd);
+    }
   return e;
 }
 
@@ -832,12 +865,7 @@ static bool misaligned(const void* p, int type) { return reinterpret_cast<uintpt
 }  // namespace norm
 
 std::string layer_norm_setup() {
-  cudaError_t e = norm::setup_gt<32>();
-  if (e == cudaSuccess) e = norm::setup_gt<64>();
-  if (e == cudaSuccess) e = norm::setup_gt<128>();
-  if (e == cudaSuccess) e = norm::setup_gt<256>();
-  if (e == cudaSuccess) e = norm::setup_gt<512>();
-  if (e == cudaSuccess) e = norm::setup_gt<1024>();
+  const cudaError_t e = norm::setup();
   return e == cudaSuccess ? std::string() : std::string("cudaFuncSetAttribute(layer_norm): ") + cudaGetErrorString(e);
 }
 

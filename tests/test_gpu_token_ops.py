@@ -235,8 +235,9 @@ def check_norm(got, x, w, b, eps):
     check(got, ref, dh * wf.abs() + 3 * U * ((h * wf).abs() + bf.abs()), f"norm {tuple(x.shape)}")
 
 
-DIMS = [1, 2, 3, 8, 31, 32, 33, 100, 127, 128, 129, 511, 512, 513, 768, 1000, 1024, 1025, 1280, 2047, 3072, 4096, 4100, 8191,
-        8192, 12288, 16384, 16385, 20004]
+DIMS = [1, 2, 3, 8, 31, 32, 33, 100, 127, 128, 129, 256, 384, 511, 512, 513, 640, 768, 896, 1000, 1024, 1025, 1152, 1280, 1536, 1792,
+        2047, 2048, 2304, 2560, 3072, 3584, 4096, 4100, 4608, 5120, 6144, 7168,
+        8191, 8192, 10240, 12288, 16384, 16385, 20004]
 
 
 @pytest.mark.parametrize("dim", DIMS)

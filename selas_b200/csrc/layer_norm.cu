@@ -71,6 +71,8 @@ __device__ __forceinline__ float total(f2 v) {
 }
 
 // Where a group is in its walk over rows: row = outer * inner + index, advanced by a fixed step without divisions.
+// Groups smaller than a warp take consecutive rows and walk on as long as the first group of their warp has a row, since
+// they shuffle together; a group past the last row works on zeros and writes nothing.
 struct Place {
   int row, o, i;
 };
@@ -174,7 +176,7 @@ __device__ __forceinline__ void load_row(const void* p, int type, int64_t base, 
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
       const int col = CH * (t + GT * c);
-      if (FULL || col < dim) {
+      if ((FULL && GT >= 32) || col < dim) {  // small groups: dim is 0 for one without a row
         load_chunk<CH>(p, ty, base + col, f + CH * c);
       } else {
 #pragma unroll
@@ -236,7 +238,7 @@ __device__ __forceinline__ void take_row(const uint8_t* src, int type, int t, in
   auto each = [&](int ty, int bytes) {
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-      if (FULL || 4 * (t + GT * c) < dim) {
+      if ((FULL && GT >= 32) || 4 * (t + GT * c) < dim) {
         widen4(src + c * T * bytes, ty, f + 4 * c);
       } else {
         f[4 * c] = f[4 * c + 1] = f[4 * c + 2] = f[4 * c + 3] = 0.f;
@@ -266,16 +268,18 @@ __device__ __forceinline__ void wait_fetch(int newer) {
   }
 }
 
-// Sums of two values over a group of GT threads (all of them get both). One warp: shuffles. More: one entry per warp
-// in shared memory and a barrier of the group's own; `buf` alternates between calls, so one barrier per sum is enough.
+// Sums of two values over a group of GT threads (all of them get both). Up to a warp: shuffles, the whole warp together.
+// More: one entry per warp in shared memory and a barrier of the group's own; `buf` alternates between calls, so one
+// barrier per sum is enough.
 template <int GT>
 __device__ __forceinline__ float2 group_sum2(float a, float b, int group, float2* slots, int& buf) {
-  // the lower half of the warp adds up a, the upper half b
-  const bool upper = threadIdx.x & 16;
-  float v = (upper ? b : a) + __shfl_xor_sync(0xffffffffu, upper ? a : b, 16);
+  // the lower half of the group's lanes adds up a, the upper half b
+  constexpr int L = GT < 32 ? GT : 32;
+  const bool upper = threadIdx.x & (L / 2);
+  float v = (upper ? b : a) + __shfl_xor_sync(0xffffffffu, upper ? a : b, L / 2);
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if constexpr (GT == 32) return make_float2(__shfl_sync(0xffffffffu, v, 0), __shfl_sync(0xffffffffu, v, 16));
+  for (int o = L / 4; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if constexpr (GT <= 32) return make_float2(__shfl_sync(0xffffffffu, v, 0, L), __shfl_sync(0xffffffffu, v, L / 2, L));
   constexpr int W = GT / 32;
   float2* s = slots + (buf * (blockDim.x / GT) + group) * W;
   buf ^= 1;
@@ -294,17 +298,23 @@ __device__ __forceinline__ float2 group_sum2(float a, float b, int group, float2
 constexpr int fwd_threads(int gt) { return gt < 256 ? 256 : gt; }
 constexpr int fwd_blocks(int gt, int e) { return gt >= 512 ? (gt == 512 ? 2 : 1) : e <= 4 ? 4 : e <= 12 ? 3 : 2; }
 constexpr int bwd_threads(int gt, int e) {
-  const int most = e <= 4 ? 1024 : e <= 12 ? 768 : e <= 20 ? 512 : e <= 28 ? 384 : 256;
+  const int most = e <= 4 ? 1024 : e <= 8 ? 768 : e <= 16 ? 512 : e <= 24 ? 384 : 256;
   return most < gt ? gt : most / gt * gt;  // whole groups: their barriers count on it
 }
 
 // One row of up to GT * NCH * CH elements per group of GT threads at a time; a group walks over rows
 // blockIdx.x * NG + group, + gridDim.x * NG, ... of sum group blockIdx.y, the next `depth` rows on their way to shared
 // memory while it works on one (CH == 4; the rows of odd sizes and alignments, CH == 1, are loaded where they are used).
+// How many rows ahead of its warp's first group a group is.
+template <int GT>
+__device__ __forceinline__ int ahead_of_warp() {
+  return GT < 32 ? static_cast<int>(threadIdx.x % 32) / GT : 0;
+}
+
 template <int GT, int NCH, int CH, bool FULL, int THREADS>
 struct Walk {
   static constexpr int T = THREADS, NG = T / GT, E = NCH * CH, P = E / 2;
-  static_assert(T % GT == 0 && T <= 1024 && (GT == 32 || NG <= 15), "whole groups, a barrier of its own for each");
+  static_assert(T % GT == 0 && T <= 1024 && (GT <= 32 || NG <= 15), "whole groups, a barrier of its own for each");
   // Pair k of a thread's elements lies in the chunks of columns 2k .. 2k + 1; both are inside the row or both past its
   // end for chunks of four, each by itself for single elements.
   static __device__ __forceinline__ int column(int t, int e) { return CH * (t + GT * (e / CH)) + e % CH; }
@@ -367,7 +377,7 @@ __global__ void __launch_bounds__(fwd_threads(GT), fwd_blocks(GT, NCH* CH)) fwd_
   using W = Walk<GT, NCH, CH, FULL, fwd_threads(GT)>;
   constexpr int P = W::P, T = W::T, NG = W::NG;
   extern __shared__ __align__(16) uint8_t ring[];
-  __shared__ float2 slots[2 * NG * (GT / 32)];
+  __shared__ float2 slots[GT > 32 ? 2 * NG * (GT / 32) : 1];
   const int group = threadIdx.x / GT, t = threadIdx.x % GT;
   const int rows_step = gridDim.x * NG;
   const Step step = {rows_step, rows_step / a.inner, rows_step % a.inner};
@@ -387,8 +397,9 @@ __global__ void __launch_bounds__(fwd_threads(GT), fwd_blocks(GT, NCH* CH)) fwd_
   f2 w[P], b[P];
   int have = -1;  // the outer index whose w and b are in registers
   int buf = 0, stage = 0;
-  for (; at.row < a.rows; advance(at, step, a.inner)) {
-    if (have < 0 || (a.w_stride != 0 && have != at.o)) {
+  for (; at.row - ahead_of_warp<GT>() < a.rows; advance(at, step, a.inner)) {
+    const bool live = GT >= 32 || at.row < a.rows;
+    if (live && (have < 0 || (a.w_stride != 0 && have != at.o))) {
       have = at.o;
       W::weight(a, at.o, t, w);
       if (a.b != nullptr) {
@@ -401,9 +412,9 @@ __global__ void __launch_bounds__(fwd_threads(GT), fwd_blocks(GT, NCH* CH)) fwd_
     f2 x[P];
     if constexpr (CH == 4) {
       wait_fetch(a.depth - 1);
-      W::take(mine + stage * a.stage_bytes, a.x_type, t, a.dim, x);
+      W::take(mine + stage * a.stage_bytes, a.x_type, t, live ? a.dim : 0, x);
     } else {
-      W::load(a.x, a.x_type, at.o * a.xo + at.i * a.xi, t, a.dim, x);
+      W::load(a.x, a.x_type, at.o * a.xo + at.i * a.xi, t, live ? a.dim : 0, x);
     }
     f2 s = pack2(0.f, 0.f);
 #pragma unroll
@@ -423,7 +434,7 @@ __global__ void __launch_bounds__(fwd_threads(GT), fwd_blocks(GT, NCH* CH)) fwd_
     const f2 r = pack2(rstd, rstd);
 #pragma unroll
     for (int k = 0; k < P; ++k) x[k] = fma2(mul2(x[k], r), w[k], b[k]);
-    W::store(a.out, a.y_type, at.o * a.oo + at.i * a.oi, t, a.dim, x);
+    if (live) W::store(a.out, a.y_type, at.o * a.oo + at.i * a.oi, t, a.dim, x);
   }
 }
 
@@ -432,7 +443,7 @@ __global__ void __launch_bounds__(bwd_threads(GT, NCH* CH), 1) bwd_kernel(const 
   using W = Walk<GT, NCH, CH, FULL, bwd_threads(GT, NCH * CH)>;
   constexpr int E = W::E, P = W::P, T = W::T, NG = W::NG;
   extern __shared__ __align__(16) uint8_t ring[];
-  __shared__ float2 slots[2 * NG * (GT / 32)];
+  __shared__ float2 slots[GT > 32 ? 2 * NG * (GT / 32) : 1];
   const int group = threadIdx.x / GT, t = threadIdx.x % GT;
   const int rows_step = gridDim.x * NG;
   const Step step = {rows_step, rows_step / a.inner, rows_step % a.inner};
@@ -464,8 +475,10 @@ __global__ void __launch_bounds__(bwd_threads(GT, NCH* CH), 1) bwd_kernel(const 
   // w waits in shared memory: the sums need its registers
   ulonglong2* ws = reinterpret_cast<ulonglong2*>(ring + (CH == 4 ? a.depth * a.stage_bytes : 0)) + threadIdx.x;
   int have = -1;  // the outer index whose w that is
-  for (; at.row < a.rows; advance(at, step, a.inner)) {
-    if (have < 0 || (a.w_stride != 0 && have != at.o)) {
+  for (; at.row - ahead_of_warp<GT>() < a.rows; advance(at, step, a.inner)) {
+    const bool live = GT >= 32 || at.row < a.rows;
+    const int dim = live ? a.dim : 0;
+    if (live && (have < 0 || (a.w_stride != 0 && have != at.o))) {
       have = at.o;
       f2 w[P];
       W::weight(a, at.o, t, w);
@@ -474,11 +487,11 @@ __global__ void __launch_bounds__(bwd_threads(GT, NCH* CH), 1) bwd_kernel(const 
     f2 x[P], g[P];
     if constexpr (CH == 4) {
       wait_fetch(a.depth - 1);
-      W::take(mx + stage * a.stage_bytes, a.x_type, t, a.dim, x);
-      W::take(my + stage * a.stage_bytes, a.y_type, t, a.dim, g);
+      W::take(mx + stage * a.stage_bytes, a.x_type, t, dim, x);
+      W::take(my + stage * a.stage_bytes, a.y_type, t, dim, g);
     } else {
-      W::load(a.x, a.x_type, at.o * a.xo + at.i * a.xi, t, a.dim, x);
-      W::load(a.dy, a.y_type, at.o * a.yo + at.i * a.yi, t, a.dim, g);
+      W::load(a.x, a.x_type, at.o * a.xo + at.i * a.xi, t, dim, x);
+      W::load(a.dy, a.y_type, at.o * a.yo + at.i * a.yi, t, dim, g);
     }
     f2 sx = pack2(0.f, 0.f), sg = sx;
 #pragma unroll
@@ -501,7 +514,7 @@ __global__ void __launch_bounds__(bwd_threads(GT, NCH* CH), 1) bwd_kernel(const 
       }
     }
     const float2 v = group_sum2<GT>(total(qx), total(qg), group, slots, buf);
-    const float rstd = rsqrtf(v.x * inv + a.eps);
+    const float rstd = live ? rsqrtf(v.x * inv + a.eps) : 0.f;  // 0: nothing for the sums, not even 0 * inf
     // dx = rstd (g w - mean(g w) - xhat mean(g w xhat)), xhat = x rstd
     const float c0 = -rstd * m.y * inv, c1 = -rstd * (v.y * inv * rstd);
     const f2 r = pack2(rstd, rstd), k0 = pack2(c0, c0), k1 = pack2(c1, c1);
@@ -519,14 +532,14 @@ __global__ void __launch_bounds__(bwd_threads(GT, NCH* CH), 1) bwd_kernel(const 
     if (a.add != nullptr) {
       f2 ad[P];
       if (CH == 4 && a.add_staged) {
-        W::take(ma + stage * a.stage_bytes, a.x_type, t, a.dim, ad);
+        W::take(ma + stage * a.stage_bytes, a.x_type, t, dim, ad);
       } else {
-        W::load(a.add, a.x_type, at.o * a.ao + at.i * a.ai, t, a.dim, ad);
+        W::load(a.add, a.x_type, at.o * a.ao + at.i * a.ai, t, dim, ad);
       }
 #pragma unroll
       for (int k = 0; k < P; ++k) x[k] = add2(x[k], ad[k]);
     }
-    W::store(a.out, a.x_type, at.o * a.oo + at.i * a.oi, t, a.dim, x);
+    if (live) W::store(a.out, a.x_type, at.o * a.oo + at.i * a.oi, t, a.dim, x);
     if constexpr (CH == 4) {
       fetch(stage);  // every value of the stage has been used
       if (++stage == a.depth) stage = 0;
@@ -534,19 +547,32 @@ __global__ void __launch_bounds__(bwd_threads(GT, NCH* CH), 1) bwd_kernel(const 
   }
   if (a.dw == nullptr) return;
   if constexpr (CH == 4) wait_fetch(0);  // the ring is free
-  // join the groups' sums, in the order of the groups
+  // Join the groups' sums. A pair of columns is added up by several threads, each over a run of the groups, and their
+  // sums in the order of the runs by the first group's thread that owns the pair.
   if constexpr (NG > 1) {
+    constexpr int PAIRS = P * GT, RUNS = T / PAIRS > 1 ? T / PAIRS : 1;
     f2* join = reinterpret_cast<f2*>(ring);
     for (int s = 0; s < 2; ++s) {
       __syncthreads();
 #pragma unroll
       for (int k = 0; k < P; ++k) join[k * T + threadIdx.x] = s ? db[k] : dw[k];
       __syncthreads();
+      if constexpr (RUNS > 1) {
+        const int q = threadIdx.x % PAIRS, run = threadIdx.x / PAIRS;
+        f2 v = pack2(0.f, 0.f);
+        if (run < RUNS) {
+          const f2* p = join + q / GT * T + q % GT;
+          for (int n = NG * run / RUNS; n < NG * (run + 1) / RUNS; ++n) v = add2(v, p[n * GT]);
+        }
+        __syncthreads();
+        if (run < RUNS) join[run * PAIRS + q] = v;
+        __syncthreads();
+      }
       if (group == 0) {
 #pragma unroll
         for (int k = 0; k < P; ++k) {
-          f2 v = join[k * T + t];
-          for (int n = 1; n < NG; ++n) v = add2(v, join[k * T + n * GT + t]);
+          f2 v = join[RUNS > 1 ? k * GT + t : k * T + t];
+          for (int n = 1; n < (RUNS > 1 ? RUNS : NG); ++n) v = add2(v, join[RUNS > 1 ? n * PAIRS + k * GT + t : k * T + n * GT + t]);
           (s ? db[k] : dw[k]) = v;
         }
       }
@@ -698,11 +724,11 @@ static int size_of(int t) { return t == FB_F32 ? 4 : 2; }
 // 16 single elements. Fewer threads per row mean fewer barriers and more rows at once; more elements per thread than
 // 20 no longer leave registers for two blocks per SM in the backward pass.
 static int group_threads(int dim, bool vec, bool bwd) {
-  int gt = 32;
-  while (gt * (vec ? (bwd && dim <= 10240 ? 40 : 20) : 16) < dim && gt < 1024) gt *= 2;
+  int gt = 8;
+  while (gt * (gt < 32 ? 8 : vec ? (bwd && dim <= 10240 ? 40 : 20) : 16) < dim && gt < 1024) gt *= 2;
   return gt;
 }
-static int elements(int dim, int gt, bool vec) { return vec ? 4 * ((dim + 4 * gt - 1) / (4 * gt)) : 16; }
+static int elements(int dim, int gt, bool vec) { return vec ? 4 * ((dim + 4 * gt - 1) / (4 * gt)) : gt < 32 ? 8 : 16; }
 
 // Blocks per sum group of the backward pass: the SMs shared out over the groups, fewer where there are fewer rows than
 // groups of threads.
@@ -774,7 +800,9 @@ template <typename F>
 static cudaError_t with_fwd(int dim, bool vec, F f) {
   const int gt = group_threads(dim, vec, false), chunks = (dim + 4 * gt - 1) / (4 * gt);
   switch (gt) {
-    case 32: return vec ? with_chunks<32, 1, 5>(chunks, f) : f(Int<32>(), Int<16>(), Int<1>());
+    case 8: return vec ? with_chunks<8, 1, 2>(chunks, f) : f(Int<8>(), Int<8>(), Int<1>());
+    case 16: return vec ? with_chunks<16, 2, 2>(chunks, f) : f(Int<16>(), Int<8>(), Int<1>());
+    case 32: return vec ? with_chunks<32, 2, 5>(chunks, f) : f(Int<32>(), Int<16>(), Int<1>());
     case 64: return vec ? with_chunks<64, 3, 5>(chunks, f) : f(Int<64>(), Int<16>(), Int<1>());
     case 128: return vec ? with_chunks<128, 3, 5>(chunks, f) : f(Int<128>(), Int<16>(), Int<1>());
     case 256: return vec ? with_chunks<256, 3, 5>(chunks, f) : f(Int<256>(), Int<16>(), Int<1>());
@@ -786,7 +814,9 @@ template <typename F>
 static cudaError_t with_bwd(int dim, bool vec, F f) {
   const int gt = group_threads(dim, vec, true), chunks = (dim + 4 * gt - 1) / (4 * gt);
   switch (gt) {
-    case 32: return vec ? with_chunks<32, 1, 10>(chunks, f) : f(Int<32>(), Int<16>(), Int<1>());
+    case 8: return vec ? with_chunks<8, 1, 2>(chunks, f) : f(Int<8>(), Int<8>(), Int<1>());
+    case 16: return vec ? with_chunks<16, 2, 2>(chunks, f) : f(Int<16>(), Int<8>(), Int<1>());
+    case 32: return vec ? with_chunks<32, 2, 10>(chunks, f) : f(Int<32>(), Int<16>(), Int<1>());
     case 64: return vec ? with_chunks<64, 6, 10>(chunks, f) : f(Int<64>(), Int<16>(), Int<1>());
     case 128: return vec ? with_chunks<128, 6, 10>(chunks, f) : f(Int<128>(), Int<16>(), Int<1>());
     case 256: return vec ? with_chunks<256, 6, 10>(chunks, f) : f(Int<256>(), Int<16>(), Int<1>());
@@ -845,7 +875,7 @@ static cudaError_t setup() {
     return e;
   };
   for (int vec = 0; vec < 2; ++vec)
-    for (int dim = 32 * 4; dim <= kMaxDimRegs; dim += 32 * 4) {
+    for (int dim = 32; dim <= kMaxDimRegs; dim += dim < 128 ? 32 : 128) {
       with_fwd(dim, vec, fwd);
       with_bwd(dim, vec, bwd);
     }

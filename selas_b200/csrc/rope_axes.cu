@@ -215,7 +215,9 @@ static cudaError_t go(Args& a, cudaStream_t st) {
   const int64_t fair = (static_cast<int64_t>(a.tokens) * a.heads + room - 1) / room;
   const int64_t runs = (a.heads + most - 1) / most;
   a.per_item = static_cast<int>(std::min<int64_t>(fair, (a.heads + runs - 1) / runs));
-  a.items = a.tokens * static_cast<uint32_t>((a.heads + a.per_item - 1) / a.per_item);
+  const int64_t items = static_cast<int64_t>(a.tokens) * ((a.heads + a.per_item - 1) / a.per_item);
+  if (items > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;  // more than 180 GB hold in any layout but broadcast ones
+  a.items = static_cast<uint32_t>(items);
   const unsigned grid = (a.items + groups - 1) / groups;
   const int smem = V * sizeof(T) == 16 ? a.per_item * (HALVES ? 2 : 1) * kThreads * 16 : 0;
   rope_axes_kernel<T, V, HALVES><<<grid, kThreads, smem, st>>>(a);

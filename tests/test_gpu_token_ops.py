@@ -235,7 +235,7 @@ def check_norm(got, x, w, b, eps):
     check(got, ref, dh * wf.abs() + 3 * U * ((h * wf).abs() + bf.abs()), f"norm {tuple(x.shape)}")
 
 
-DIMS = [1, 2, 3, 8, 31, 32, 33, 100, 127, 128, 129, 256, 384, 511, 512, 513, 640, 768, 896, 1000, 1024, 1025, 1152, 1280, 1536, 1792,
+DIMS = [1, 2, 3, 4, 7, 8, 16, 24, 31, 32, 33, 63, 64, 65, 96, 100, 127, 128, 129, 256, 384, 511, 512, 513, 640, 768, 896, 1000, 1024, 1025, 1152, 1280, 1536, 1792,
         2047, 2048, 2304, 2560, 3072, 3584, 4096, 4100, 4608, 5120, 6144, 7168,
         8191, 8192, 10240, 12288, 16384, 16385, 20004]
 
@@ -381,6 +381,16 @@ def test_mod_backward(b, l, d, yt):
     rx, rw, rb = grad_ref(dy, x, 1 + scale[:1].double()[:, None], 1e-6, None, False)
     check_grads((dx1, dscale1, dshift1), (rx, (rw[0][None], rw[1][None]), (rb[0][None], rb[1][None])))
     assert ops().ln_mod_backward(dy, x, scale, sums=False)[1:] == (None, None)
+
+
+@pytest.mark.parametrize("dim", [8, 24, 63, 64, 100, 128])
+def test_norm_small_rows_eps_zero(dim):
+    """Many short rows per warp, the last warp not full, and no eps to hide a division by nothing behind."""
+    g = gen(26)
+    for rows in (1, 3, 70001):
+        x, dy, w = randn(g, rows, dim), randn(g, rows, dim), randn(g, dim, mean=1.0)
+        check_norm(ops().layer_norm(x, w, None, 0.0), x, w, None, 0.0)
+        check_grads(ops().layer_norm_backward(dy, x, w, 0.0), grad_ref(dy, x, w.double(), 0.0, None, False))
 
 
 def test_norm_backward_no_rows():

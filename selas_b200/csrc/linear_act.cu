@@ -838,11 +838,39 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
 }  // namespace many
 
 // Rows of a 16-bit matrix whose start or stride is not a multiple of 16 bytes, copied to rows of `ldo` elements (a
-// multiple of 8): what TMA can read. The columns past k are never read (the tensor map ends at k).
+// multiple of 8): what TMA can read. The columns past k are never read (the tensor map ends at k). Eight elements per
+// thread, one 16-byte store: inside a row from the four or five aligned words that hold them, near its ends one by one
+// (a word there may reach out of the matrix).
 __global__ void __launch_bounds__(256) align_rows_kernel(const uint16_t* __restrict__ in, int64_t ld, int64_t rows, int k,
                                                          uint16_t* __restrict__ out, int64_t ldo) {
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x)
-    for (int c = threadIdx.x; c < k; c += 256) out[row * ldo + c] = __ldg(in + row * ld + c);
+  const int64_t per_row = ldo / 8, all = rows * per_row;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t row = i / per_row;
+    const int c = static_cast<int>(i - row * per_row) * 8;
+    const uint16_t* s = in + row * ld + c;
+    uint32_t w[4];
+    if (c >= 8 && c + 9 <= k) {
+      if (reinterpret_cast<uintptr_t>(s) & 2u) {
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(s - 1);
+        uint32_t v[5];
+#pragma unroll
+        for (int j = 0; j < 5; ++j) v[j] = __ldg(p + j);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = __funnelshift_r(v[j], v[j + 1], 16);
+      } else {
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(s);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = __ldg(p + j);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t lo = c + 2 * j < k ? __ldg(s + 2 * j) : 0, hi = c + 2 * j + 1 < k ? __ldg(s + 2 * j + 1) : 0;
+        w[j] = lo | hi << 16;
+      }
+    }
+    *reinterpret_cast<uint4*>(out + row * ldo + c) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
 }
 
 template <typename K>
@@ -994,13 +1022,17 @@ int launch_linear_act(const fb_linear_act_args& p, cudaStream_t st, std::string&
   Args a;
   memset(&a, 0, sizeof(a));
   const bool half = p.dtype == FB_F16;
+  a.vec = align(p.out, 4 * osz) && p.ld_out % 4 == 0 && align(p.bias, 8) &&
+          (!p.residual || (align(p.residual, 4 * rsz) && p.ld_residual % 4 == 0));
   a.num_kb = (p.k + BK - 1) / BK;
   const int64_t tiles_many = ((p.m + 255ll) / 256) * ((p.n + 255ll) / 256);
   // many_kernel's larger tiles pay once there is work for them; below, few_kernel is done sooner (no second CTA to meet, a
   // smaller tile to fill and write). Measured, few against many, each call with a cold L2: 256 x 3072 x 3072 (m x k x n)
   // 14.7 / 16.6 us, 2048 x 1024 x 1024 12.4 / 14.5, 1024 x 1024 x 4096 14.5 / 14.5, 1024 x 3072 x 3072 26.8 / 24.8,
   // 8192 x 1024 x 1024 26.8 / 20.7, 4608 x 3072 x 3072 82 / 60; up to 128 rows few_kernel's one token tile is never worse.
-  const bool many_rows = p.m > 128 && static_cast<double>(p.m) * p.n * p.k >= 4294967296.0;
+  // With many tiles and little K it is the epilogue that counts, which many_kernel overlaps (2000 x 100 x 17000 79 / 70;
+  // with outputs written one by one, 17001, it is the slower of the two, 126 / 182).
+  const bool many_rows = p.m > 128 && (static_cast<double>(p.m) * p.n * p.k >= 4294967296.0 || (a.vec && tiles_many >= kNumSms));
   const int bt = many_rows ? 128 : p.m <= 16 ? 16 : p.m <= 32 ? 32 : p.m <= 64 ? 64 : 128;
   if (p.k > 0) {
     const void *x = p.x, *w = p.w;
@@ -1011,7 +1043,8 @@ int launch_linear_act(const fb_linear_act_args& p, cudaStream_t st, std::string&
         return bad(FB_ERR_ARG, "rows that do not start on 16 bytes need a workspace (fb_linear_act_work_bytes), 16-byte aligned");
       char* work = static_cast<char*>(p.work);
       auto copy = [&](const void*& q, int64_t& ld, int rows) {
-        align_rows_kernel<<<std::min(rows, 16 * kNumSms), 256, 0, st>>>(static_cast<const uint16_t*>(q), ld, rows, p.k,
+        const int64_t chunks = rows * (up8(p.k) / 8);
+        align_rows_kernel<<<static_cast<unsigned>(std::min<int64_t>((chunks + 255) / 256, 16 * kNumSms)), 256, 0, st>>>(static_cast<const uint16_t*>(q), ld, rows, p.k,
                                                                        reinterpret_cast<uint16_t*>(work), up8(p.k));
         q = work;
         ld = up8(p.k);
@@ -1039,8 +1072,6 @@ int launch_linear_act(const fb_linear_act_args& p, cudaStream_t st, std::string&
   a.half = half;
   a.res_f32 = p.residual_dtype == FB_F32;
   a.out_f32 = p.out_dtype == FB_F32;
-  a.vec = align(p.out, 4 * osz) && p.ld_out % 4 == 0 && align(p.bias, 8) &&
-          (!p.residual || (align(p.residual, 4 * rsz) && p.ld_residual % 4 == 0));
   a.idesc = many_rows ? idesc_bf16_f32(256, 256, false) : idesc_bf16_f32(kFeat, bt, false);
   if (half) a.idesc &= ~((1u << 7) | (1u << 10));  // operand format 0: fp16
   a.status = dev->status;

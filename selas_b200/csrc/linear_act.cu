@@ -550,7 +550,8 @@ constexpr int kCols = 4 * kTile / kEpiWarps;  // sums of a thread
 // Three warpgroups: loads and MMAs (two of its warps idle), and the two of the epilogue, which take the registers that
 // the first gives back. 128 x 40 + 256 x 232 = 384 x 168, what the block is launched with.
 constexpr int kThreads = 128 + 32 * kEpiWarps;
-constexpr int kLeanRegs = 40, kEpiRegs = 232;
+constexpr int kLeanRegs = 40, kEpiRegs = 232, kLaunchRegs = 168;
+static_assert(128 * kLeanRegs + 256 * kEpiRegs == (128 + 32 * kEpiWarps) * kLaunchRegs, "the split is what the launch allots");
 constexpr int kSub = 2;
 constexpr int kStages = 3;
 constexpr int kChunkStages = 8;
@@ -950,6 +951,7 @@ static int64_t copy_bytes(int rows, int k) { return 2 * static_cast<int64_t>(row
 std::string linear_act_setup() {
   using namespace lact;
   cudaError_t e = cudaSuccess;
+  bool split_ok = true;
   auto raise = [&](auto kernel, int bytes) {
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   };
@@ -962,9 +964,18 @@ std::string linear_act_setup() {
       raise(few_kernel<128, ACT>, Few<128>::kSmemBytes);
       raise(many::many_kernel<ACT, false>, many::kSmemBytes);
       raise(many::many_kernel<ACT, true>, many::kSmemBytes);
+      for (const void* k : {reinterpret_cast<const void*>(many::many_kernel<ACT, false>),
+                            reinterpret_cast<const void*>(many::many_kernel<ACT, true>)}) {
+        cudaFuncAttributes at;
+        if (e == cudaSuccess) e = cudaFuncGetAttributes(&at, k);
+        if (e == cudaSuccess && at.numRegs != many::kLaunchRegs) split_ok = false;
+      }
       return cudaSuccess;
     });
   }
+  // The register split takes more than a launch with fewer registers per thread would have: setmaxnreg.inc would wait
+  // for good. So a build that compiled to another number is refused here.
+  if (!split_ok) return "linear_act: many_kernel is not compiled to " + std::to_string(many::kLaunchRegs) + " registers";
   for (int s = 2; e == cudaSuccess && s <= many::kMaxSplits; ++s) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * s * 74, 1, 1);

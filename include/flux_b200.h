@@ -250,7 +250,8 @@ int32_t fb_rope_axes(const fb_rope_args* args, void* stream);
  * Backward (dy like x; x is normalised again, nothing is saved by the forward):
  *   g = dy * w,  dx = (g - mean(g) - xhat * mean(g * xhat)) / sqrt(var + eps) [+ add],
  *   dweight = sum of dy * xhat,  dbias = sum of dy   (fp32 [dim], or [outer, dim] with sum_per_outer; both or neither),
- * summed in a fixed order through `work` (fb_layer_norm_work_floats floats). dx has x's type. */
+ * summed in a fixed order through `work` (fb_layer_norm_work_floats floats). dx has x's type. A weight per outer index
+ * has its sums per outer index, of which there are at most 65535. */
 typedef struct fb_layer_norm_args {
   const void* x; int64_t x_outer_stride, x_inner_stride;
   const void* dy; int64_t dy_outer_stride, dy_inner_stride;        /* backward */

@@ -353,11 +353,6 @@ struct Walk {
     }
     store_row<GT, NCH, CH, FULL>(p, type, base, t, dim, f);
   }
-  // A thread's own pairs in shared memory, two to a 16-byte place.
-  static __device__ __forceinline__ void keep(ulonglong2* at, const f2 (&v)[P]) {
-#pragma unroll
-    for (int k = 0; k < P; k += 2) at[(k / 2) * T] = make_ulonglong2(v[k], v[k + 1]);
-  }
   // w of outer index o, as it multiplies: w_plus + w, or ones
   static __device__ __forceinline__ void weight(const Args& a, int o, int t, f2 (&w)[P]) {
     if (a.w != nullptr) {
@@ -416,21 +411,21 @@ __global__ void __launch_bounds__(fwd_threads(GT), fwd_blocks(GT, NCH* CH)) fwd_
     } else {
       W::load(a.x, a.x_type, at.o * a.xo + at.i * a.xi, t, live ? a.dim : 0, x);
     }
-    f2 s = pack2(0.f, 0.f);
+    f2 s[2], q[2];  // two running sums: the additions of one would wait for one another
+    s[0] = s[1] = q[0] = q[1] = pack2(0.f, 0.f);
 #pragma unroll
-    for (int k = 0; k < P; ++k) s = add2(s, x[k]);
-    const float mean = group_sum2<GT>(total(s), 0.f, group, slots, buf).x * inv;
+    for (int k = 0; k < P; ++k) s[k & 1] = add2(s[k & 1], x[k]);
+    const float mean = group_sum2<GT>(total(add2(s[0], s[1])), 0.f, group, slots, buf).x * inv;
     if constexpr (CH == 4) {
       fetch(stage);  // the stage's values are in registers
       if (++stage == a.depth) stage = 0;
     }
-    f2 q = pack2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < P; ++k) {
       x[k] = add2(x[k], W::inside(t, k, a.dim, -mean));
-      q = fma2(x[k], x[k], q);
+      q[k & 1] = fma2(x[k], x[k], q[k & 1]);
     }
-    const float rstd = rsqrtf(group_sum2<GT>(total(q), 0.f, group, slots, buf).x * inv + a.eps);
+    const float rstd = rsqrtf(group_sum2<GT>(total(add2(q[0], q[1])), 0.f, group, slots, buf).x * inv + a.eps);
     const f2 r = pack2(rstd, rstd);
 #pragma unroll
     for (int k = 0; k < P; ++k) x[k] = fma2(mul2(x[k], r), w[k], b[k]);
@@ -472,18 +467,19 @@ __global__ void __launch_bounds__(bwd_threads(GT, NCH* CH), 1) bwd_kernel(const 
   f2 dw[P], db[P];
 #pragma unroll
   for (int k = 0; k < P; ++k) dw[k] = db[k] = pack2(0.f, 0.f);
-  // w waits in shared memory: the sums need its registers
-  ulonglong2* ws = reinterpret_cast<ulonglong2*>(ring + (CH == 4 ? a.depth * a.stage_bytes : 0)) + threadIdx.x;
-  int have = -1;  // the outer index whose w that is
+  // w waits in shared memory, once for all groups: the sums need its registers. All rows of a block have the same w (a
+  // w per outer index comes with a sum group per outer index).
+  ulonglong2* ws = reinterpret_cast<ulonglong2*>(ring + (CH == 4 ? a.depth * a.stage_bytes : 0)) + t;
+  if (group == 0) {
+    f2 w[P];
+    W::weight(a, at.o, t, w);
+#pragma unroll
+    for (int k = 0; k < P; k += 2) ws[(k / 2) * GT] = make_ulonglong2(w[k], w[k + 1]);
+  }
+  __syncthreads();
   for (; at.row - ahead_of_warp<GT>() < a.rows; advance(at, step, a.inner)) {
     const bool live = GT >= 32 || at.row < a.rows;
     const int dim = live ? a.dim : 0;
-    if (live && (have < 0 || (a.w_stride != 0 && have != at.o))) {
-      have = at.o;
-      f2 w[P];
-      W::weight(a, at.o, t, w);
-      W::keep(ws, w);
-    }
     f2 x[P], g[P];
     if constexpr (CH == 4) {
       wait_fetch(a.depth - 1);
@@ -493,34 +489,39 @@ __global__ void __launch_bounds__(bwd_threads(GT, NCH* CH), 1) bwd_kernel(const 
       W::load(a.x, a.x_type, at.o * a.xo + at.i * a.xi, t, dim, x);
       W::load(a.dy, a.y_type, at.o * a.yo + at.i * a.yi, t, dim, g);
     }
-    f2 sx = pack2(0.f, 0.f), sg = sx;
+    // two running sums of each kind: the additions of one would wait for one another
+    f2 sx[2], sg[2];
+    sx[0] = sx[1] = sg[0] = sg[1] = pack2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < P; k += 2) {
-      const ulonglong2 w = ws[(k / 2) * T];
-      sx = add2(add2(sx, x[k]), x[k + 1]);
-      sg = fma2(g[k + 1], w.y, fma2(g[k], w.x, sg));
+      const ulonglong2 w = ws[(k / 2) * GT];
+      sx[0] = add2(sx[0], x[k]);
+      sx[1] = add2(sx[1], x[k + 1]);
+      sg[0] = fma2(g[k], w.x, sg[0]);
+      sg[1] = fma2(g[k + 1], w.y, sg[1]);
     }
-    const float2 m = group_sum2<GT>(total(sx), total(sg), group, slots, buf);
+    const float2 m = group_sum2<GT>(total(add2(sx[0], sx[1])), total(add2(sg[0], sg[1])), group, slots, buf);
     const float mean = m.x * inv;
-    f2 qx = pack2(0.f, 0.f), qg = qx;
+    f2 qx[2], qg[2];
+    qx[0] = qx[1] = qg[0] = qg[1] = pack2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < P; k += 2) {
-      const ulonglong2 w = ws[(k / 2) * T];
+      const ulonglong2 w = ws[(k / 2) * GT];
 #pragma unroll
-      for (int j = k; j < k + 2; ++j) {
-        x[j] = add2(x[j], W::inside(t, j, a.dim, -mean));
-        qx = fma2(x[j], x[j], qx);
-        qg = fma2(mul2(g[j], j == k ? w.x : w.y), x[j], qg);
+      for (int j = 0; j < 2; ++j) {
+        x[k + j] = add2(x[k + j], W::inside(t, k + j, a.dim, -mean));
+        qx[j] = fma2(x[k + j], x[k + j], qx[j]);
+        qg[j] = fma2(mul2(g[k + j], j ? w.y : w.x), x[k + j], qg[j]);
       }
     }
-    const float2 v = group_sum2<GT>(total(qx), total(qg), group, slots, buf);
+    const float2 v = group_sum2<GT>(total(add2(qx[0], qx[1])), total(add2(qg[0], qg[1])), group, slots, buf);
     const float rstd = live ? rsqrtf(v.x * inv + a.eps) : 0.f;  // 0: nothing for the sums, not even 0 * inf
     // dx = rstd (g w - mean(g w) - xhat mean(g w xhat)), xhat = x rstd
     const float c0 = -rstd * m.y * inv, c1 = -rstd * (v.y * inv * rstd);
     const f2 r = pack2(rstd, rstd), k0 = pack2(c0, c0), k1 = pack2(c1, c1);
 #pragma unroll
     for (int k = 0; k < P; k += 2) {
-      const ulonglong2 w = ws[(k / 2) * T];
+      const ulonglong2 w = ws[(k / 2) * GT];
 #pragma unroll
       for (int j = k; j < k + 2; ++j) {
         const f2 h = mul2(x[j], r);
@@ -595,10 +596,11 @@ __global__ void __launch_bounds__(bwd_threads(GT, NCH* CH), 1) bwd_kernel(const 
   }
 }
 
-// dw, db [sum group][dim] = the partials' sums. 32 columns x 8 runs of the partials per block, joined in order.
-__global__ void __launch_bounds__(256) join_kernel(const float* part, int blocks, int dim,
-                                                   float* __restrict__ dw, float* __restrict__ db) {
-  __shared__ float s[8][32];
+// dw, db [sum group][dim] = the partials' sums. 32 columns x 32 runs of the partials per block, joined in order: with a
+// partial per SM a thread has four or five loads, all on their way at once.
+__global__ void __launch_bounds__(1024) join_kernel(const float* part, int blocks, int dim, float* __restrict__ dw,
+                                                    float* __restrict__ db) {
+  __shared__ float s[32][33];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 31, run = threadIdx.x >> 5;
   const int64_t n2 = 2ll * dim;
@@ -606,16 +608,15 @@ __global__ void __launch_bounds__(256) join_kernel(const float* part, int blocks
   const float* p = part + static_cast<int64_t>(blockIdx.y) * blocks * n2 + col;
   float v = 0.f;
   if (col < n2) {
-    const int lo = static_cast<int>(static_cast<int64_t>(blocks) * run / 8);
-    const int hi = static_cast<int>(static_cast<int64_t>(blocks) * (run + 1) / 8);
-#pragma unroll 8
+    const int lo = blocks * run / 32, hi = blocks * (run + 1) / 32;
+#pragma unroll 5
     for (int k = lo; k < hi; ++k) v += p[k * n2];
   }
   s[run][lane] = v;
   __syncthreads();
   if (run == 0 && col < n2) {
 #pragma unroll
-    for (int r = 1; r < 8; ++r) v += s[r][lane];
+    for (int r = 1; r < 32; ++r) v += s[r][lane];
     float* d = col < dim ? dw : db - dim;
     d[static_cast<int64_t>(blockIdx.y) * dim + col] = v;
   }
@@ -756,8 +757,8 @@ static cudaError_t go_fwd(Args a, cudaStream_t st) {
 
 template <int GT, int NCH, int CH, bool FULL>
 static cudaError_t go_bwd(Args a, int64_t sum_groups, cudaStream_t st) {
-  constexpr int T = bwd_threads(GT, NCH * CH), w_bytes = NCH * CH * T * 4;
-  int smem = w_bytes;  // after the walk, the groups' sums take this much too
+  constexpr int T = bwd_threads(GT, NCH * CH), w_bytes = NCH * CH * GT * 4;
+  int smem = w_bytes;
   if (CH == 4) {
     const int xb = size_of(a.x_type), yb = size_of(a.y_type);
     const int two = 4 * NCH * T * (xb + yb), three = two + 4 * NCH * T * xb;
@@ -766,6 +767,7 @@ static cudaError_t go_bwd(Args a, int64_t sum_groups, cudaStream_t st) {
     a.depth = std::max(1, std::min(4, (kRingPerSm - w_bytes) / a.stage_bytes));
     smem += a.depth * a.stage_bytes;
   }
+  smem = std::max(smem, NCH * CH * T * 4);  // after the walk, the groups' sums
   const int64_t blocks = bwd_blocks(a.rows, a.dim, sum_groups, CH == 4);
   const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(sum_groups));
   bwd_kernel<GT, NCH, CH, FULL><<<grid, T, smem, st>>>(a);
@@ -774,7 +776,7 @@ static cudaError_t go_bwd(Args a, int64_t sum_groups, cudaStream_t st) {
     // launched while the last blocks of the walk still run; it waits for them before it reads
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>((2ll * a.dim + 31) / 32), static_cast<unsigned>(sum_groups));
-    cfg.blockDim = dim3(256);
+    cfg.blockDim = dim3(1024);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -923,7 +925,9 @@ int launch_layer_norm(const fb_layer_norm_args& p, bool bwd, cudaStream_t st, st
   if (sums && (!p.dweight || !p.dbias)) return bad(FB_ERR_ARG, "dweight and dbias come together");
   const int64_t rows_all = (p.inner > 0 && p.outer > (1ll << 31) / p.inner) ? (1ll << 40) : p.outer * p.inner;
   if (rows_all > (1ll << 30)) return bad(FB_ERR_UNSUPPORTED, "at most 2^30 rows per call");
-  const bool per_outer = sums && p.sum_per_outer;
+  // A block of the backward pass works with one w, so a w per outer index makes a sum group of each.
+  const bool per_outer = bwd && ((sums && p.sum_per_outer) || p.w_outer_stride != 0);
+  if (sums && per_outer && !p.sum_per_outer) return bad(FB_ERR_UNSUPPORTED, "a weight per outer index has sums per outer index");
   const int64_t groups = per_outer ? p.outer : 1;
   if (groups > 65535) return bad(FB_ERR_UNSUPPORTED, "at most 65535 gradients of their own per call");
   if (rows_all == 0) {

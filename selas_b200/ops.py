@@ -582,9 +582,15 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     return out
 
 
+@functools.lru_cache(maxsize=4096)
+def _norm_work(outer: int, inner: int, d: int, per_outer: int) -> int:
+    return _lib.load().fb_layer_norm_work_floats(outer, inner, d, per_outer)
+
+
 def _norm_backward(what: str, index: int, dy, x, eps: float, weight: int, w_code: int, w_stride: int, plus_one: bool, add,
-                   sums: bool, groups: int):
-    """(dx, dweight, dbias) with one dweight and dbias per group of rows: all rows, or those of an outer index."""
+                   sums: bool, groups: int, flat: bool):
+    """(dx, dweight, dbias) with one dweight and dbias per group of rows: all rows, or those of an outer index; [D]
+    (flat) or [groups, D]."""
     outer, inner, d, code = _norm_rows(what, x)
     y_code = _DTYPE_CODE.get(dy.dtype)
     if y_code is None or dy.shape != x.shape:
@@ -603,10 +609,11 @@ def _norm_backward(what: str, index: int, dy, x, eps: float, weight: int, w_code
     per_outer = 1 if groups > 1 else 0
     if sums:
         # the two gradients and the partial sums in one allocation
-        need = _lib.load().fb_layer_norm_work_floats(outer, inner, d, per_outer)
+        need = _norm_work(outer, inner, d, per_outer)
         n = groups * d
         buf = x.new_empty(2 * n + need, dtype=F32)
-        dw, db = buf[:n], buf[n:2 * n]
+        shape, strides = ((d,), (1,)) if flat else ((groups, d), (d, 1))
+        dw, db = buf.as_strided(shape, strides, 0), buf.as_strided(shape, strides, n)
         pw = buf.data_ptr()
         pb, work = pw + 4 * n, pw + 8 * n
     rows = outer * inner
@@ -629,7 +636,7 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor 
     w = w_code = 0
     if weight is not None:
         w, w_code = _norm_vector("layer_norm_backward", "weight", x.shape[-1] if x.dim() else 0, weight)
-    return _norm_backward("layer_norm_backward", index, dy, x, eps, w, w_code, 0, False, add, sums, 1)
+    return _norm_backward("layer_norm_backward", index, dy, x, eps, w, w_code, 0, 0, add, sums, 1, True)
 
 
 def ln_mod_backward(dy: torch.Tensor, x: torch.Tensor, scale: torch.Tensor, *, add: torch.Tensor | None = None,
@@ -643,13 +650,11 @@ def ln_mod_backward(dy: torch.Tensor, x: torch.Tensor, scale: torch.Tensor, *, a
     b, _, d = x.shape
     sc, stride = _mod_rows(scale, b, d)
     rows = sc.shape[0]
-    dx, dscale, dshift = _norm_backward("ln_mod_backward", index, dy, x, 1e-6, sc.data_ptr(), _lib.FB_BF16, stride, True, add,
-                                        sums and rows > 0, rows)
+    dx, dscale, dshift = _norm_backward("ln_mod_backward", index, dy, x, 1e-6, sc.data_ptr(), _lib.FB_BF16, stride, 1, add,
+                                        sums and rows > 0, rows, False)
     if sums and rows == 0:
-        dscale = dshift = x.new_empty(0)
-    if dscale is None:
-        return dx, None, None
-    return dx, dshift.view(rows, d), dscale.view(rows, d)
+        dscale, dshift = x.new_empty((0, d)), x.new_empty((0, d))
+    return dx, dshift, dscale
 
 
 def _rows(t: torch.Tensor, rows: int, cols: int) -> tuple[torch.Tensor, int]:

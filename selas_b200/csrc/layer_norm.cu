@@ -721,20 +721,26 @@ __global__ void __launch_bounds__(256) sums_wide_kernel(const __grid_constant__ 
 
 static int size_of(int t) { return t == FB_F32 ? 4 : 2; }
 
-// The group of threads for a row of `dim` elements, and the chunks a thread holds: at most 5 chunks of 4 (vectors), or
-// 16 single elements. Fewer threads per row mean fewer barriers and more rows at once; more elements per thread than
-// 20 no longer leave registers for two blocks per SM in the backward pass.
-static int group_threads(int dim, bool vec, bool bwd) {
+// The group of threads for a row of `dim` elements. Few threads with many elements each cost the fewest barriers,
+// shuffles and addresses per element, and the independent arithmetic of many elements hides latency better than more
+// warps do (65537 x 768 in bf16, forward and backward: 47 and 84 us with 12 to 16 elements a thread, 39 and 66 with 24;
+// 6000 x 6144 backward: 110 with 12, 78 with 24). The bound is what the registers hold: x, w and b forward at two blocks
+// of 256 threads per SM, x, dy and the two running column sums backward, where blocks get smaller as threads hold more.
+static int group_threads(int dim, bool vec, int most) {
   int gt = 8;
-  while (gt * (gt < 32 ? 8 : vec ? (bwd && dim <= 10240 ? 40 : 20) : 16) < dim && gt < 1024) gt *= 2;
+  while (gt * (gt < 32 ? 8 : vec ? most : 16) < dim && gt < 1024) gt *= 2;
   return gt;
 }
+// The most elements a thread holds: forward 32 of 16-bit rows, whose widening costs instructions, and 20 of fp32 rows,
+// which need the warps more (18432 x 3072 57 us with 12, 61 with 24); 20 where wider rows would spill.
+static int most_fwd(int dim, int x_type) { return x_type != FB_F32 && dim <= 8192 ? 32 : 20; }
+static int most_bwd(int dim) { return dim <= 10240 ? 40 : 20; }
 static int elements(int dim, int gt, bool vec) { return vec ? 4 * ((dim + 4 * gt - 1) / (4 * gt)) : gt < 32 ? 8 : 16; }
 
 // Blocks per sum group of the backward pass: the SMs shared out over the groups, fewer where there are fewer rows than
 // groups of threads.
 static int64_t bwd_blocks(int64_t rows, int dim, int64_t sum_groups, bool vec) {
-  const int gt = group_threads(dim, vec, true), ng = bwd_threads(gt, elements(dim, gt, vec)) / gt;
+  const int gt = group_threads(dim, vec, most_bwd(dim)), ng = bwd_threads(gt, elements(dim, gt, vec)) / gt;
   const int64_t need = std::max<int64_t>(1, (rows + ng - 1) / ng);
   return std::max<int64_t>(1, std::min<int64_t>(need, kNumSms / std::max<int64_t>(1, sum_groups)));
 }
@@ -799,22 +805,22 @@ static cudaError_t with_chunks(int chunks, F f) {
   return f(Int<GT>(), Int<FROM>(), Int<4>());
 }
 template <typename F>
-static cudaError_t with_fwd(int dim, bool vec, F f) {
-  const int gt = group_threads(dim, vec, false), chunks = (dim + 4 * gt - 1) / (4 * gt);
+static cudaError_t with_fwd(int dim, bool vec, int x_type, F f) {
+  const int gt = group_threads(dim, vec, most_fwd(dim, x_type)), chunks = (dim + 4 * gt - 1) / (4 * gt);
   switch (gt) {
     case 8: return vec ? with_chunks<8, 1, 2>(chunks, f) : f(Int<8>(), Int<8>(), Int<1>());
     case 16: return vec ? with_chunks<16, 2, 2>(chunks, f) : f(Int<16>(), Int<8>(), Int<1>());
-    case 32: return vec ? with_chunks<32, 2, 5>(chunks, f) : f(Int<32>(), Int<16>(), Int<1>());
-    case 64: return vec ? with_chunks<64, 3, 5>(chunks, f) : f(Int<64>(), Int<16>(), Int<1>());
-    case 128: return vec ? with_chunks<128, 3, 5>(chunks, f) : f(Int<128>(), Int<16>(), Int<1>());
-    case 256: return vec ? with_chunks<256, 3, 5>(chunks, f) : f(Int<256>(), Int<16>(), Int<1>());
+    case 32: return vec ? with_chunks<32, 2, 8>(chunks, f) : f(Int<32>(), Int<16>(), Int<1>());
+    case 64: return vec ? with_chunks<64, 3, 8>(chunks, f) : f(Int<64>(), Int<16>(), Int<1>());
+    case 128: return vec ? with_chunks<128, 3, 8>(chunks, f) : f(Int<128>(), Int<16>(), Int<1>());
+    case 256: return vec ? with_chunks<256, 3, 8>(chunks, f) : f(Int<256>(), Int<16>(), Int<1>());
     case 512: return vec ? with_chunks<512, 3, 5>(chunks, f) : f(Int<512>(), Int<16>(), Int<1>());
     default: return vec ? with_chunks<1024, 3, 4>(chunks, f) : f(Int<1024>(), Int<16>(), Int<1>());
   }
 }
 template <typename F>
 static cudaError_t with_bwd(int dim, bool vec, F f) {
-  const int gt = group_threads(dim, vec, true), chunks = (dim + 4 * gt - 1) / (4 * gt);
+  const int gt = group_threads(dim, vec, most_bwd(dim)), chunks = (dim + 4 * gt - 1) / (4 * gt);
   switch (gt) {
     case 8: return vec ? with_chunks<8, 1, 2>(chunks, f) : f(Int<8>(), Int<8>(), Int<1>());
     case 16: return vec ? with_chunks<16, 2, 2>(chunks, f) : f(Int<16>(), Int<8>(), Int<1>());
@@ -855,7 +861,7 @@ static cudaError_t dispatch(const Args& a, bool bwd, int64_t sum_groups, bool ve
     }
     return go_bwd<GT, NCH, CH, false>(a, sum_groups, st);
   };
-  return bwd ? with_bwd(a.dim, vec, back) : with_fwd(a.dim, vec, run);
+  return bwd ? with_bwd(a.dim, vec, back) : with_fwd(a.dim, vec, a.x_type, run);
 }
 
 // Raises the shared-memory limits of every instance (ring of up to kRingPerSm bytes).
@@ -878,7 +884,8 @@ static cudaError_t setup() {
   };
   for (int vec = 0; vec < 2; ++vec)
     for (int dim = 32; dim <= kMaxDimRegs; dim += dim < 128 ? 32 : 128) {
-      with_fwd(dim, vec, fwd);
+      with_fwd(dim, vec, FB_F32, fwd);
+      with_fwd(dim, vec, FB_BF16, fwd);
       with_bwd(dim, vec, bwd);
     }
   return e;

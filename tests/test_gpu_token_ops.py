@@ -240,11 +240,12 @@ DIMS = [1, 2, 3, 4, 7, 8, 16, 24, 31, 32, 33, 63, 64, 65, 96, 100, 127, 128, 129
         8191, 8192, 10240, 12288, 16384, 16385, 20004]
 
 
+@pytest.mark.parametrize("xt", [F32, BF16])
 @pytest.mark.parametrize("dim", DIMS)
-def test_norm_sizes(dim):
+def test_norm_sizes(dim, xt):
     g = gen(10)
-    for rows in (1, 2, 9, 77):
-        x = randn(g, rows, dim, mean=0.3)
+    for rows in (1, 2, 9, 77, 1500 if dim < 1300 else 400):
+        x = randn(g, rows, dim, mean=0.3, dtype=xt)
         w, b = randn(g, dim, std=0.3, mean=1.0), randn(g, dim, std=0.3)
         check_norm(ops().layer_norm(x, w, b), x, w, b, 1e-5)
 
@@ -322,11 +323,12 @@ def check_grads(got, refs):
         check(t, ref, bound, name)
 
 
+@pytest.mark.parametrize("xt", [F32, BF16])
 @pytest.mark.parametrize("dim", DIMS)
-def test_norm_backward_sizes(dim):
+def test_norm_backward_sizes(dim, xt):
     g = gen(20)
     for rows in (1, 3, 77, 1500 if dim < 1300 else 400):
-        x, dy = randn(g, rows, dim, mean=0.3), randn(g, rows, dim)
+        x, dy = randn(g, rows, dim, mean=0.3, dtype=xt), randn(g, rows, dim, dtype=xt)
         w = randn(g, dim, std=0.3, mean=1.0)
         got = ops().layer_norm_backward(dy, x, w)
         assert got[1].dtype == got[2].dtype == F32

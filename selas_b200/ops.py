@@ -529,7 +529,7 @@ def _outer_inner(what: str, t: torch.Tensor) -> tuple[int, int]:
         return 0, st[0] if n == 2 else 0
     if not t.is_contiguous():
         _refuse(f"{what}: a tensor of more than three dims must be contiguous")
-    return st[-3], st[-2]
+    return t.shape[-2] * t.shape[-1], t.shape[-1]  # not its strides, which mean nothing where a dim is 1
 
 
 def _norm_rows(what: str, x: torch.Tensor) -> tuple[int, int, int, int]:

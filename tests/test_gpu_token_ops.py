@@ -276,6 +276,17 @@ def test_norm_strides():
         check_norm(ops().layer_norm(v, w[:d].clone(), b[:d].clone()), v, w[:d], b[:d], 1e-5)
 
 
+def test_norm_many_dims_with_a_dim_of_one():
+    """Contiguous tensors of four and five dims whose dim of one has some other stride, forward and backward."""
+    g = gen(14)
+    w, b = randn(g, 96, mean=1.0), randn(g, 96)
+    for x in (randn(g, 4, 6, 1, 96).transpose(1, 2), randn(g, 6, 1, 1, 96).transpose(0, 2), randn(g, 5, 2, 1, 3, 96).transpose(1, 2)):
+        assert x.is_contiguous()
+        check_norm(ops().layer_norm(x, w, b), x, w, b, 1e-5)
+        dy = randn(g, *x.shape)
+        check_grads(ops().layer_norm_backward(dy, x, w, add=x), grad_ref(dy, x, w.double(), 1e-5, x, False))
+
+
 def test_norm_hard_rows():
     """A large mean, constant rows, tiny and large values; a row that is not finite stays alone."""
     g = gen(13)

@@ -187,3 +187,20 @@ def test_linear_workspace_only_for_rows_off_16_bytes():
     assert need(1, 7, 63, 63, 64) == 0  # a single row has no stride
     assert need(1, 7, 64, 64, 64, x=4098) == 64 * 2
     assert need(0, 7, 63, 63, 63) == 0 and need(5, 7, 0, 0, 0) == 0
+
+
+@pytest.mark.parametrize("x", [torch.zeros(4, 6, 1, 8).transpose(1, 2), torch.zeros(4, 1, 6, 8), torch.zeros(6, 1, 1, 8).transpose(0, 2),
+                               torch.zeros(2, 3, 5, 8), torch.zeros(5, 2, 1, 3, 8).transpose(1, 2)])
+def test_norm_rows_of_many_dims_are_where_torch_has_them(monkeypatch, x):
+    """A dim of one may have any stride and leaves a tensor contiguous: the rows the kernels walk over are the tensor's."""
+    packed = []
+    monkeypatch.setattr(ops, "_cuda", lambda *ts: None)
+    monkeypatch.setattr(ops, "_launch", lambda index, entry, flops, nbytes, args: packed.append(args))
+    ops.layer_norm(x)
+    ops.layer_norm_backward(x, x, add=x, sums=False)
+    want = (torch.arange(x.numel()).view(-1, 8)[:, 0]).tolist()  # contiguous: row r starts at 8 r
+    for raw in packed:
+        a = _lib.FbLayerNormArgs.from_buffer_copy(raw)
+        for outer, inner in ((a.x_outer_stride, a.x_inner_stride), (a.dy_outer_stride, a.dy_inner_stride),
+                             (a.add_outer_stride, a.add_inner_stride)) if a.dy else ((a.x_outer_stride, a.x_inner_stride),):
+            assert [o * outer + i * inner for o in range(a.outer) for i in range(a.inner)] == want

@@ -251,7 +251,8 @@ int32_t fb_rope_axes(const fb_rope_args* args, void* stream);
  *   g = dy * w,  dx = (g - mean(g) - xhat * mean(g * xhat)) / sqrt(var + eps) [+ add],
  *   dweight = sum of dy * xhat,  dbias = sum of dy   (fp32 [dim], or [outer, dim] with sum_per_outer; both or neither),
  * summed in a fixed order through `work` (fb_layer_norm_work_floats floats). dx has x's type. A weight per outer index
- * has its sums per outer index, of which there are at most 65535. */
+ * has its sums per outer index, of which there are at most 65535. out overlaps no input, but dx may be add with add's
+ * strides. At most 2^30 rows of at most 2^30 elements. */
 typedef struct fb_layer_norm_args {
   const void* x; int64_t x_outer_stride, x_inner_stride;
   const void* dy; int64_t dy_outer_stride, dy_inner_stride;        /* backward */
@@ -282,8 +283,9 @@ enum fb_act {
 
 /* out = act(x w^T + bias) + residual, on the fp32 accumulator with one rounding: x [m, k] and w [n, k] both bf16 or both
  * fp16, bias [n] of their type or NULL, residual [m, n] of their type or fp32 or NULL, out of their type or fp32; unit
- * stride along the last dim, row strides in elements, any m, n and k >= 0. residual may be out. x or w whose rows do
- * not start on 16 bytes is copied to `work` first (fb_linear_act_work_bytes bytes, 16-byte aligned; 0 when both do). */
+ * stride along the last dim, row strides in elements, any m, n and k >= 0 (up to 2^30). residual may be out, with its
+ * type and strides; no other overlap is allowed. x or w whose rows do not start on 16 bytes is copied to `work` first
+ * (fb_linear_act_work_bytes bytes, 16-byte aligned; 0 when both do). */
 typedef struct fb_linear_act_args {
   const void* x; int64_t ldx;
   const void* w; int64_t ldw;

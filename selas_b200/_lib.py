@@ -170,8 +170,17 @@ def _format(t) -> str:
 def packer(t):
     """A function that lays its arguments out as the C struct of the ctypes Structure ``t``, field after field (arrays
     and inner structs spread out, 0 for a null pointer), as bytes: the struct to pass to the library. One call costs a
-    fraction of setting the fields of a Structure one by one, which for small launches is most of the call."""
-    return struct.Struct("=" + _format(t)).pack
+    fraction of setting the fields of a Structure one by one, which for small launches is most of the call. A value that
+    its field cannot hold is a FluxB200Error."""
+    pack = struct.Struct("=" + _format(t)).pack
+
+    def packed(*values) -> bytes:
+        try:
+            return pack(*values)
+        except (struct.error, OverflowError) as e:
+            raise FluxB200Error(f"{t.__name__}: a size or value is out of range ({e})") from None
+
+    return packed
 
 
 pack_rope = packer(FbRopeArgs)

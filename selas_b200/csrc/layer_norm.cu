@@ -925,6 +925,7 @@ int launch_layer_norm(const fb_layer_norm_args& p, bool bwd, cudaStream_t st, st
     return code;
   };
   if (p.outer < 0 || p.inner < 0 || p.dim < 1) return bad(FB_ERR_ARG, "need outer, inner >= 0 and dim >= 1");
+  if (p.dim > (1 << 30)) return bad(FB_ERR_UNSUPPORTED, "at most 2^30 elements per row");
   if (!norm::is_dtype(p.x_dtype) || !norm::is_dtype(p.y_dtype) || !norm::is_dtype(p.w_dtype))
     return bad(FB_ERR_ARG, "dtypes must be FB_F32, FB_F16 or FB_BF16");
   if (!(p.eps >= 0.0f)) return bad(FB_ERR_ARG, "eps must be >= 0");
@@ -950,6 +951,7 @@ int launch_layer_norm(const fb_layer_norm_args& p, bool bwd, cudaStream_t st, st
     return FB_OK;
   }
   if (!p.x || !p.out || (bwd && !p.dy)) return bad(FB_ERR_ARG, "null pointer");
+  if (p.out == p.x || (bwd && p.out == p.dy)) return bad(FB_ERR_ARG, "out must not be x or dy");  // rows may be read again
   if (norm::misaligned(p.x, p.x_dtype) || norm::misaligned(p.out, bwd ? p.x_dtype : p.y_dtype) ||
       (bwd && (norm::misaligned(p.dy, p.y_dtype) || (p.add && norm::misaligned(p.add, p.x_dtype)))) ||
       (p.weight && norm::misaligned(p.weight, p.w_dtype)) || (p.bias && norm::misaligned(p.bias, p.w_dtype)) ||

@@ -1011,6 +1011,7 @@ int launch_linear_act(const fb_linear_act_args& p, cudaStream_t st, std::string&
     return code;
   };
   if (p.m < 0 || p.n < 1 || p.k < 0) return bad(FB_ERR_ARG, "need m >= 0, n >= 1, k >= 0");
+  if (p.m > (1 << 30) || p.n > (1 << 30) || p.k > (1 << 30)) return bad(FB_ERR_UNSUPPORTED, "m, n and k are at most 2^30");
   if (p.dtype != FB_BF16 && p.dtype != FB_F16) return bad(FB_ERR_UNSUPPORTED, "x and w must be FB_BF16 or FB_F16");
   if (p.out_dtype != p.dtype && p.out_dtype != FB_F32) return bad(FB_ERR_UNSUPPORTED, "out is of x's type or FB_F32");
   if (p.residual && p.residual_dtype != p.dtype && p.residual_dtype != FB_F32)

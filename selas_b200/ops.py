@@ -648,6 +648,7 @@ def ln_mod_backward(dy: torch.Tensor, x: torch.Tensor, scale: torch.Tensor, *, a
     index = _one_device("ln_mod_backward", x, dy, scale, add)
     _need(x.dtype == F32 and x.dim() == 3, "ln_mod_backward: x must be fp32 [B, L, D]")
     b, _, d = x.shape
+    _need(scale.dim() in (2, 3), "ln_mod_backward: scale must be bf16 [B, D] or [B, 1, D]")
     sc, stride = _mod_rows(scale, b, d)
     rows = sc.shape[0]
     dx, dscale, dshift = _norm_backward("ln_mod_backward", index, dy, x, 1e-6, sc.data_ptr(), _lib.FB_BF16, stride, 1, add,
@@ -700,7 +701,7 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = Non
     code = _DTYPE_CODE[dt]
     r = ldr = b = res_code = 0
     if residual is not None:
-        if (residual.dtype != dt and residual.dtype != F32) or residual.shape[:-1] != lead or residual.shape[-1] != n:
+        if (residual.dtype != dt and residual.dtype != F32) or residual.shape != (*lead, n):
             _refuse("linear_act: residual must be [..., N] of x's type or fp32")
         residual, ldr = _rows(residual, m, n)
         r, res_code = residual.data_ptr(), _DTYPE_CODE[residual.dtype]

@@ -606,7 +606,7 @@ def test_c_entries_refuse():
     from selas_b200 import _lib
 
     lib = _lib.lib()
-    x = torch.zeros(64, 64, dtype=BF16, device=DEV)
+    x, y = torch.zeros(2, 64, 64, dtype=BF16, device=DEV)
 
     def linear(**kw):
         a = _lib.FbLinearActArgs()
@@ -618,7 +618,7 @@ def test_c_entries_refuse():
             setattr(a, f, v)
         return lib.fb_linear_act(ctypes.addressof(a), None)
 
-    for kw in (dict(m=-1), dict(n=0), dict(k=-1), dict(dtype=_lib.FB_F32), dict(out_dtype=_lib.FB_F16), dict(act=6), dict(x=None),
+    for kw in (dict(m=-1), dict(n=0), dict(k=-1), dict(m=(1 << 30) + 1), dict(n=(1 << 30) + 1), dict(k=(1 << 30) + 1), dict(dtype=_lib.FB_F32), dict(out_dtype=_lib.FB_F16), dict(act=6), dict(x=None),
                dict(out=None), dict(ldx=7), dict(ld_out=4), dict(ldx=9, k=9), dict(out=x.data_ptr() + 1),
                dict(residual=x.data_ptr(), ld_residual=4), dict(residual=x.data_ptr(), ld_residual=8, residual_dtype=_lib.FB_F16)):
         assert linear(**kw) != 0, kw
@@ -627,7 +627,8 @@ def test_c_entries_refuse():
 
     def norm(fn, **kw):
         a = _lib.FbLayerNormArgs()
-        a.x = a.out = a.dy = x.data_ptr()
+        a.x = a.dy = x.data_ptr()
+        a.out = y.data_ptr()
         a.outer, a.inner, a.dim = 1, 4, 64
         a.x_inner_stride = a.out_inner_stride = a.dy_inner_stride = 64
         a.x_dtype = a.y_dtype = a.w_dtype = _lib.FB_BF16
@@ -638,10 +639,10 @@ def test_c_entries_refuse():
 
     for fn in (lib.fb_layer_norm, lib.fb_layer_norm_backward):
         for kw in (dict(dim=0), dict(outer=-1), dict(x_dtype=3), dict(eps=-1.0), dict(eps=float("nan")), dict(x=None), dict(out=None),
-                   dict(x=x.data_ptr() + 1), dict(outer=1 << 20, inner=1 << 20)):
+                   dict(x=x.data_ptr() + 1), dict(outer=1 << 20, inner=1 << 20), dict(out=x.data_ptr()), dict(dim=(1 << 30) + 1)):
             assert norm(fn, **kw) != 0, kw
         assert fn(None, None) != 0
-    for kw in (dict(dy=None), dict(dweight=x.data_ptr()), dict(dweight=x.data_ptr(), dbias=x.data_ptr(), inner=4000),
+    for kw in (dict(dy=None), dict(dy=y.data_ptr()), dict(dweight=x.data_ptr()), dict(dweight=x.data_ptr(), dbias=x.data_ptr(), inner=4000),
                dict(dweight=x.data_ptr(), dbias=x.data_ptr(), outer=70000, inner=1, sum_per_outer=1)):
         assert norm(lib.fb_layer_norm_backward, **kw) != 0, kw
 
@@ -662,7 +663,7 @@ def test_c_entries_refuse():
         assert rope(**kw) != 0, kw
     assert lib.fb_rope_axes(None, None) != 0
     torch.cuda.synchronize()
-    assert not x.any()
+    assert not x.any() and not y.any()
 
 
 # ------------------------------------------------------------------------------------------ as they are used

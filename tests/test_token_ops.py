@@ -71,6 +71,14 @@ def test_packed_arguments_fill_the_struct(struct, pack, n):
     assert [int(v) for v in leaves(struct.from_buffer_copy(raw))] == list(range(1, n + 1))
 
 
+def test_values_that_no_field_holds_are_refused(no_launch):
+    wide = torch.zeros(1, dtype=BF16).expand(1 << 31, 1)
+    for call in (lambda: ops.layer_norm(X, eps=1e300), lambda: _lib.pack_linear_act(*(1 << 31,) * 18),
+                 lambda: ops.linear_act(torch.zeros(1, 0, dtype=BF16), wide[:, :0])):
+        with pytest.raises(FluxB200Error, match="out of range"):
+            call()
+
+
 def test_cpu_tensors_are_refused():
     x, w = torch.zeros(2, 8, dtype=BF16), torch.zeros(8, 8, dtype=BF16)
     ids = torch.zeros(2, 1)
@@ -125,6 +133,7 @@ W = torch.ones(8)
     ("x must be fp32", lambda: ops.ln_mod_backward(X, X.bfloat16(), torch.zeros(2, 8, dtype=BF16))),
     ("x must be fp32", lambda: ops.ln_mod_backward(X[0], X[0], torch.zeros(1, 8, dtype=BF16))),
     ("must be bf16", lambda: ops.ln_mod_backward(X, X, torch.zeros(2, 8))),
+    ("scale must be", lambda: ops.ln_mod_backward(torch.zeros(8, 2, 8), torch.zeros(8, 2, 8), torch.zeros(8, dtype=BF16))),
     ("batch does not match", lambda: ops.ln_mod_backward(X, X, torch.zeros(3, 8, dtype=BF16))),
 ])
 def test_norm_refuses(no_launch, match, call):
@@ -145,6 +154,7 @@ A, B = torch.zeros(3, 16, dtype=BF16), torch.zeros(8, 16, dtype=BF16)
     ("bias must be", lambda: ops.linear_act(A, B, torch.zeros(7, dtype=BF16))),
     ("residual must be", lambda: ops.linear_act(A, B, residual=torch.zeros(3, 8, dtype=F16))),
     ("residual must be", lambda: ops.linear_act(A, B, residual=torch.zeros(2, 8))),
+    ("residual must be", lambda: ops.linear_act(A[0], B, residual=torch.zeros(()))),
     ("at least one row", lambda: ops.linear_act(A, B[:0])),
 ])
 def test_linear_act_refuses(no_launch, match, call):

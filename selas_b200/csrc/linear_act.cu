@@ -19,6 +19,10 @@
 // 1.3e-5 of the result's norm), so an accumulator takes 1024 of K at most; the epilogue warps then add it to fp32
 // registers, which are the sum proper, while the other TMEM buffer takes the next 1024. That costs 2 % of the time at
 // most (every 512 cost 10 %) and holds the error of an fp32 output near 1e-6.
+//
+// Measured: 28 x 3072 x 18432 (m x k x n) 24.6 us, 4.6 TB/s of weight, which a kernel that only loads the weight by TMA
+// also takes; 4608 x 12288 x 3072 onto an fp32 residual 231 us, 1505 TFLOP/s, in a single call and 243 to 290 us back to
+// back under the power cap; 512 x 12288 x 3072 49 us; one row, 256 to 3072 features, 6.3 us.
 #include <atomic>
 #include <type_traits>
 

@@ -9,9 +9,10 @@
 // Angles: phi / 2 pi is formed in 64 bits (one multiply by omega / 2 pi, minus its nearest whole number), which
 // keeps positions of millions exact to ~1e-9 turns, and only the fraction in [-1/2, 1/2] goes to sincospif in 32 bits.
 //
-// Bound: HBM, every element read once and written once. A group of threads owns a token and up to twelve of its heads, of q and
-// of k alike: each thread keeps the sines and cosines of its own slots in registers for all of them, so no table is read
-// from memory.
+// Bound: HBM, every element read once and written once. A group of threads owns a token and up to twelve of its heads, of q
+// and of k alike: each thread keeps the sines and cosines of its own slots in registers for all of them, so no table is read
+// from memory. Measured (q and k of 24 heads x 128 in bf16): 61440 tokens, 1.51 GB, 229 us = 6.6 TB/s, the speed of a copy;
+// 4608 tokens read in place from a fused projection, 113 MB, 22.5 us, of which a copy of that layout takes 22 to 25 too.
 #include "fb_internal.h"
 
 namespace fb {

@@ -11,7 +11,8 @@
 // next rows are on their way to shared memory meanwhile, each thread's elements to places that only it reads. The
 // column sums dw and db stay in registers too (a thread owns the same columns of every row it takes), are joined
 // across the block's groups in shared memory, and go out as one fp32 partial row per block; a second kernel adds the
-// partials in a fixed order, so results do not depend on the order in which blocks run.
+// partials in a fixed order, so results do not depend on the order in which blocks run. The blocks of a call with few rows
+// are a cluster instead, and add their sums over distributed shared memory in order of rank.
 //
 // Measured: forward 18432 x 3072 fp32 to bf16 57 us (5.9 TB/s), 65537 x 768 bf16 41 us (4.9); backward 65537 x 1280 bf16
 // 95 us (5.3), 18432 x 3072 fp32 with bf16 dy 105 us (5.4), 4608 x 3072 fp32 with the adaLN scale and add 43.5 us (4.6; ten
@@ -23,6 +24,7 @@
 namespace fb {
 namespace norm {
 
+constexpr int kMaxCluster = 8;      // blocks of a portable cluster
 constexpr int kMaxDimRegs = 16384;  // the widest row that a group of 1024 threads holds in registers
 
 struct Args {
@@ -38,6 +40,7 @@ struct Args {
   int x_type, y_type, w_type;              // fb_dtype; y_type: y (forward) or dy
   int depth, stage_bytes;                  // rows on their way to shared memory, and the bytes of one
   int add_staged;                          // add is one of what comes that way
+  int cluster;                             // the blocks of a sum group are a cluster and join their sums themselves
   float w_plus;                            // w is read as w_plus + w (1 for adaLN's scale)
   float eps;
 };
@@ -69,6 +72,12 @@ __device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
   f2 d;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
   return d;
+}
+// A pair of another block of the cluster, at its own shared-memory address there.
+__device__ __forceinline__ f2 ld_cluster2(uint32_t addr, int rank) {
+  f2 v;
+  asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(v) : "r"(mapa_shared(addr, rank)) : "memory");
+  return v;
 }
 __device__ __forceinline__ float total(f2 v) {
   const float2 r = unpack2(v);
@@ -583,8 +592,38 @@ __global__ void __launch_bounds__(bwd_threads(GT, NCH* CH), 1) bwd_kernel(const 
         }
       }
     }
-    if (group != 0) return;
   }
+  if (a.cluster) {
+    // The blocks' sums, added in order of rank by the blocks alike, each its share of the columns.
+    constexpr int PAIRS = P * GT;
+    f2* sums = reinterpret_cast<f2*>(ring);  // [dw, db][pair]
+    __syncthreads();                         // nobody reads the ring any more
+    if (group == 0) {
+#pragma unroll
+      for (int k = 0; k < P; ++k) sums[k * GT + t] = dw[k], sums[PAIRS + k * GT + t] = db[k];
+    }
+    __syncwarp();
+    cluster_sync_all();
+    for (int q = blockIdx.x * T + threadIdx.x; q < 2 * PAIRS; q += gridDim.x * T) {
+      const uint32_t at = smem_u32(sums + q);
+      f2 part[kMaxCluster];
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r) part[r] = ld_cluster2(at, min(r, static_cast<int>(gridDim.x) - 1));
+      f2 v = part[0];
+#pragma unroll
+      for (int r = 1; r < kMaxCluster; ++r)
+        if (r < gridDim.x) v = add2(v, part[r]);
+      const int p = q < PAIRS ? q : q - PAIRS, c0 = W::column(p % GT, p / GT * 2), c1 = W::column(p % GT, p / GT * 2 + 1);
+      float* d = (q < PAIRS ? a.dw : a.db) + static_cast<int64_t>(blockIdx.y) * a.dim;
+      const float2 s = unpack2(v);
+      if (FULL || c0 < a.dim) d[c0] = s.x;
+      if (FULL || c1 < a.dim) d[c1] = s.y;
+    }
+    __syncwarp();
+    cluster_sync_all();  // nobody reads this block's sums any more
+    return;
+  }
+  if (NG > 1 && group != 0) return;
   float *pw, *pb;
   if (gridDim.x == 1) {
     pw = a.dw + static_cast<int64_t>(blockIdx.y) * a.dim;
@@ -742,12 +781,23 @@ static int most_fwd(int dim, int x_type) { return x_type != FB_F32 && dim <= 819
 static int most_bwd(int dim) { return dim <= 10240 ? 40 : 20; }
 static int elements(int dim, int gt, bool vec) { return vec ? 4 * ((dim + 4 * gt - 1) / (4 * gt)) : gt < 32 ? 8 : 16; }
 
+// Rows per group of threads up to which a sum group's rows go to one cluster of up to eight blocks, which joins its sums
+// without a second launch. Measured, partial rows and a second launch against a cluster, bf16: 77 x 768 a call 16.9 / 14.7 us
+// (device 10.3 / 10.0), 8 x 12288 22.1 / 16.4 on the device; at three rows per group the longer walk costs what the join
+// saved (256 x 768 12.3 / 14.3).
+constexpr int kClusterSteps = 2;
 // Blocks per sum group of the backward pass: the SMs shared out over the groups, fewer where there are fewer rows than
 // groups of threads.
-static int64_t bwd_blocks(int64_t rows, int dim, int64_t sum_groups, bool vec) {
+struct Blocks {
+  int64_t n;
+  bool cluster;
+};
+static Blocks bwd_blocks(int64_t rows, int dim, int64_t sum_groups, bool vec, bool sums) {
   const int gt = group_threads(dim, vec, most_bwd(dim)), ng = bwd_threads(gt, elements(dim, gt, vec)) / gt;
   const int64_t need = std::max<int64_t>(1, (rows + ng - 1) / ng);
-  return std::max<int64_t>(1, std::min<int64_t>(need, kNumSms / std::max<int64_t>(1, sum_groups)));
+  const int64_t few = std::min<int64_t>(need, kMaxCluster);
+  if (sums && need > 1 && need <= kClusterSteps * kMaxCluster && sum_groups * few <= kNumSms / 2) return {few, true};
+  return {std::max<int64_t>(1, std::min<int64_t>(need, kNumSms / std::max<int64_t>(1, sum_groups))), false};
 }
 
 constexpr int kRingPerSm = 208 * 1024;  // shared memory of an SM that the rows on their way (and w) may take
@@ -778,23 +828,35 @@ static cudaError_t go_bwd(Args a, int64_t sum_groups, cudaStream_t st) {
     a.depth = std::max(1, std::min(4, (kRingPerSm - w_bytes) / a.stage_bytes));
     smem += a.depth * a.stage_bytes;
   }
-  smem = std::max(smem, NCH * CH * T * 4);  // after the walk, the groups' sums
-  const int64_t blocks = bwd_blocks(a.rows, a.dim, sum_groups, CH == 4);
-  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(sum_groups));
-  bwd_kernel<GT, NCH, CH, FULL><<<grid, T, smem, st>>>(a);
-  cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess && a.dw != nullptr && blocks > 1) {
+  const Blocks blocks = bwd_blocks(a.rows, a.dim, sum_groups, CH == 4, a.dw != nullptr);
+  a.cluster = blocks.cluster;
+  // after the walk, the groups' sums, then the block's
+  smem = std::max(smem, std::max(NCH * CH * T * 4, a.cluster ? NCH * CH * GT * 8 : 0));
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks.n), static_cast<unsigned>(sum_groups));
+  cfg.blockDim = dim3(T);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 0;
+  if (a.cluster) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(blocks.n);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.numAttrs = 1;
+  }
+  cudaError_t e = cudaLaunchKernelEx(&cfg, bwd_kernel<GT, NCH, CH, FULL>, a);
+  if (e == cudaSuccess && a.dw != nullptr && blocks.n > 1 && !a.cluster) {
     // launched while the last blocks of the walk still run; it waits for them before it reads
-    cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>((2ll * a.dim + 31) / 32), static_cast<unsigned>(sum_groups));
     cfg.blockDim = dim3(1024);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cfg.dynamicSmemBytes = 0;
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, join_kernel, static_cast<const float*>(a.part), static_cast<int>(blocks), a.dim, a.dw, a.db);
+    e = cudaLaunchKernelEx(&cfg, join_kernel, static_cast<const float*>(a.part), static_cast<int>(blocks.n), a.dim, a.dw, a.db);
   }
   return e;
 }
@@ -918,8 +980,11 @@ int64_t layer_norm_work_floats(int64_t outer, int64_t inner, int32_t dim, int32_
   if (rows <= 0 || groups <= 0 || dim <= 0) return 0;
   if (dim > norm::kMaxDimRegs) return 2 * rows * groups;
   // which of the two layouts runs depends on alignments that are not known here: room for either
-  const int64_t blocks = std::max(norm::bwd_blocks(rows, dim, groups, false),
-                                  dim % 4 == 0 ? norm::bwd_blocks(rows, dim, groups, true) : 1);
+  int64_t blocks = 1;
+  for (int vec = 0; vec < (dim % 4 == 0 ? 2 : 1); ++vec) {
+    const norm::Blocks b = norm::bwd_blocks(rows, dim, groups, vec, true);
+    if (!b.cluster) blocks = std::max(blocks, b.n);
+  }
   return blocks > 1 ? groups * blocks * 2 * dim : 0;
 }
 

@@ -346,6 +346,20 @@ def test_norm_backward_sizes(dim, xt):
         check_grads(got, grad_ref(dy, x, w.double(), 1e-5, None, False))
 
 
+@pytest.mark.parametrize("dim", [8, 64, 100, 250, 768, 1000, 2049, 3072, 6144, 12288, 16384])
+def test_norm_backward_few_rows(dim):
+    """Sums of two rows to many, of one image and of several: one block, the blocks of a cluster, a partial row of sums per
+    block. Without the sums dx has the same bits."""
+    g = gen(23)
+    for b, l in ((1, 2), (1, 5), (1, 9), (1, 20), (1, 33), (1, 64), (1, 129), (1, 260), (2, 7), (5, 13), (9, 8), (9, 20), (17, 40), (40, 3)):
+        x, dy = randn(g, b, l, dim, mean=0.3), randn(g, b, l, dim, dtype=BF16)
+        s = randn(g, b, dim, std=0.3, dtype=BF16)
+        got = ops().ln_mod_backward(dy, x, s)
+        ref = grad_ref(dy, x, 1.0 + s.double()[:, None], 1e-6, None, True)
+        check_grads((got[0], got[2], got[1]), ref)
+        assert torch.equal(ops().ln_mod_backward(dy, x, s, sums=False)[0], got[0])
+
+
 @pytest.mark.parametrize("xt", [F32, BF16, F16])
 @pytest.mark.parametrize("yt", [F32, BF16, F16])
 @pytest.mark.parametrize("wt", [F32, BF16, F16, None])

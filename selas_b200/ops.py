@@ -554,8 +554,8 @@ def _norm_vector(what: str, name: str, d: int, t: torch.Tensor) -> tuple[int, in
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5,
                *, out_dtype: torch.dtype | None = None) -> torch.Tensor:
-    """(x - mean) / sqrt(var + eps) * weight + bias over the last dim of x [..., D] (fp32, bf16 or fp16; rows may be
-    strided), statistics in fp32, rounded once to ``out_dtype`` (x's by default). weight and bias: [D] of one type, or
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last dim of x [..., D] (fp32, bf16 or fp16; rows of up
+    to three dims may be strided, a tensor of more is contiguous), statistics in fp32, rounded once to ``out_dtype`` (x's by default). weight and bias: [D] of one type, or
     None. Returns a contiguous tensor."""
     index = _one_device("layer_norm", x, weight, bias)
     outer, inner, d, code = _norm_rows("layer_norm", x)

@@ -1048,7 +1048,9 @@ int launch_linear_act(const fb_linear_act_args& p, cudaStream_t st, std::string&
   // 8192 x 1024 x 1024 26.8 / 20.7, 4608 x 3072 x 3072 82 / 60; up to 128 rows few_kernel's one token tile is never worse.
   // With many tiles and little K it is the epilogue that counts, which many_kernel overlaps (2000 x 100 x 17000 79 / 70;
   // with outputs written one by one, 17001, it is the slower of the two, 126 / 182).
-  const bool many_rows = p.m > 128 && (static_cast<double>(p.m) * p.n * p.k >= 4294967296.0 || (a.vec && tiles_many >= kNumSms));
+  // Without depth (k = 0) there are no tensor maps, which many_kernel would prefetch: few_kernel then touches none.
+  const bool many_rows =
+      p.k > 0 && p.m > 128 && (static_cast<double>(p.m) * p.n * p.k >= 4294967296.0 || (a.vec && tiles_many >= kNumSms));
   const int bt = many_rows ? 128 : p.m <= 16 ? 16 : p.m <= 32 ? 32 : p.m <= 64 ? 64 : 128;
   if (p.k > 0) {
     const void *x = p.x, *w = p.w;

@@ -317,12 +317,6 @@ __device__ __forceinline__ void finish_share(const Args& a, uint32_t base, int c
   }
 }
 
-// A barrier of the cluster that orders no memory: enough where what was read has been used (with release semantics it
-// would also wait for the outputs to reach L2).
-__device__ __forceinline__ void cluster_sync_relaxed() {
-  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-}
-
 // Adds NC accumulator columns at `taddr` (this warp's 32 lanes) to v; the first time they are the sum.
 template <int NC, int CW>
 __device__ __forceinline__ void promote(uint32_t taddr, bool first, float (&v)[NC]) {
@@ -523,7 +517,7 @@ __global__ void __launch_bounds__(Few<BT>::kThreads, 2) few_kernel(const __grid_
   finish_share<ACT, C::kWarps, kFeat, false>(a, smem_u32(tile), 0, BT, t0, j0, j1, f0, whole, b, warp, lane, a.splits, 0, 1);
   __syncwarp();
   if (a.splits > 1) {
-    cluster_sync_relaxed();  // nobody reads this CTA's tile any more
+    cluster_sync_all();  // nobody reads this CTA's tile any more: it may exit
   } else {
     __syncthreads();
   }
@@ -715,8 +709,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
     }
     if constexpr (SPLIT) {
       __syncwarp();
-      cluster_sync_all();      // the partial sums are in shared memory
-      cluster_sync_relaxed();  // and have been read
+      cluster_sync_all();  // the partial sums are in shared memory; the barrier before the exit: they have been read
     }
   } else {
     reg_alloc<kEpiRegs>();
@@ -778,8 +771,6 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
                                                     live * (split + 1) / a.splits, f0, whole, lane_bias(a, f0, whole, lane),
                                                     warp - 4, lane, a.splits, rank, 2);
         }
-        __syncwarp();
-        cluster_sync_relaxed();
         break;
       }
       if (!ok) break;
@@ -834,7 +825,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
   }
   tc_fence_before_sync();
   __syncthreads();
-  cluster_sync_all();  // the peer no longer signals this CTA and nobody reads this CTA's TMEM
+  cluster_sync_all();  // the peer no longer signals this CTA; nobody reads this CTA's TMEM, or its partial sums
   if (warp == 1) {
     tc_fence_after_sync();
     tmem_dealloc_pair(tmem_base, kTmemCols);

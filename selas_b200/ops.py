@@ -608,14 +608,14 @@ def _norm_backward(what: str, index: int, dy, x, eps: float, weight: int, w_code
     pw = pb = work = need = 0
     per_outer = 1 if groups > 1 else 0
     if sums:
-        # the two gradients and the partial sums in one allocation
+        # each gradient has storage of its own: it may be kept or saved, and the partial sums not with it
         need = _norm_work(outer, inner, d, per_outer)
-        n = groups * d
-        buf = x.new_empty(2 * n + need, dtype=F32)
-        shape, strides = ((d,), (1,)) if flat else ((groups, d), (d, 1))
-        dw, db = buf.as_strided(shape, strides, 0), buf.as_strided(shape, strides, n)
-        pw = buf.data_ptr()
-        pb, work = pw + 4 * n, pw + 8 * n
+        shape = (d,) if flat else (groups, d)
+        dw, db = x.new_empty(shape, dtype=F32), x.new_empty(shape, dtype=F32)
+        pw, pb = dw.data_ptr(), db.data_ptr()
+        if need:
+            partial = x.new_empty(need, dtype=F32)
+            work = partial.data_ptr()
     rows = outer * inner
     if rows or (sums and groups):
         nbytes = rows * d * ((2 if add is None else 3) * (4 if code == _lib.FB_F32 else 2) + (4 if y_code == _lib.FB_F32 else 2))

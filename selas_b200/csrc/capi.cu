@@ -75,9 +75,6 @@ DeviceState* current_device(std::string& err) {
   }
   std::string msg = gemm_setup();
   if (msg.empty()) msg = attention_setup();
-  if (msg.empty()) msg = linear_act_setup();
-  if (msg.empty()) msg = layer_norm_setup();
-  if (msg.empty()) msg = rope_axes_setup();
   if (!msg.empty()) {
     err = msg;
     return nullptr;
@@ -102,6 +99,36 @@ DeviceState* current_device(std::string& err) {
   s.sm_count = sms;
   s.ready.store(true, std::memory_order_release);
   return &s;
+}
+
+DeviceState* device_for(Operator op, std::string& err) {
+  DeviceState* s = current_device(err);
+  if (!s) return nullptr;
+  std::atomic<bool>& ready = s->operator_ready[static_cast<int>(op)];
+  if (ready.load(std::memory_order_acquire)) return s;
+  std::lock_guard<std::mutex> lock(g_dev_mu);
+  if (ready.load(std::memory_order_relaxed)) return s;
+  // The first call may be one that a stream captures. Set-up enqueues nothing, but loads kernels, which a capture in its
+  // default mode may forbid this thread.
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) {
+    err = std::string("cudaThreadExchangeStreamCaptureMode: ") + cudaGetErrorString(e);
+    return nullptr;
+  }
+  std::string msg;
+  switch (op) {
+    case Operator::kLinearAct: msg = linear_act_setup(); break;
+    case Operator::kLayerNorm: msg = layer_norm_setup(); break;
+    default: msg = rope_axes_setup(); break;
+  }
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (!msg.empty()) {
+    err = msg;
+    return nullptr;
+  }
+  ready.store(true, std::memory_order_release);
+  return s;
 }
 
 }  // namespace fb

@@ -17,6 +17,9 @@ namespace fb {
 
 constexpr int kNumSms = 148;
 
+// Operators that set themselves up on their first call on a device (device_for).
+enum class Operator { kLinearAct, kLayerNorm, kRopeAxes, kCount };
+
 // Per-device state resolved once by fb_init / ensure_device.
 struct DeviceState {
   int* status = nullptr;  // device status word (fb_device_code)
@@ -27,10 +30,14 @@ struct DeviceState {
   int* splitk_count = nullptr;
   // set (release) after every field above is filled; the unlocked fast path reads it with acquire
   std::atomic<bool> ready{false};
+  // which operators have been set up on this device
+  std::atomic<bool> operator_ready[static_cast<int>(Operator::kCount)] = {};
 };
 
 // Returns the state of the current device (initialising it on first use), or nullptr with `err` set.
 DeviceState* current_device(std::string& err);
+// The same with `op` set up on the device; where that fails, calls of this operator are refused and no others.
+DeviceState* device_for(Operator op, std::string& err);
 
 // cuTensorMapEncodeTiled, resolved through the runtime's driver entry point (no libcuda link).
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -84,7 +91,8 @@ int64_t layer_norm_work_floats(int64_t outer, int64_t inner, int32_t dim, int32_
 int launch_linear_act(const fb_linear_act_args& args, cudaStream_t st, std::string& err);
 int64_t linear_act_work_bytes(const fb_linear_act_args& args);
 
-// One-time kernel attribute set-up (dynamic shared memory limits); returns an error string or "".
+// Kernel attribute set-up (dynamic shared memory limits), once per device; returns an error string or "". The first two
+// run with the device's initialisation, the others on their operator's first call (device_for).
 std::string gemm_setup();
 std::string attention_setup();
 std::string linear_act_setup();

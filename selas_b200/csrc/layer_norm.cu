@@ -1028,7 +1028,7 @@ int launch_layer_norm(const fb_layer_norm_args& p, bool bwd, cudaStream_t st, st
       norm::misaligned(p.dweight, FB_F32) || norm::misaligned(p.dbias, FB_F32) || norm::misaligned(p.work, FB_F32))
     return bad(FB_ERR_ALIGN, "a pointer is not aligned to its elements");
   std::string derr;
-  if (!current_device(derr)) {  // raises the kernels' shared-memory limits on this device
+  if (!device_for(Operator::kLayerNorm, derr)) {  // raises the kernels' shared-memory limits on this device
     err = derr;
     return FB_ERR_INIT;
   }

@@ -1021,7 +1021,7 @@ int launch_linear_act(const fb_linear_act_args& p, cudaStream_t st, std::string&
   if (!align(p.x, 2) || !align(p.w, 2) || !align(p.bias, 2) || !align(p.out, osz) || (p.residual && !align(p.residual, rsz)))
     return bad(FB_ERR_ALIGN, "a pointer is not aligned to its elements");
   std::string derr;
-  DeviceState* dev = current_device(derr);
+  DeviceState* dev = device_for(Operator::kLinearAct, derr);
   if (!dev) {
     err = derr;
     return FB_ERR_INIT;

@@ -313,7 +313,7 @@ int launch_rope_axes(const fb_rope_args& p, cudaStream_t st, std::string& err) {
     }
   }
   std::string derr;
-  if (!current_device(derr)) {  // raises the kernels' shared-memory limits on this device
+  if (!device_for(Operator::kRopeAxes, derr)) {  // raises the kernels' shared-memory limits on this device
     err = derr;
     return FB_ERR_INIT;
   }

@@ -437,13 +437,14 @@ def _launch(index: int, entry: str, flops: float, nbytes: float, packed: bytes) 
 
 @functools.lru_cache(maxsize=64)
 def _rope_plan(axes_dim: tuple, theta) -> tuple:
-    """(head_dim, the C struct's theta and axes_dim arrays) for the axes' dims and bases."""
+    """(head_dim, the C struct's theta and axes_dim arrays) for the axes' dims and bases: whole numbers and floats, nothing
+    whose value could change under the cached plan."""
     n = len(axes_dim)
     thetas = theta if isinstance(theta, tuple) else (theta,) * n
     _need(1 <= n <= 8, "rope_axes: 1 to 8 axes")
     _need(len(thetas) == n, "rope_axes: theta is one base, or one per axis")
     pad = (0,) * (8 - n)
-    return sum(axes_dim), (*(float(t) for t in thetas), *pad, *(int(d) for d in axes_dim), *pad)
+    return sum(axes_dim), (*thetas, *pad, *axes_dim, *pad)
 
 
 def _rope(q: torch.Tensor, k: torch.Tensor | None, ids: torch.Tensor, axes_dim, theta, pairs: str, inverse: bool):
@@ -453,8 +454,15 @@ def _rope(q: torch.Tensor, k: torch.Tensor | None, ids: torch.Tensor, axes_dim, 
     if code is None or q.dim() != 4:
         _refuse("rope_axes: fp32, bf16 or fp16 [B, H, L, hd] tensors")
     b, h, l, hd = q.shape
-    axes_dim = tuple(axes_dim)
-    total, arrays = _rope_plan(axes_dim, tuple(theta) if isinstance(theta, (tuple, list)) else theta)
+    try:
+        axes_dim = tuple(axes_dim)
+        dims = tuple(map(int, axes_dim))
+        bases = tuple(map(float, theta)) if isinstance(theta, (tuple, list)) else float(theta)
+    except (TypeError, ValueError, OverflowError):
+        _refuse("rope_axes: axes_dim is a sequence of whole numbers, theta one base, or one per axis")
+    if dims != axes_dim:
+        _refuse(f"rope_axes: the axes' dims must be whole numbers, got {axes_dim}")
+    total, arrays = _rope_plan(dims, bases)
     if hd != total:
         _refuse(f"rope_axes: the axes' dims {axes_dim} must add up to head_dim {hd}")
     order = _PAIRS.get(pairs)

@@ -69,7 +69,8 @@ template <int ACT>
 __device__ __forceinline__ float activate(float z) {
   if constexpr (ACT == FB_ACT_RELU) return z < 0.f ? 0.f : z;  // keeps a NaN
   if constexpr (ACT == FB_ACT_GELU) {
-    const float s = fminf(fabsf(z), 30.f);  // past 30 nothing is left of erfc; keeps inf * 0 out
+    // |z|, up to 30 where z > 0: nothing is left of erfc there, and +inf * 0 stays out. -inf gives NaN as z/2 * (1 + erf) does.
+    const float s = fmaxf(-z, fminf(z, 30.f));
     const float t = rcp_approx(fmaf(0.3275911f * 0.70710678f, s, 1.0f));
     float h = fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
     h = fmaf(h, t, 0.5f * 1.421413741f);

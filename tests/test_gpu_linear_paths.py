@@ -72,3 +72,38 @@ def test_no_depth_needs_no_tensor_map(m, n):
     assert [k for k, _, _ in launches(call)] == ["few_kernel"]
     assert torch.equal(call(), b.float().clamp_min(0) + r)
     assert not ops().linear_act(x, w).any()
+
+
+def act_ref(z, act):
+    if act == "relu":
+        return torch.where(z < 0, 0.0, z)
+    if act == "gelu":
+        return 0.5 * z * torch.erfc(-z / math.sqrt(2))
+    if act == "gelu_tanh":
+        return 0.5 * z * (1 + torch.tanh(math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3)))
+    if act == "quick_gelu":
+        return z * torch.sigmoid(1.702 * z)
+    if act == "silu":
+        return z * torch.sigmoid(z)
+    return z
+
+
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "gelu_tanh", "quick_gelu", "silu"])
+@pytest.mark.parametrize("m,n,kernel", [(20, 40, "few_kernel"), (300, 20000, "many_kernel")])
+def test_activations_of_infinities(act, m, n, kernel):
+    """Pre-activations that are infinite, NaN or far out give what the formula gives: NaN where it is inf * 0 or inf - inf.
+    With one value per feature times one the pre-activation is exact. An exp that is off by (2 + 1.2 |x|) 2^-23, a
+    division by 2^-22 and an erfc by 1.5e-7 move a result by less than 2^-21 |z|; what __fdividef drops is below 1e-36."""
+    vals = torch.tensor([-math.inf, math.inf, math.nan, -1e30, 1e30, -3e4, 3e4, -100, 100, -88.5, 88.5, -30, 30, -9, -5, -3, -1, -0.25, 0, 1, 5], device=DEV)
+    x, w = torch.zeros(m, 8, dtype=BF16, device=DEV), torch.zeros(n, 8, dtype=BF16, device=DEV)
+    x[:, 0] = 1
+    w[:, 0] = vals[torch.arange(n, device=DEV) % len(vals)].to(BF16)
+    call = lambda: ops().linear_act(x, w, None, act, out_dtype=F32)  # noqa: E731
+    assert [k for k, _, _ in launches(call)] == [kernel]
+    got, z = call().double(), w[:, 0].double()
+    ref = act_ref(z, act)
+    assert torch.equal(got.isnan(), ref.isnan().expand(m, n)), (got[0, :21].tolist(), ref[:21].tolist())
+    infinite = lambda t: torch.where(t.isinf(), t.sign(), 0.0)  # noqa: E731
+    assert torch.equal(infinite(got), infinite(ref).expand(m, n))
+    ok = ref.isfinite()
+    assert ((got - ref).abs()[:, ok] <= (z.abs() * 2.0 ** -21 + 1e-36)[ok]).all()

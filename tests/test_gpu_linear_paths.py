@@ -107,3 +107,130 @@ def test_activations_of_infinities(act, m, n, kernel):
     assert torch.equal(infinite(got), infinite(ref).expand(m, n))
     ok = ref.isfinite()
     assert ((got - ref).abs()[:, ok] <= (z.abs() * 2.0 ** -21 + 1e-36)[ok]).all()
+
+
+# ------------------------------------------------------------------------------------------ large products
+#
+# Elementwise bounds, with u = 2^-24 and S the sum of magnitudes |x||w|: an accumulator takes 1024 of K, 16 at a time, each
+# step off by at most 2^-22 S; its sum is then added in fp32, one rounding per 1024 of K, and partial sums of a shared K are
+# added likewise: (min(K, 1024) / 16 + K / 1024 + 8) 2^-22 S, carried through the activation (slope at most 1.13), which
+# itself is off by 2^-21 |z| (see above), and two roundings of the sum with the residual.
+
+
+def randn(g, *shape, dtype=F32, std=1.0):
+    return (torch.randn(*shape, generator=g, device=DEV) * std).to(dtype)
+
+
+class Product:
+    """x [m, k], w [n, k], bias and the sums in 64 bits."""
+
+    def __init__(self, m, n, k, dt, seed=1):
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        self.k, self.dt = k, dt
+        self.x, self.w, self.b = randn(g, m, k, dtype=dt), randn(g, n, k, dtype=dt, std=1 / math.sqrt(k)), randn(g, n, dtype=dt)
+        self.res = {None: None, dt: randn(g, m, n, dtype=dt), F32: randn(g, m, n)}
+        self.z = self.x.double() @ self.w.double().t()
+        self.s = self.x.double().abs() @ self.w.double().abs().t()
+
+    def call(self, act="none", bias=True, res=None, out=None):
+        return ops().linear_act(self.x, self.w, self.b if bias else None, act, self.res[res], out_dtype=out or self.dt)
+
+    def check(self, got, act="none", bias=True, res=None):
+        z, s = (self.z + self.b.double(), self.s + self.b.double().abs()) if bias else (self.z, self.s)
+        y = act_ref(z, act)
+        r = 0.0 if self.res[res] is None else self.res[res].double()
+        ref = y + r
+        slack = 1.13 * (min(self.k, 1024) / 16 + self.k / 1024 + 8) * 2.0 ** -22 * s + 2.0 ** -21 * z.abs() + 2.0 ** -23 * (y.abs() + abs(r))
+        half = ref.abs() * (torch.finfo(got.dtype).eps / 2) + (2.0 ** -25 if got.dtype == F16 else 0.0)
+        assert got.shape == ref.shape and torch.isfinite(got).all()
+        worst = ((got.double() - ref).abs() / (slack * (1 + torch.finfo(got.dtype).eps) + half + 1e-36)).max().item()
+        assert worst <= 1.0, f"{act} bias={bias} residual={res} out={got.dtype}: {worst:.3f} of the bound"
+
+
+# (m, n, k), the CTAs that share a tile (2: a pair, each tile by itself; more: pairs that share its K; how many fit at once
+# depends on how the GPU's SMs are grouped). Rows and columns past the last whole tile, K past the last whole step, columns
+# that are no multiple of four (each output by itself), more tiles than pairs, fewer than pairs.
+PERSISTENT = [((2601, 4004, 424), (2,)), ((2601, 4003, 424), (2,)), ((2000, 17000, 100), (2,)), ((1500, 9001, 2100), (2,))]
+SHARED = [((500, 1020, 8456), (8,)), ((500, 1019, 8456), (8,)), ((1153, 1000, 3736), (4, 6)), ((1000, 2044, 2104), (4,)), ((130, 4097, 8200), (6, 8))]
+
+
+@pytest.mark.parametrize("size,ctas", PERSISTENT + SHARED)
+@pytest.mark.parametrize("dt", [BF16, F16])
+def test_large_products(size, ctas, dt):
+    """The pair kernel with every activation, bias, residual and output type."""
+    p = Product(*size, dt)
+    for code, act in enumerate(("none", "relu", "gelu", "gelu_tanh", "quick_gelu", "silu")):
+        (kernel, (a, shared), cluster), = [v for v in launches(lambda: p.call(act)) if v[0] != "align_rows_kernel"]
+        assert (kernel, a, bool(shared)) == ("many_kernel", code, ctas[0] > 2) and cluster in ctas
+        for bias, res, out in ((True, F32, F32), (False, None, dt), (True, dt, dt), (False, F32, dt), (True, dt, F32), (True, None, F32)):
+            got = p.call(act, bias, res, out)
+            assert got.dtype == out
+            p.check(got, act, bias, res)
+
+
+LARGE = [(2601, 4004, 424), (2601, 4003, 424), (500, 1020, 8456), (500, 1019, 8456)]
+
+
+@pytest.mark.parametrize("m,n,k", LARGE)
+def test_large_products_write_only_their_rows(m, n, k):
+    """Through the C entry, with a row stride of the output's own: what lies between the rows and after the last stays."""
+    import ctypes
+
+    from selas_b200 import _lib
+
+    p = Product(m, n, k, BF16)
+    for ld in (n + 4, n + 37):
+        out = torch.full((m + 3, ld), 7.0, dtype=BF16, device=DEV)
+        a = _lib.FbLinearActArgs()
+        a.x, a.ldx, a.w, a.ldw, a.bias = p.x.data_ptr(), k, p.w.data_ptr(), k, p.b.data_ptr()
+        a.out, a.ld_out, a.m, a.n, a.k = out.data_ptr(), ld, m, n, k
+        a.dtype, a.out_dtype, a.act = _lib.FB_BF16, _lib.FB_BF16, _lib.FB_ACT_NONE
+        call = lambda: _lib.check(_lib.lib().fb_linear_act(ctypes.addressof(a), torch.cuda.current_stream().cuda_stream), "fb_linear_act")  # noqa: E731
+        assert [v[0] for v in launches(call)] == ["many_kernel"]
+        call()
+        p.check(out[:m, :n])
+        assert (out[:m, n:] == 7).all() and (out[m:] == 7).all()
+
+
+@pytest.mark.parametrize("m,n,k", LARGE)
+def test_not_finite_stays_in_its_row_and_column_of_a_large_product(m, n, k):
+    p = Product(m, n, k, BF16)
+    clean = p.call("none", True, F32)
+    p.x[m - 1, 7] = float("nan")
+    p.w[n - 2, k - 1] = float("inf")
+    got = p.call("none", True, F32)
+    assert got[m - 1].isnan().all() and not torch.isfinite(got[:, n - 2]).any()
+    rows, cols = torch.arange(m, device=DEV) != m - 1, torch.arange(n, device=DEV) != n - 2
+    assert torch.equal(got[rows][:, cols], clean[rows][:, cols])
+
+
+def test_large_products_same_bits_on_streams_and_from_graphs():
+    """Several in flight at once on streams of their own, and two captured graphs replayed in turn after an input changed."""
+    ps = [Product(*size, BF16) for size in LARGE]
+    calls = [lambda p=p: p.call("silu", True, F32, F32) for p in ps]
+    first = [f() for f in calls]
+    for p, y in zip(ps, first):
+        p.check(y, "silu", True, F32)
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append([f() for f in calls])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for got in outs for a, b in zip(first, got))
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = [f() for f in calls]
+        graphs.append((g, out))
+    for k in range(3):
+        for p in ps:
+            p.x.mul_(1.25)
+        graphs[0][0].replay()
+        want = [f() for f in calls]
+        graphs[1][0].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for _, out in graphs for a, b in zip(out, want))

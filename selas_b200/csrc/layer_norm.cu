@@ -104,35 +104,44 @@ __device__ __forceinline__ void advance(Place& p, const Step& s, int inner) {
   if (p.i >= inner) p.i -= inner;
 }
 
-// CH consecutive elements (4: one vector access, 1: any alignment) widened to fp32.
-template <int CH>
+// CH consecutive elements (4: one vector access, 1: any alignment) widened to fp32. KEPT: nothing writes the tensor while the
+// kernel runs, so it may be read through the read-only path (not add, which dx may take the place of).
+template <bool KEPT, typename T>
+__device__ __forceinline__ T read(const T* p) {
+  if constexpr (KEPT) {
+    return __ldg(p);
+  } else {
+    return *p;
+  }
+}
+template <int CH, bool KEPT = true>
 __device__ __forceinline__ void load_chunk(const void* p, int type, int64_t at, float* f) {
   if (type == FB_F32) {
     const float* s = static_cast<const float*>(p) + at;
     if constexpr (CH == 4) {
-      const float4 v = __ldg(reinterpret_cast<const float4*>(s));
+      const float4 v = read<KEPT>(reinterpret_cast<const float4*>(s));
       f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
     } else {
-      f[0] = __ldg(s);
+      f[0] = read<KEPT>(s);
     }
   } else if (type == FB_BF16) {
     const uint16_t* s = static_cast<const uint16_t*>(p) + at;
     if constexpr (CH == 4) {
-      const uint2 u = __ldg(reinterpret_cast<const uint2*>(s));
+      const uint2 u = read<KEPT>(reinterpret_cast<const uint2*>(s));
       f[0] = __uint_as_float(u.x << 16), f[1] = __uint_as_float(u.x & 0xFFFF0000u);
       f[2] = __uint_as_float(u.y << 16), f[3] = __uint_as_float(u.y & 0xFFFF0000u);
     } else {
-      f[0] = bf16_bits_to_f32(__ldg(s));
+      f[0] = bf16_bits_to_f32(read<KEPT>(s));
     }
   } else {
     const __half* s = static_cast<const __half*>(p) + at;
     if constexpr (CH == 4) {
-      const uint2 u = __ldg(reinterpret_cast<const uint2*>(s));
+      const uint2 u = read<KEPT>(reinterpret_cast<const uint2*>(s));
       const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
       const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
       f[0] = lo.x, f[1] = lo.y, f[2] = hi.x, f[3] = hi.y;
     } else {
-      f[0] = __half2float(__ldg(s));
+      f[0] = __half2float(read<KEPT>(s));
     }
   }
 }
@@ -184,14 +193,14 @@ __device__ __forceinline__ void widen4(const uint8_t* p, int type, float* f) {
 
 // The elements of a row that one thread of its group holds: NCH chunks of CH, chunk c at column CH * (t + GT * c);
 // zeros past the end (FULL: the row ends with the last thread's last chunk). The type branch is outside the loop, so the loads of a row go out together.
-template <int GT, int NCH, int CH, bool FULL>
+template <int GT, int NCH, int CH, bool FULL, bool KEPT>
 __device__ __forceinline__ void load_row(const void* p, int type, int64_t base, int t, int dim, float (&f)[NCH * CH]) {
   auto each = [&](int ty) {
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
       const int col = CH * (t + GT * c);
       if ((FULL && GT >= 32) || col < dim) {  // small groups: dim is 0 for one without a row
-        load_chunk<CH>(p, ty, base + col, f + CH * c);
+        load_chunk<CH, KEPT>(p, ty, base + col, f + CH * c);
       } else {
 #pragma unroll
         for (int j = 0; j < CH; ++j) f[CH * c + j] = 0.f;
@@ -346,9 +355,10 @@ struct Walk {
 #pragma unroll
     for (int k = 0; k < P; ++k) v[k] = pack2(f[2 * k], f[2 * k + 1]);
   }
+  template <bool KEPT = true>
   static __device__ __forceinline__ void load(const void* p, int type, int64_t base, int t, int dim, f2 (&v)[P]) {
     float f[E];
-    load_row<GT, NCH, CH, FULL>(p, type, base, t, dim, f);
+    load_row<GT, NCH, CH, FULL, KEPT>(p, type, base, t, dim, f);
     pairs(f, v);
   }
   static __device__ __forceinline__ void take(const uint8_t* src, int type, int t, int dim, f2 (&v)[P]) {
@@ -549,7 +559,7 @@ __global__ void __launch_bounds__(bwd_threads(GT, NCH* CH), 1) bwd_kernel(const 
       if (CH == 4 && a.add_staged) {
         W::take(ma + stage * a.stage_bytes, a.x_type, t, dim, ad);
       } else {
-        W::load(a.add, a.x_type, at.o * a.ao + at.i * a.ai, t, dim, ad);
+        W::template load<false>(a.add, a.x_type, at.o * a.ao + at.i * a.ai, t, dim, ad);
       }
 #pragma unroll
       for (int k = 0; k < P; ++k) x[k] = add2(x[k], ad[k]);
@@ -730,7 +740,11 @@ __global__ void __launch_bounds__(1024) bwd_wide_kernel(const __grid_constant__ 
   for (int c = threadIdx.x; c < a.dim; c += 1024) {
     const float h = (at(a.x, a.x_type, xb + c) - mean) * rstd;
     float dx = rstd * (at(a.dy, a.y_type, yb + c) * weight(c) - gmean - h * gx);
-    if (a.add) dx += at(a.add, a.x_type, ab + c);
+    if (a.add) {
+      float ad;
+      load_chunk<1, false>(a.add, a.x_type, ab + c, &ad);
+      dx += ad;
+    }
     store_chunk<1>(a.out, a.x_type, ob + c, &dx);
   }
 }

@@ -57,3 +57,58 @@ def test_dx_in_the_place_of_add(dim, xt):
         a.x_dtype, a.y_dtype, a.w_dtype = CODE[xt], CODE[BF16], CODE[F32]
         call("fb_layer_norm_backward", a)
         assert torch.equal(add, want) and torch.equal(room[..., dim:], after)
+
+
+@pytest.mark.parametrize("pairs", ["interleaved", "halves"])
+@pytest.mark.parametrize("dt", [BF16, F16, F32])
+@pytest.mark.parametrize("hd,axes", [(64, (16, 24, 24)), (128, (16, 56, 56)), (10, (4, 6)), (80, (10, 30, 40))])
+def test_rope_in_place(pairs, dt, hd, axes):
+    """q and k turned where they are, inside a fused projection's rows: the bits of the turn beside them, and what else
+    the rows hold stays."""
+    from selas_b200 import _lib, ops
+
+    g = torch.Generator(device=DEV).manual_seed(51)
+    for b, l, h, kv, pad in ((1, 1, 24, 24, 0), (2, 45, 6, 2, 0), (1, 3001, 5, 1, 0), (2, 37, 3, 3, 3)):
+        width = (h + 2 * kv) * hd + pad
+        rows = randn(g, b, l, width, dtype=dt)
+        heads = rows[..., :(h + 2 * kv) * hd].unflatten(-1, (h + 2 * kv, hd))
+        q, k = heads[:, :, :h].transpose(1, 2), heads[:, :, h:h + kv].transpose(1, 2)
+        ids = torch.randint(0, 90, (l, len(axes)), generator=g, device=DEV)
+        wq, wk = ops.rope_axes_qk(q, k, ids, axes, pairs=pairs)
+        rest = rows[..., (h + kv) * hd:].clone()
+        a = _lib.FbRopeArgs()
+        for i, (t, n) in enumerate(((q, h), (k, kv))):
+            st = t.stride()[:3]
+            a.tensor[i] = _lib.FbRopeTensor(t.data_ptr(), t.data_ptr(), *st, *st, n)
+        a.ids, a.ids_stride_l, a.ids_stride_a, a.ids_type = ids.data_ptr(), len(axes), 1, _lib.FB_IDS_I64
+        a.axes_dim[:len(axes)], a.theta[:len(axes)] = axes, (10000.0,) * len(axes)
+        a.count, a.dtype, a.batch, a.seq, a.head_dim, a.axes = 2, CODE[dt], b, l, hd, len(axes)
+        a.pairs = _lib.FB_ROPE_INTERLEAVED if pairs == "interleaved" else _lib.FB_ROPE_HALVES
+        call("fb_rope_axes", a)
+        assert torch.equal(q, wq) and torch.equal(k, wk) and torch.equal(rows[..., (h + kv) * hd:], rest)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 300, 256), (28, 3072, 3072), (77, 1001, 512), (333, 1111, 1000), (2000, 640, 128), (2601, 4004, 424), (2601, 4003, 424),
+                                   (500, 1020, 8456), (500, 1019, 8456)])
+@pytest.mark.parametrize("dt", [BF16, F16])
+def test_residual_in_the_place_of_out(m, n, k, dt):
+    """The output written over the residual, with a row stride of its own, has the bits of an output of that stride beside it
+    (with another stride the bias may be added in another order)."""
+    from selas_b200 import _lib
+
+    g = torch.Generator(device=DEV).manual_seed(52)
+    x, w, b = randn(g, m, k, dtype=dt), randn(g, n, k, dtype=dt, std=k ** -0.5), randn(g, n, dtype=dt)
+    for out_type in (dt, F32):
+        for ld in (n, n + 4, n + 3):
+            room = randn(g, m, ld, dtype=out_type)
+            res, after, beside = room[:, :n], room[:, n:].clone(), torch.zeros_like(room)
+            for out in (beside, room):
+                a = _lib.FbLinearActArgs()
+                a.x, a.ldx, a.w, a.ldw, a.bias = x.data_ptr(), k, w.data_ptr(), k, b.data_ptr()
+                a.residual, a.ld_residual, a.out, a.ld_out = res.data_ptr(), ld, out.data_ptr(), ld
+                a.m, a.n, a.k = m, n, k
+                a.dtype, a.residual_dtype, a.out_dtype, a.act = CODE[dt], CODE[out_type], CODE[out_type], _lib.FB_ACT_GELU
+                call("fb_linear_act", a)
+            assert torch.equal(res, beside[:, :n]) and torch.equal(room[:, n:], after) and not beside[:, n:].any()
+            y = torch.nn.functional.gelu(x.double() @ w.double().t() + b.double())
+            assert beside[:, :n].isfinite().all() and (beside[:, :n] - y).norm() > 0.5 * y.norm()  # the residual is in it

@@ -112,3 +112,48 @@ def test_residual_in_the_place_of_out(m, n, k, dt):
             assert torch.equal(res, beside[:, :n]) and torch.equal(room[:, n:], after) and not beside[:, n:].any()
             y = torch.nn.functional.gelu(x.double() @ w.double().t() + b.double())
             assert beside[:, :n].isfinite().all() and (beside[:, :n] - y).norm() > 0.5 * y.norm()  # the residual is in it
+
+
+@pytest.mark.parametrize("dim", [8, 24, 64, 77, 128, 1000, 3072, 16388])
+@pytest.mark.parametrize("xt,wt", [(F32, BF16), (BF16, F32), (F16, F16)])
+def test_norm_with_a_weight_row_per_outer_index(dim, xt, wt):
+    """fb_layer_norm with weight and bias rows of their own per outer index (strided), as scale (1 + weight) and as weight,
+    against the formula in 64 bits: groups of threads that share a warp stand at different outer indices. Bounds as for
+    one weight: a centred value is off by 32 u mean|x| + 2 u |x|, rstd by 24 u relative, and product and sum add three
+    roundings (u = 2^-24) and the output's half step."""
+    from selas_b200 import _lib
+
+    g = torch.Generator(device=DEV).manual_seed(53)
+    u = 2.0 ** -24
+    for outer, inner in ((2, 1), (5, 7), (3, 333), (700, 3), (1, 40)):
+        if outer * inner * dim > 8_000_000:
+            continue
+        x = randn(g, outer, inner, dim, dtype=xt, mean=0.3)
+        xd = x.double()
+        c = xd - xd.mean(-1, keepdim=True)
+        rstd = 1 / torch.sqrt(c.square().mean(-1, keepdim=True) + 1e-5)
+        h = c * rstd
+        dh = u * (32 * rstd * xd.abs().mean(-1, keepdim=True) + 2 * rstd * xd.abs() + 24 * h.abs())
+        for pad in (0, 4, 3):
+            rows = randn(g, 2, outer, dim + pad, dtype=wt, std=0.3)
+            w, b = rows[0, :, :dim], rows[1, :, :dim]
+            for plus in (0, 1):
+                for has_w, has_b in ((1, 1), (1, 0), (0, 1)):
+                    for yt in (xt, BF16):
+                        out = torch.empty(outer, inner, dim, dtype=yt, device=DEV)
+                        a = _lib.FbLayerNormArgs()
+                        a.x, a.out = x.data_ptr(), out.data_ptr()
+                        a.weight, a.bias = (w.data_ptr() if has_w else None), (b.data_ptr() if has_b else None)
+                        a.x_outer_stride = a.out_outer_stride = inner * dim
+                        a.x_inner_stride = a.out_inner_stride = dim
+                        a.w_outer_stride, a.weight_plus_one = dim + pad, plus
+                        a.outer, a.inner, a.dim, a.eps = outer, inner, dim, 1e-5
+                        a.x_dtype, a.y_dtype, a.w_dtype = CODE[xt], CODE[yt], CODE[wt]
+                        call("fb_layer_norm", a)
+                        wf = (w.double() + plus)[:, None] if has_w else torch.ones(1, device=DEV).double()
+                        bf = b.double()[:, None] if has_b else 0.0 * wf
+                        ref = h * wf + bf
+                        slack = dh * wf.abs() + 3 * u * ((h * wf).abs() + bf.abs())
+                        half = ref.abs() * (torch.finfo(yt).eps / 2) + (2.0 ** -25 if yt == F16 else 0.0)
+                        worst = ((out.double() - ref).abs() / (slack * (1 + torch.finfo(yt).eps) + half + 1e-37)).max().item()
+                        assert worst <= 1.0, (outer, inner, pad, plus, has_w, has_b, yt, worst)

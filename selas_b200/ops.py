@@ -90,7 +90,7 @@ def nf4_dequant(packed: torch.Tensor, absmax: torch.Tensor, blocksize: int, code
 
 def _mod_rows(v: torch.Tensor, batch: int, dim: int) -> tuple[torch.Tensor, int]:
     """A [B, dim] (or [B, 1, dim]) bf16 view whose rows may be strided: returns (tensor, batch stride)."""
-    v = v.reshape(v.shape[0], -1) if v.dim() == 3 else v
+    v = v.flatten(1) if v.dim() == 3 else v
     _need(v.dtype == BF16, "modulation vectors must be bf16")
     _need(v.shape[-1] == dim and v.stride(-1) == 1, "modulation row must be contiguous with the model width")
     _need(v.shape[0] in (1, batch), "modulation batch does not match")

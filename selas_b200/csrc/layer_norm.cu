@@ -14,9 +14,13 @@
 // partials in a fixed order, so results do not depend on the order in which blocks run. The blocks of a call with few rows
 // are a cluster instead, and add their sums over distributed shared memory in order of rank.
 //
-// Measured: forward 18432 x 3072 fp32 to bf16 57 us (5.9 TB/s), 65537 x 768 bf16 41 us (4.9); backward 65537 x 1280 bf16
-// 95 us (5.3), 18432 x 3072 fp32 with bf16 dy 105 us (5.4), 4608 x 3072 fp32 with the adaLN scale and add 43.5 us (4.6; ten
-// rows per SM, and about 3 us to join the partials).
+// Measured on the device: forward 18432 x 3072 fp32 to bf16 56 us (6.0 TB/s), 65537 x 768 bf16 36 us (5.7); backward
+// 65537 x 1280 bf16 96 us (5.3), 18432 x 3072 fp32 with bf16 dy 103 us (5.5), 4608 x 3072 fp32 with the adaLN scale and add
+// 43 us (4.6; 31 rows per SM, ten per group of threads, and about 3 us to join the partials). Further from the copy's speed:
+// 16-bit rows above some 2000 wide, whose groups are one block per SM and stop at two barriers per row (6000 x 6144 31 us
+// forward, 75 backward: 4.8 and 3.0 TB/s); widths that are no multiple of four, loaded value by value without rows on their
+// way (20000 x 1001 bf16 29 and 56 us: 2.8 and 2.1); above 10240 the 1024 threads' registers spill (4000 x 12288 bf16 70 and
+// 129 us: 2.8 and 2.3), and above 16384 a block reads its row again for every pass (3000 x 20000 fp32 1.7 and 1.0 TB/s).
 #include <type_traits>
 
 #include "fb_internal.h"
@@ -801,7 +805,8 @@ static int elements(int dim, int gt, bool vec) { return vec ? 4 * ((dim + 4 * gt
 // saved (256 x 768 12.3 / 14.3).
 constexpr int kClusterSteps = 2;
 // Blocks per sum group of the backward pass: the SMs shared out over the groups, fewer where there are fewer rows than
-// groups of threads.
+// groups of threads. The share is a whole number, so sum groups (images) of 75 to 147 get a block each and leave SMs idle
+// (fp32 3072 wide, 64 rows an image: 80 images 55 us, 147 images 57), and 50 to 74 get two (74 images 82 us).
 struct Blocks {
   int64_t n;
   bool cluster;
@@ -863,7 +868,7 @@ static cudaError_t go_bwd(Args a, int64_t sum_groups, cudaStream_t st) {
   }
   cudaError_t e = cudaLaunchKernelEx(&cfg, bwd_kernel<GT, NCH, CH, FULL>, a);
   if (e == cudaSuccess && a.dw != nullptr && blocks.n > 1 && !a.cluster) {
-    // launched while the last blocks of the walk still run; it waits for them before it reads
+    // launched without a gap when the last block of the walk ends; it waits for their writes before it reads
     cfg.gridDim = dim3(static_cast<unsigned>((2ll * a.dim + 31) / 32), static_cast<unsigned>(sum_groups));
     cfg.blockDim = dim3(1024);
     cfg.dynamicSmemBytes = 0;

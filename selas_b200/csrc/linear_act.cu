@@ -15,14 +15,16 @@
 //    always gives the same bits).
 //  * many_kernel, for the rest: 256 tokens x 256 features per CTA pair (tcgen05.mma.cta_group::2), persistent over tiles.
 //
-// Precision: the tensor core adds into its accumulator with less care than an fp32 add (over K = 12288 the error grew to
-// 1.3e-5 of the result's norm), so an accumulator takes 1024 of K at most; the epilogue warps then add it to fp32
-// registers, which are the sum proper, while the other TMEM buffer takes the next 1024. That costs 2 % of the time at
-// most (every 512 cost 10 %) and holds the error of an fp32 output near 1e-6.
+// Precision: the tensor core adds into its accumulator with less care than an fp32 add, it truncates (over K = 12288 the
+// error grew to 1.4e-5 of the result's norm), so an accumulator takes 1024 of K at most; the epilogue warps then add it to
+// fp32 registers, which are the sum proper, while the other TMEM buffer takes the next 1024. That costs 2 % of the time at
+// most (every 512 cost 10 %) and holds the error of an fp32 output at 1.0e-6 (bf16) and 1.25e-6 (fp16) of its norm for any
+// K (4608 x 12288 x 3072 onto its fp32 residual: 6.7e-7, elementary fp32 operations 8.3e-7). Within 1024 of K the
+// accumulator's truncation is what there is.
 //
-// Measured: 28 x 3072 x 18432 (m x k x n) 24.6 us, 4.6 TB/s of weight, which a kernel that only loads the weight by TMA
-// also takes; 4608 x 12288 x 3072 onto an fp32 residual 231 us, 1505 TFLOP/s, in a single call and 243 to 290 us back to
-// back under the power cap; 512 x 12288 x 3072 49 us; one row, 256 to 3072 features, 6.3 us.
+// Measured on the device: 28 x 3072 x 18432 (m x k x n) 24.6 us, 4.6 TB/s of weight, which a kernel that only loads the
+// weight by TMA also takes; 4608 x 12288 x 3072 onto an fp32 residual 231 us, 1505 TFLOP/s, in a single call and 243 to 290
+// us back to back under the power cap; 512 x 12288 x 3072 49 us; one row, 256 to 3072 features, 4.8 us back to back.
 #include <atomic>
 #include <type_traits>
 
@@ -52,9 +54,12 @@ struct Args {
 // epilogue outgrew the instruction caches (a 256 x 256 tile took 80 us).
 //
 // The erf of GELU is Abramowitz and Stegun's 7.1.26 for erfc(|x|), x = z / sqrt 2, off by at most 1.5e-7: y = z h for
-// z < 0 and z - z h otherwise, h = erfc(|x|) / 2, which keeps the small values of the negative side. With CUDA's erff the
-// epilogue of a 256 x 256 tile at K = 3072 took longer than its products. The sigmoids divide by 1 + exp with the
-// hardware's exp2 and division (2 ulp); tanh(u) = 2 sigmoid(2u) - 1.
+// z < 0 and z - z h otherwise, h = erfc(|x|) / 2. A value is off by 3.4e-7 at most, of standard normal inputs 8.4e-8 of the
+// norm (6.1e-8 with an fp32 erf), which only an fp32 output shows. Small negative values keep their size, unlike those of
+// 1 + erf in fp32, but not every bit: off by 5e-5 of themselves at z = -3 (1 + erf: 1.4e-6), 5e-4 at -4 (3e-4), 4e-3 at -6
+// and 2 % at -10 (all). With CUDA's erff the epilogue of a 256 x 256 tile at K = 3072 took longer than its products. The
+// sigmoids divide by 1 + exp with the hardware's exp2 and division, (2 + 1.2 |z|) 2^-23 and 2^-22 relative, for the same
+// reason; tanh(u) = 2 sigmoid(2u) - 1.
 __device__ __forceinline__ float rcp_approx(float x) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));

@@ -391,6 +391,8 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, o
 # These take tensors on any device of the process: the launch goes to the current stream of the tensors' device. The
 # smallest calls take a few microseconds on the GPU, less than a wrapper spends on setting a ctypes.Structure's fields or
 # asking for a Stream object, so the arguments are packed in one go (_lib.packer) and the stream is read as its handle.
+# Nothing is registered with autograd: a result has no history, also where an input requires a gradient, and the gradients are
+# calls of their own.
 _IDS_CODE = {torch.float32: _lib.FB_IDS_F32, torch.float64: _lib.FB_IDS_F64, torch.int32: _lib.FB_IDS_I32,
              torch.int64: _lib.FB_IDS_I64}
 _PAIRS = {"interleaved": _lib.FB_ROPE_INTERLEAVED, "halves": _lib.FB_ROPE_HALVES}
@@ -562,9 +564,9 @@ def _norm_vector(what: str, name: str, d: int, t: torch.Tensor) -> tuple[int, in
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5,
                *, out_dtype: torch.dtype | None = None) -> torch.Tensor:
-    """(x - mean) / sqrt(var + eps) * weight + bias over the last dim of x [..., D] (fp32, bf16 or fp16; rows of up
-    to three dims may be strided, a tensor of more is contiguous), statistics in fp32, rounded once to ``out_dtype`` (x's by default). weight and bias: [D] of one type, or
-    None. Returns a contiguous tensor."""
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last dim of x [..., D] (fp32, bf16 or fp16; rows of up to three
+    dims may be strided, a tensor of more is contiguous), statistics in fp32, rounded once to ``out_dtype`` (x's by
+    default). weight and bias: [D] of one type, or None. Returns a contiguous tensor."""
     index = _one_device("layer_norm", x, weight, bias)
     outer, inner, d, code = _norm_rows("layer_norm", x)
     w = b = w_code = 0
@@ -638,8 +640,8 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor 
     """The gradients of ``layer_norm`` for the gradient dy of its output: (dx, dweight, dbias). x is what the forward
     took (its statistics are computed again, nothing has to be saved); dy fp32, bf16 or fp16 of x's shape. ``add`` (x's
     type and shape) is added to dx before its one rounding: the gradient that reaches x past the norm, as in a residual
-    stream. dx has x's type; dweight = sum of dy * xhat and dbias = sum of dy are fp32 [D], summed in a fixed order;
-    ``sums=False`` leaves them out (None)."""
+    stream. dx has x's type; dweight = sum of dy * xhat and dbias = sum of dy are fp32 [D], summed in a fixed order, each with
+    storage of its own; ``sums=False`` leaves them out (None)."""
     index = _one_device("layer_norm_backward", x, dy, weight, add)
     w = w_code = 0
     if weight is not None:

@@ -109,11 +109,16 @@ DeviceState* device_for(Operator op, std::string& err) {
   std::lock_guard<std::mutex> lock(g_dev_mu);
   if (ready.load(std::memory_order_relaxed)) return s;
   // The first call may be one that a stream captures. Set-up enqueues nothing, but loads kernels, which a capture in its
-  // default mode may forbid this thread.
-  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-  cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
-  if (e != cudaSuccess) {
-    err = std::string("cudaThreadExchangeStreamCaptureMode: ") + cudaGetErrorString(e);
+  // default mode may forbid this thread. The caller's mode comes back also if set-up runs out of host memory.
+  struct Relaxed {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    const cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+    ~Relaxed() {
+      if (e == cudaSuccess) cudaThreadExchangeStreamCaptureMode(&mode);
+    }
+  } relaxed;
+  if (relaxed.e != cudaSuccess) {
+    err = std::string("cudaThreadExchangeStreamCaptureMode: ") + cudaGetErrorString(relaxed.e);
     return nullptr;
   }
   std::string msg;
@@ -122,7 +127,6 @@ DeviceState* device_for(Operator op, std::string& err) {
     case Operator::kLayerNorm: msg = layer_norm_setup(); break;
     default: msg = rope_axes_setup(); break;
   }
-  cudaThreadExchangeStreamCaptureMode(&mode);
   if (!msg.empty()) {
     err = msg;
     return nullptr;

@@ -43,12 +43,15 @@ void __cudaRegisterFunction(void**, const char*, char*, const char*, int, void*,
 
 SETUPS = r"""
 #include <cstdio>
+#include <new>
 #include "CSRC/fb_internal.h"
 
 extern int device, mode;
 static int ran[5] = {}, broken[5] = {};
+static bool throws = false;
 static std::string run(int i) {
   ++ran[i];
+  if (throws) throw std::bad_alloc();
   if (i >= 2 && mode != cudaStreamCaptureModeRelaxed) return "set-up without a relaxed capture mode";
   return broken[i] ? "broken set-up " + std::to_string(i) : std::string();
 }
@@ -85,6 +88,15 @@ int main() {
   CHECK(fb::device_for(Operator::kRopeAxes, err) == d && ran[4] == 1 && mode == cudaStreamCaptureModeGlobal);
   device = 1;  // each device by itself
   CHECK(fb::device_for(Operator::kLayerNorm, err) != d && ran[3] == 2 && ran[0] == 2 && ran[4] == 1);
+  throws = true;
+  bool thrown = false;
+  try {
+    fb::device_for(Operator::kRopeAxes, err);
+  } catch (const std::bad_alloc&) {
+    thrown = true;
+  }
+  CHECK(thrown && mode == cudaStreamCaptureModeGlobal);
+  throws = false;
   broken[2] = 0;
   CHECK(fb::device_for(Operator::kLinearAct, err));
   return 0;

@@ -17,8 +17,8 @@
 // Measured on the device: forward 18432 x 3072 fp32 to bf16 56 us (6.0 TB/s), 65537 x 768 bf16 36 us (5.7); backward
 // 65537 x 1280 bf16 96 us (5.3), 18432 x 3072 fp32 with bf16 dy 103 us (5.5), 4608 x 3072 fp32 with the adaLN scale and add
 // 43 us (4.6; 31 rows per SM, ten per group of threads, and about 3 us to join the partials). Further from the copy's speed:
-// 16-bit rows above some 2000 wide, whose groups are one block per SM and stop at two barriers per row (6000 x 6144 31 us
-// forward, 75 backward: 4.8 and 3.0 TB/s); widths that are no multiple of four, loaded value by value without rows on their
+// 16-bit rows above some 2000 wide, whose few groups per SM stop at two barriers per row (6000 x 6144 31 us forward, 75
+// backward: 4.8 and 3.0 TB/s); widths that are no multiple of four, loaded value by value without rows on their
 // way (20000 x 1001 bf16 29 and 56 us: 2.8 and 2.1); above 10240 the 1024 threads' registers spill (4000 x 12288 bf16 70 and
 // 129 us: 2.8 and 2.3), and above 16384 a block reads its row again for every pass (3000 x 20000 fp32 1.7 and 1.0 TB/s).
 #include <type_traits>

@@ -74,7 +74,8 @@ template <int ACT>
 __device__ __forceinline__ float activate(float z) {
   if constexpr (ACT == FB_ACT_RELU) return z < 0.f ? 0.f : z;  // keeps a NaN
   if constexpr (ACT == FB_ACT_GELU) {
-    // |z|, up to 30 where z > 0: nothing is left of erfc there, and +inf * 0 stays out. -inf gives NaN as z/2 * (1 + erf) does.
+    // |z|, up to 30 where z > 0: nothing is left of erfc there, and +inf * 0 stays out. -inf gives NaN as z/2 * (1 + erf) does
+    // (a clamp of |z| would give 0; 8192 x 512 x 4096, bound by the epilogue, 71.6 us with that, 72.8 with this).
     const float s = fmaxf(-z, fminf(z, 30.f));
     const float t = rcp_approx(fmaf(0.3275911f * 0.70710678f, s, 1.0f));
     float h = fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
@@ -829,6 +830,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const __grid_constant
       }
     }
   }
+  __syncwarp();
   tc_fence_before_sync();
   __syncthreads();
   cluster_sync_all();  // the peer no longer signals this CTA; nobody reads this CTA's TMEM, or its partial sums
